@@ -264,6 +264,98 @@ int n550_attention_decode(void *stream, const uint16_t *q, int ldq, const uint16
                           int ldo, void *workspace, size_t workspace_bytes);
 size_t n550_attention_decode_workspace(int n_seqs, int max_len);
 
+/* ---------------------------------------------------------------------------
+ * The 8-bit KV cache: K and V of the BF16 cache's planes as e4m3 codes with an
+ * FP32 scale for each block of N550_KV8_BLOCK positions and KV head, half the
+ * bytes a decode step reads. The caller owns the memory (device pointers):
+ *   k, v              [n_slots][n_layers][8 kv heads][max_len][128] codes
+ *   k_scale, v_scale  [n_slots][n_layers][8][n_blocks] powers of two,
+ *                     n_blocks = ceil(max_len / N550_KV8_BLOCK)
+ *   k_bounds          [n_slots][n_layers][8][n_blocks][2][128] codes: the smallest
+ *                     and the largest K code of the block in each channel
+ *                     (NULL: not kept; n550_kv8_select_blocks needs them)
+ * A value is its code times its block's scale, which BF16 holds exactly. k, v
+ * and k_bounds are 16-byte aligned. Nothing needs to be initialised:
+ * n550_kv8_append defines what later calls read. max_len need not be a multiple
+ * of the block.
+ *
+ * seq_ids and pos are device int32 arrays, as for the BF16 cache. A slot id
+ * outside the cache or a negative position makes a sequence empty: append
+ * skips its rows, the attentions write zero rows for it and the selection -1. A
+ * query position past the cache's end reads the whole slot. Row pointers (k, v,
+ * q, out) are 16-byte aligned and row strides a multiple of 16 bytes, else
+ * N550_ERR_ARG. A slot may be read by several sequences of one call, but be
+ * appended to by one. No counterpart in the reference (FP32 cache).
+ * ------------------------------------------------------------------------- */
+#define N550_KV8_BLOCK 64
+typedef struct {
+    uint8_t *k, *v;
+    float   *k_scale, *v_scale;
+    uint8_t *k_bounds;
+    int      n_slots, n_layers, max_len;
+} n550_kv8_cache;
+
+/* Quantises n_seqs x L rows of K and V (type N550_F32 or N550_BF16, after
+ * QK-norm and RoPE; rows [n_seqs * L][ld >= 1024], KV head h at columns h*128)
+ * into positions pos[s] .. pos[s]+L-1 of slot seq_ids[s]. Each touched block takes
+ * the smallest power of two s with |x| <= 448 s for its new rows (2^-126 at
+ * least); a block that already holds positions below pos[s] keeps its scale if
+ * that is larger, and if not its held codes are rounded anew at the larger one.
+ * Codes are rounded to nearest even; an infinity becomes the largest code and
+ * does not count for the scale; a NaN stays NaN and counts as 0 in the bounds.
+ * Positions from pos[s]+L on keep their codes. The positions below pos[s] of its
+ * block must have been appended (in any number of calls). A sequence whose
+ * range leaves the cache is skipped whole. Appending at a lower position than before (after
+ * rejected drafts, or a slot used anew from position 0) is allowed: a block
+ * kept in part keeps its scale and bounds, which then may be wider than its
+ * codes. */
+int n550_kv8_append(void *stream, const n550_kv8_cache *c, int layer, const void *k, const void *v,
+                    int type, int ld, const int32_t *seq_ids, const int32_t *pos, int n_seqs, int L);
+
+/* n550_attention_decode over the 8-bit cache: one query per sequence at
+ * position pos[s], q [n_seqs][ldq >= 2048] BF16, out [n_seqs][ldo >= 2048] BF16.
+ * workspace may be NULL (one CTA per sequence and KV head) or
+ * n550_attention_kv8_workspace(n_seqs) bytes, 16-byte aligned, not shared by calls
+ * that can overlap; its contents before and after a call mean nothing. */
+int n550_attention_decode_kv8(void *stream, const uint16_t *q, int ldq, const n550_kv8_cache *c,
+                              int layer, const int32_t *seq_ids, const int32_t *pos, int n_seqs,
+                              uint16_t *out, int ldo, void *workspace, size_t workspace_bytes);
+size_t n550_attention_kv8_workspace(int n_seqs);
+
+/* n550_attention_prefill over the 8-bit cache: n_seqs x L queries at positions
+ * pos0 .. pos0+L-1 whose K/V were appended, causal; q and out [n_seqs*L] rows.
+ * workspace may be NULL (slower) or
+ * n550_attention_prefill_kv8_workspace(n_seqs, L, pos0) bytes, as above. */
+int n550_attention_prefill_kv8(void *stream, const uint16_t *q, int ldq, const n550_kv8_cache *c,
+                               int layer, const int32_t *seq_ids, int n_seqs, int L, int pos0,
+                               uint16_t *out, int ldo, void *workspace, size_t workspace_bytes);
+size_t n550_attention_prefill_kv8_workspace(int n_seqs, int L, int pos0);
+
+/* The n_select blocks of each sequence's context (positions 0..pos[s]) whose
+ * bounds promise the largest scores for its query, per KV head:
+ *   score_b = s_b * max over the KV head's two query heads of
+ *             sum_d max(q_d lo_bd, q_d hi_bd),
+ * which no q . k_t of the block exceeds. The first n_sink and the last n_recent
+ * blocks of the context are always among them (n_sink + n_recent <= n_select;
+ * the block of position pos[s] is the last one); then the largest scores, the
+ * lower index first among equals (a NaN score ranks last). blocks
+ * [n_seqs][8][n_select] int32 receives the indices in ascending order and -1
+ * behind them when the context has fewer blocks. Caches of more than
+ * N550_KV8_SELECT_MAX_BLOCKS blocks: N550_ERR_UNSUPPORTED. */
+#define N550_KV8_SELECT_MAX_BLOCKS 24576
+int n550_kv8_select_blocks(void *stream, const uint16_t *q, int ldq, const n550_kv8_cache *c, int layer,
+                           const int32_t *seq_ids, const int32_t *pos, int n_seqs, int n_select,
+                           int n_sink, int n_recent, int32_t *blocks);
+
+/* n550_attention_decode_kv8 over listed blocks only: sequence s and KV head h
+ * attend to those positions <= pos[s] that lie in the blocks blocks[s][h][0 ..
+ * n_select). Entries that are negative or past the context are skipped; a block
+ * listed twice counts twice; with no position left the rows are zero. */
+int n550_attention_sparse_kv8(void *stream, const uint16_t *q, int ldq, const n550_kv8_cache *c,
+                              int layer, const int32_t *seq_ids, const int32_t *pos,
+                              const int32_t *blocks, int n_select, int n_seqs, uint16_t *out, int ldo,
+                              void *workspace, size_t workspace_bytes);
+
 /* Device status word written by bounded waits inside kernels; returns it and
  * clears it (N550_OK, or N550_ERR_TIMEOUT). Synchronises the device. */
 int n550_device_status(void);

@@ -17,6 +17,8 @@ HEADER = PKG.parent / "include" / "n550_qwen3.h"
 
 # Status codes (include/n550_qwen3.h)
 OK = 0
+KV8_BLOCK = 64                 # N550_KV8_BLOCK
+KV8_SELECT_MAX_BLOCKS = 24576  # N550_KV8_SELECT_MAX_BLOCKS
 ERR_MAGIC, ERR_VERSION, ERR_DTYPE, ERR_SHAPE, ERR_SIZE, ERR_OOM, ERR_LAYOUT = -1, -2, -3, -4, -5, -6, -7
 ERR_ARG, ERR_CUDA, ERR_UNSUPPORTED, ERR_TIMEOUT = -101, -102, -103, -104
 MODE_EXACT, MODE_FAST = 0, 1
@@ -35,6 +37,13 @@ class N550Error(RuntimeError):
 
 class SpecStats(C.Structure):
     _fields_ = [("rounds", C.c_int64), ("drafted", C.c_int64), ("accepted", C.c_int64)]
+
+
+class KV8CacheStruct(C.Structure):
+    """n550_kv8_cache."""
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("k_scale", C.c_void_p),
+                ("v_scale", C.c_void_p), ("k_bounds", C.c_void_p), ("n_slots", C.c_int),
+                ("n_layers", C.c_int), ("max_len", C.c_int)]
 
 
 class ModelConfig(C.Structure):
@@ -90,6 +99,13 @@ def lib() -> C.CDLL:
         "n550_attention_decode": (i, [vp, vp, i, vp, vp, i, i, i, vp, vp, i, vp, i, vp, sz]),
         "n550_attention_decode_workspace": (sz, [i, i]),
         "n550_rope_table": (i, [vp, vp, i]),
+        "n550_kv8_append": (i, [vp, vp, i, vp, vp, i, i, vp, vp, i, i]),
+        "n550_attention_decode_kv8": (i, [vp, vp, i, vp, i, vp, vp, i, vp, i, vp, sz]),
+        "n550_attention_kv8_workspace": (sz, [i]),
+        "n550_attention_prefill_kv8": (i, [vp, vp, i, vp, i, vp, i, i, i, vp, i, vp, sz]),
+        "n550_attention_prefill_kv8_workspace": (sz, [i, i, i]),
+        "n550_kv8_select_blocks": (i, [vp, vp, i, vp, i, vp, vp, i, i, i, i, vp]),
+        "n550_attention_sparse_kv8": (i, [vp, vp, i, vp, i, vp, vp, vp, i, i, vp, i, vp, sz]),
         "n550_qkv_rope_kv": (i, [vp, vp, i, vp, vp, vp, vp, vp, vp, i, vp, i, i, vp, vp, i, i]),
     }
     optional = {
@@ -184,5 +200,7 @@ def set_gemm_mode(mode: int, kblock: int = 16) -> None:
 
 
 from .api import *  # noqa: E402,F401,F403
+from .kv8 import (KV8Cache, attention_decode_kv8, attention_prefill_kv8,  # noqa: E402,F401
+                  attention_sparse_kv8, kv8_append, kv8_select_blocks)
 from .model import Model  # noqa: E402,F401
 from .tokenizer import Tokenizer  # noqa: E402,F401

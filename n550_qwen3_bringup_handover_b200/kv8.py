@@ -1,0 +1,185 @@
+"""The 8-bit KV cache over torch CUDA tensors: quantising append, attention over
+it, block selection and sparse attention (n550_kv8_*, n550_attention_*_kv8)."""
+from __future__ import annotations
+
+import ctypes as C
+
+from . import BF16, F32, KV8_BLOCK, KV8CacheStruct, check, lib
+
+_LAYERS, _NKV, _HD, _NH = 28, 8, 128, 16
+
+
+def _on_current(*tensors):
+    """The current CUDA device's stream; the tensors must live on that device."""
+    import torch
+    dev = torch.cuda.current_device()
+    for t in tensors:
+        if t.device.type != "cuda" or t.device.index != dev:
+            raise ValueError(f"tensor on {t.device}, but the current CUDA device is cuda:{dev}")
+    return torch.cuda.current_stream().cuda_stream
+
+
+class KV8Cache:
+    """K and V of n_slots sequences as e4m3 codes with a scale per block of 64
+    positions and KV head (n550_kv8_cache). Tensors: k, v [n_slots, n_layers, 8,
+    max_len, 128] float8_e4m3fn, k_scale, v_scale [n_slots, n_layers, 8, n_blocks]
+    float32, k_bounds [n_slots, n_layers, 8, n_blocks, 2, 128] float8_e4m3fn or
+    None. Allocated here, or handed over by keyword."""
+
+    def __init__(self, n_slots=None, max_len=None, n_layers=_LAYERS, device="cuda", bounds=True, *,
+                 k=None, v=None, k_scale=None, v_scale=None, k_bounds=None):
+        import torch
+        e4 = torch.float8_e4m3fn
+        given = [k, v, k_scale, v_scale]
+        if all(t is None for t in given) and k_bounds is None:
+            if n_slots is None or max_len is None or min(n_slots, max_len, n_layers) < 1:
+                raise ValueError("n_slots, max_len and n_layers must be at least 1")
+            nb = -(-max_len // KV8_BLOCK)
+            plane = (n_slots, n_layers, _NKV)
+            k = torch.empty(plane + (max_len, _HD), dtype=e4, device=device)
+            v = torch.empty_like(k)
+            k_scale = torch.empty(plane + (nb,), dtype=torch.float32, device=device)
+            v_scale = torch.empty_like(k_scale)
+            if bounds:
+                k_bounds = torch.empty(plane + (nb, 2, _HD), dtype=e4, device=device)
+        elif any(t is None for t in given):
+            raise ValueError("k, v, k_scale and v_scale belong together")
+        if k.dim() != 5 or k.shape[2] != _NKV or k.shape[4] != _HD:
+            raise ValueError("KV cache must be [slots, layers, 8, max_len, 128]")
+        nb = -(-k.shape[3] // KV8_BLOCK)
+        plane = tuple(k.shape[:3])
+        want = {"k": (k, tuple(k.shape), e4), "v": (v, tuple(k.shape), e4),
+                "k_scale": (k_scale, plane + (nb,), torch.float32),
+                "v_scale": (v_scale, plane + (nb,), torch.float32),
+                "k_bounds": (k_bounds, plane + (nb, 2, _HD), e4)}
+        for name, (t, shape, dt) in want.items():
+            if t is None and name == "k_bounds":
+                continue
+            if tuple(t.shape) != shape or t.dtype != dt or not t.is_contiguous():
+                raise ValueError(f"{name} must be a contiguous {dt} tensor of shape {shape}")
+            if t.device.type != "cuda" or t.device != k.device:
+                raise ValueError("the cache's tensors must be on one CUDA device")
+        self.k, self.v, self.k_scale, self.v_scale, self.k_bounds = k, v, k_scale, v_scale, k_bounds
+        self.n_slots, self.n_layers, self.max_len, self.n_blocks = k.shape[0], k.shape[1], k.shape[3], nb
+        self._c = KV8CacheStruct(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
+                                 k_bounds.data_ptr() if k_bounds is not None else None,
+                                 self.n_slots, self.n_layers, self.max_len)
+        self._ref = C.byref(self._c)
+
+
+def _ids(name, t, n=None):
+    import torch
+    if t.dtype != torch.int32 or t.dim() != 1 or not t.is_contiguous() or (n is not None and t.numel() != n):
+        raise ValueError(f"{name} must be a contiguous int32 vector" + (f" of {n}" if n is not None else ""))
+    return t.numel()
+
+
+def _rows(name, t, rows, cols, dtypes):
+    if t.dim() != 2 or t.shape[0] != rows or t.shape[1] < cols or t.dtype not in dtypes or \
+            (t.stride(1) != 1 and rows > 0):
+        raise ValueError(f"{name} must be [{rows}, >= {cols}] with contiguous rows of {dtypes}")
+    # the stride of a single row is never used; torch reports any number there
+    return t.stride(0) if rows > 1 else t.shape[1]
+
+
+def kv8_append(cache, k, v, seq_ids, pos, L, layer):
+    """Quantise len(seq_ids) x L rows of k and v ([n_seqs*L, >= 1024] float32 or
+    bfloat16) into positions pos[s] .. pos[s]+L-1 of slot seq_ids[s]."""
+    import torch
+    st = _on_current(cache.k, k, v, seq_ids, pos)
+    n = _ids("seq_ids", seq_ids)
+    _ids("pos", pos, n)
+    if L < 0:
+        raise ValueError("L must not be negative")
+    ld = _rows("k", k, n * L, _NKV * _HD, (torch.float32, torch.bfloat16))
+    if _rows("v", v, n * L, _NKV * _HD, (k.dtype,)) != ld:
+        raise ValueError("k and v must have the same row stride")
+    check(lib().n550_kv8_append(st, cache._ref, layer, k.data_ptr(), v.data_ptr(),
+                                F32 if k.dtype == torch.float32 else BF16, ld, seq_ids.data_ptr(),
+                                pos.data_ptr(), n, L), "n550_kv8_append")
+
+
+def _q_out(q, rows, out):
+    import torch
+    ldq = _rows("q", q, rows, _NH * _HD, (torch.bfloat16,))
+    if out is None:
+        out = torch.empty((rows, _NH * _HD), dtype=torch.bfloat16, device=q.device)
+    return ldq, out, _rows("out", out, rows, _NH * _HD, (torch.bfloat16,))
+
+
+def _workspace(nbytes, device):
+    import torch
+    return torch.empty(max(nbytes, 16), dtype=torch.uint8, device=device)
+
+
+def attention_decode_kv8(q, cache, seq_ids, pos, layer, out=None, split=True):
+    """One query per sequence (rows of q, BF16) at position pos[s] over the 8-bit
+    cache; split=True passes a split-KV workspace, split=False runs one CTA per
+    (sequence, KV head)."""
+    n = _ids("seq_ids", seq_ids)
+    _ids("pos", pos, n)
+    ldq, out, ldo = _q_out(q, n, out)
+    st = _on_current(cache.k, q, seq_ids, pos, out)
+    L = lib()
+    nbytes = L.n550_attention_kv8_workspace(n) if split else 0
+    ws = _workspace(nbytes, q.device).data_ptr() if nbytes else None
+    check(L.n550_attention_decode_kv8(st, q.data_ptr(), ldq, cache._ref, layer, seq_ids.data_ptr(),
+                                      pos.data_ptr(), n, out.data_ptr(), ldo, ws, nbytes),
+          "n550_attention_decode_kv8")
+    return out
+
+
+def attention_sparse_kv8(q, cache, seq_ids, pos, blocks, layer, out=None, split=True):
+    """attention_decode_kv8 over the positions <= pos[s] of the listed blocks only:
+    blocks int32 [n_seqs, 8, n_select], entries outside the context skipped."""
+    import torch
+    n = _ids("seq_ids", seq_ids)
+    _ids("pos", pos, n)
+    if blocks.dtype != torch.int32 or blocks.dim() != 3 or tuple(blocks.shape[:2]) != (n, _NKV) or \
+            not blocks.is_contiguous():
+        raise ValueError(f"blocks must be a contiguous int32 tensor [{n}, 8, n_select]")
+    ldq, out, ldo = _q_out(q, n, out)
+    st = _on_current(cache.k, q, seq_ids, pos, blocks, out)
+    L = lib()
+    nbytes = L.n550_attention_kv8_workspace(n) if split else 0
+    ws = _workspace(nbytes, q.device).data_ptr() if nbytes else None
+    check(L.n550_attention_sparse_kv8(st, q.data_ptr(), ldq, cache._ref, layer, seq_ids.data_ptr(),
+                                      pos.data_ptr(), blocks.data_ptr(), blocks.shape[2], n,
+                                      out.data_ptr(), ldo, ws, nbytes), "n550_attention_sparse_kv8")
+    return out
+
+
+def attention_prefill_kv8(q, cache, seq_ids, L, pos0, layer, out=None, workspace=True):
+    """Causal attention of len(seq_ids) sequences x L queries (rows of q, BF16) at
+    positions pos0.. over the 8-bit cache, which holds their K/V already."""
+    n = _ids("seq_ids", seq_ids)
+    if L < 0:
+        raise ValueError("L must not be negative")
+    ldq, out, ldo = _q_out(q, n * L, out)
+    st = _on_current(cache.k, q, seq_ids, out)
+    lb = lib()
+    nbytes = lb.n550_attention_prefill_kv8_workspace(n, L, pos0) if workspace else 0
+    ws = _workspace(nbytes, q.device).data_ptr() if nbytes else None
+    check(lb.n550_attention_prefill_kv8(st, q.data_ptr(), ldq, cache._ref, layer, seq_ids.data_ptr(), n,
+                                        L, pos0, out.data_ptr(), ldo, ws, nbytes),
+          "n550_attention_prefill_kv8")
+    return out
+
+
+def kv8_select_blocks(q, cache, seq_ids, pos, layer, n_select, n_sink=1, n_recent=2, out=None):
+    """The n_select blocks of each context whose bounds promise the largest scores
+    for the sequence's query, per KV head: int32 [n_seqs, 8, n_select], ascending,
+    -1 behind the last."""
+    import torch
+    n = _ids("seq_ids", seq_ids)
+    _ids("pos", pos, n)
+    ldq = _rows("q", q, n, _NH * _HD, (torch.bfloat16,))
+    if out is None:
+        out = torch.empty((n, _NKV, max(n_select, 0)), dtype=torch.int32, device=q.device)
+    elif tuple(out.shape) != (n, _NKV, n_select) or out.dtype != torch.int32 or not out.is_contiguous():
+        raise ValueError(f"out must be a contiguous int32 tensor [{n}, 8, {n_select}]")
+    st = _on_current(cache.k, q, seq_ids, pos, out)
+    check(lib().n550_kv8_select_blocks(st, q.data_ptr(), ldq, cache._ref, layer, seq_ids.data_ptr(),
+                                       pos.data_ptr(), n, n_select, n_sink, n_recent, out.data_ptr()),
+          "n550_kv8_select_blocks")
+    return out

@@ -1,0 +1,108 @@
+"""The 8-bit KV cache without a GPU: argument checks of its entry points, which
+run before any CUDA call, and the oracle's own e4m3 rounding."""
+import ctypes as C
+
+import pytest
+import torch
+
+import n550_qwen3_bringup_handover_b200 as n5
+from kv8_oracle import POS, round_codes, scale_for, values
+
+
+def struct(**kw):
+    c = dict(k=4096, v=8192, k_scale=4096, v_scale=4096, k_bounds=4096, n_slots=2, n_layers=3, max_len=100)
+    c.update(kw)
+    return n5.KV8CacheStruct(*[c[f] for f, _ in n5.KV8CacheStruct._fields_])
+
+
+P = 4096      # a well aligned address that is never read: every call below is refused first
+
+
+def calls(L, cache, layer=0, ptr=P, ld=2048, n=1, rows=4):
+    """Every entry point with otherwise good arguments."""
+    r = C.byref(cache) if cache is not None else None
+    return {
+        "append": L.n550_kv8_append(None, r, layer, ptr, ptr, n5.BF16, ld, P, P, n, rows),
+        "decode": L.n550_attention_decode_kv8(None, ptr, ld, r, layer, P, P, n, ptr, ld, None, 0),
+        "sparse": L.n550_attention_sparse_kv8(None, ptr, ld, r, layer, P, P, P, 2, n, ptr, ld, None, 0),
+        "prefill": L.n550_attention_prefill_kv8(None, ptr, ld, r, layer, P, n, rows, 0, ptr, ld, None, 0),
+        "select": L.n550_kv8_select_blocks(None, ptr, ld, r, layer, P, P, n, 4, 1, 1, P),
+    }
+
+
+@pytest.mark.parametrize("bad", [
+    dict(k=None), dict(v=None), dict(k_scale=None), dict(v_scale=None), dict(k=4104), dict(v=4097),
+    dict(k_bounds=4100), dict(k_scale=4098), dict(n_slots=0), dict(n_layers=0), dict(max_len=0), dict(max_len=-5),
+    dict(n_slots=1 << 20, n_layers=1 << 10),
+])
+def test_bad_caches_are_refused(bad):
+    for name, rc in calls(n5.lib(), struct(**bad)).items():
+        assert rc == n5.ERR_ARG, name
+
+
+def test_bad_calls_are_refused():
+    L = n5.lib()
+    for kw in [dict(cache=None), dict(cache=struct(), layer=3), dict(cache=struct(), layer=-1),
+               dict(cache=struct(), ptr=None), dict(cache=struct(), ptr=P + 8), dict(cache=struct(), ld=1000),
+               dict(cache=struct(), ld=2052), dict(cache=struct(), n=-1), dict(cache=struct(), n=65536)]:
+        for name, rc in calls(L, **kw).items():
+            assert rc == n5.ERR_ARG, (name, kw)
+    c = C.byref(struct())
+    # append: element type, negative and too many rows
+    assert L.n550_kv8_append(None, c, 0, P, P, 7, 1024, P, P, 1, 1) == n5.ERR_ARG
+    assert L.n550_kv8_append(None, c, 0, P, P, n5.F32, 1024, P, P, 1, -1) == n5.ERR_ARG
+    assert L.n550_kv8_append(None, c, 0, P, P, n5.F32, 1024, P, P, 1, 101) == n5.ERR_ARG
+    # prefill: positions outside the cache
+    assert L.n550_attention_prefill_kv8(None, P, 2048, c, 0, P, 1, 4, 97, P, 2048, None, 0) == n5.ERR_ARG
+    assert L.n550_attention_prefill_kv8(None, P, 2048, c, 0, P, 1, 4, -1, P, 2048, None, 0) == n5.ERR_ARG
+    assert L.n550_attention_prefill_kv8(None, P, 2048, c, 0, P, 1, 4, 2147483647, P, 2048, None, 0) == n5.ERR_ARG
+    # sparse: a negative list length
+    assert L.n550_attention_sparse_kv8(None, P, 2048, c, 0, P, P, P, -1, 1, P, 2048, None, 0) == n5.ERR_ARG
+    # select: counts, a cache without bounds, too long a cache
+    for n_select, sink, recent in [(0, 0, 0), (4, 3, 2), (4, -1, 2), (4, 1, -1), (4, 2147483647, 2147483647)]:
+        assert L.n550_kv8_select_blocks(None, P, 2048, c, 0, P, P, 1, n_select, sink, recent, P) == n5.ERR_ARG
+    nob = C.byref(struct(k_bounds=None))
+    assert L.n550_kv8_select_blocks(None, P, 2048, nob, 0, P, P, 1, 4, 1, 1, P) == n5.ERR_ARG
+    long = C.byref(struct(max_len=(n5.KV8_SELECT_MAX_BLOCKS + 1) * 64))
+    assert L.n550_kv8_select_blocks(None, P, 2048, long, 0, P, P, 1, 4, 1, 1, P) == n5.ERR_UNSUPPORTED
+
+
+def test_empty_calls_do_nothing():
+    L, c = n5.lib(), struct()
+    for name, rc in calls(L, c, n=0).items():
+        assert rc == n5.OK, name
+    r = C.byref(c)
+    assert L.n550_kv8_append(None, r, 0, None, None, n5.F32, 1024, None, None, 5, 0) == n5.OK
+    assert L.n550_attention_prefill_kv8(None, None, 2048, r, 0, None, 5, 0, 0, None, 2048, None, 0) == n5.OK
+    assert L.n550_attention_kv8_workspace(0) == 0
+    assert L.n550_attention_prefill_kv8_workspace(0, 4, 0) == 0
+
+
+def test_cache_class_refuses_tensors():
+    with pytest.raises(ValueError):
+        n5.KV8Cache(0, 64)
+    with pytest.raises(ValueError):
+        n5.KV8Cache()
+    z = torch.zeros((1, 1, 8, 64, 128)).to(torch.float8_e4m3fn)
+    s = torch.zeros((1, 1, 8, 1))
+    with pytest.raises(ValueError):                       # not on a GPU
+        n5.KV8Cache(k=z, v=z, k_scale=s, v_scale=s)
+    with pytest.raises(ValueError):                       # a part is missing
+        n5.KV8Cache(k=z, v=z, k_scale=s)
+    with pytest.raises(ValueError):                       # scales of another shape
+        n5.KV8Cache(k=z, v=z, k_scale=s, v_scale=torch.zeros((1, 1, 8, 2)))
+
+
+def test_oracle_rounding_is_e4m3():
+    """Every code's value, and rounding against torch's own conversion where that
+    is defined (finite values up to 448)."""
+    codes = torch.arange(256, dtype=torch.int64).to(torch.uint8)
+    v = codes.view(torch.float8_e4m3fn).double()
+    assert torch.equal(values(codes).nan_to_num(nan=999.0), v.nan_to_num(nan=999.0))
+    g = torch.Generator().manual_seed(3)
+    x = torch.cat([torch.randn(4000, generator=g) * 2.0 ** e for e in range(-12, 7)]).clamp(-448, 448)
+    mid = ((POS[1:] + POS[:-1]) / 2).float()              # ties
+    x = torch.cat([x, mid, -mid, POS.float()])
+    assert torch.equal(round_codes(x.double()), x.to(torch.float8_e4m3fn).view(torch.uint8))
+    assert scale_for(torch.tensor([448.0])) == 1.0 and scale_for(torch.tensor([448.5])) == 2.0
+    assert scale_for(torch.tensor([0.0])) == 2.0 ** -126
