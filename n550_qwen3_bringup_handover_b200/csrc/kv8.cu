@@ -20,6 +20,11 @@ int kv8_view(const n550_kv8_cache *c, int layer, Kv8View *v) {
 
 namespace {
 
+// Split partials go to a workspace that is large enough, 16-byte aligned.
+float *split_ws(void *ws, size_t bytes, size_t need) {
+    return ws && bytes >= need && ((uintptr_t)ws & 15) == 0 ? (float *)ws : nullptr;
+}
+
 // gridDim.y and .z end at 65535
 constexpr int kMaxSeqs = 65535;
 
@@ -48,7 +53,7 @@ int n550_kv8_append(void *stream, const n550_kv8_cache *c, int layer, const void
     return launch_kv8_append((cudaStream_t)stream, a, type == N550_F32, n_seqs);
 }
 
-size_t n550_attention_kv8_workspace(int n_seqs) { return kv8_attn_workspace(n_seqs); }
+size_t n550_attention_kv8_workspace(int n_seqs) { return kv8_attn_workspace(n_seqs, 1); }
 
 int n550_attention_decode_kv8(void *stream, const uint16_t *q, int ldq, const n550_kv8_cache *c,
                               int layer, const int32_t *seq_ids, const int32_t *pos, int n_seqs,
@@ -61,6 +66,7 @@ int n550_attention_decode_kv8(void *stream, const uint16_t *q, int ldq, const n5
         return N550_ERR_ARG;
     a.q = q; a.ldq = ldq; a.out = out; a.ldo = ldo; a.seq_ids = seq_ids; a.pos = pos;
     a.L = 1; a.n_seqs = n_seqs; a.n_select = -1;
+    a.part = split_ws(workspace, workspace_bytes, kv8_attn_workspace(n_seqs, 1));
     return launch_kv8_attn((cudaStream_t)stream, a);
 }
 
@@ -78,11 +84,12 @@ int n550_attention_sparse_kv8(void *stream, const uint16_t *q, int ldq, const n5
     a.q = q; a.ldq = ldq; a.out = out; a.ldo = ldo; a.seq_ids = seq_ids; a.pos = pos;
     a.blocks = blocks; a.n_select = n_select;
     a.L = 1; a.n_seqs = n_seqs;
+    a.part = split_ws(workspace, workspace_bytes, kv8_attn_workspace(n_seqs, 1));
     return launch_kv8_attn((cudaStream_t)stream, a);
 }
 
 size_t n550_attention_prefill_kv8_workspace(int n_seqs, int L, int pos0) {
-    return n_seqs > 0 && L > 0 && pos0 >= 0 ? 16 : 0;
+    return n_seqs > 0 && L > 0 && L <= KV8_FEW && pos0 >= 0 ? kv8_attn_workspace(n_seqs, L) : 0;
 }
 
 int n550_attention_prefill_kv8(void *stream, const uint16_t *q, int ldq, const n550_kv8_cache *c,
@@ -97,6 +104,8 @@ int n550_attention_prefill_kv8(void *stream, const uint16_t *q, int ldq, const n
         return N550_ERR_ARG;
     a.q = q; a.ldq = ldq; a.out = out; a.ldo = ldo; a.seq_ids = seq_ids;
     a.L = L; a.pos0 = pos0; a.n_seqs = n_seqs; a.n_select = -1;
+    if (L > KV8_FEW) return launch_kv8_prefill((cudaStream_t)stream, a);
+    a.part = split_ws(workspace, workspace_bytes, kv8_attn_workspace(n_seqs, L));
     return launch_kv8_attn((cudaStream_t)stream, a);
 }
 

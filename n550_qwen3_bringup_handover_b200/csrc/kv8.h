@@ -78,8 +78,10 @@ struct Kv8AttnArgs {
 };
 
 int launch_kv8_append(cudaStream_t st, const Kv8AppendArgs &a, bool f32, int n_seqs);
+constexpr int KV8_FEW = 8;     // most queries per sequence of launch_kv8_attn
+int launch_kv8_prefill(cudaStream_t st, const Kv8AttnArgs &a);
 int launch_kv8_attn(cudaStream_t st, const Kv8AttnArgs &a);
-size_t kv8_attn_workspace(int n_seqs);
+size_t kv8_attn_workspace(int n_seqs, int L);
 
 struct Kv8SelectArgs {
     Kv8View c;
