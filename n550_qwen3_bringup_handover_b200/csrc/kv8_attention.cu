@@ -153,8 +153,25 @@ __device__ __forceinline__ long long locate(const Kv8AttnArgs &p, const Lay lay,
     return total;
 }
 
-// First unit of CTA c of n.
-__device__ __forceinline__ long long run_start(long long total, int c, int n) { return total * c / n; }
+// `total` units cut into n runs that differ by at most one unit: as many runs as
+// CTAs, but none shorter than kMinRun units (a run's blocks are in flight
+// together, and each piece costs the merge a partial).
+constexpr int kMinRun = 2;
+struct Cut {
+    long long q;
+    int n, r;                                   // run c: q units, the first r runs one more
+    __device__ __forceinline__ Cut(long long total, int n_max) {
+        const long long most = (total + kMinRun - 1) / kMinRun;
+        n = most < n_max ? (int)most : n_max;
+        q = total / n;
+        r = (int)(total - q * n);
+    }
+    __device__ __forceinline__ long long start(int c) const { return q * c + min(c, r); }
+    __device__ __forceinline__ int run_of(long long u) const {
+        const long long big = (q + 1) * r;
+        return (int)(u < big ? u / (q + 1) : r + (u - big) / q);
+    }
+};
 
 // NT column tiles of 8: column 8 i + c is query token (8 i + c) / 2 and head
 // 2 kvh + (c & 1).
@@ -196,8 +213,12 @@ kv8_attn_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
     } else {
         long long u0 = 0, u1 = 0;
         locate(p, lay, [&](long long total) {
-            u0 = run_start(total, blockIdx.x, gridDim.x);
-            u1 = run_start(total, blockIdx.x + 1, gridDim.x);
+            const Cut cut(total, gridDim.x);
+            u0 = u1 = total;
+            if ((int)blockIdx.x < cut.n) {
+                u0 = cut.start(blockIdx.x);
+                u1 = cut.start(blockIdx.x + 1);
+            }
             return u0;
         }, &cur);
         n_units = (int)(u1 - u0);
@@ -502,7 +523,8 @@ kv8_attn_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
             if (w.slot < 0) {
                 const size_t row = (size_t)w.s * p.L + (col >> 1);
                 // no position at all: zero
-                p.out[row * p.ldo + (2 * w.kvh + (col & 1)) * KV8_HD + d] = f32_to_bf16_rne(L == 0.f ? 0.f : O / L);
+                p.out[row * p.ldo + (2 * w.kvh + (col & 1)) * KV8_HD + d] =
+                    f32_to_bf16_rne(L == 0.f ? 0.f : O * (1.f / L));
             } else {
                 float *part = p.part + (size_t)w.slot * n_col * (KV8_HD + 2);
                 part[col * KV8_HD + d] = O;
@@ -520,44 +542,82 @@ kv8_attn_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
     }
 }
 
-// Merges the pair that begins in run c and ends behind it (at most one per c).
-__global__ void __launch_bounds__(256) kv8_combine_kernel(const Kv8AttnArgs p, const Lay lay) {
+// Merges the pair that begins in run c = blockIdx.x and ends behind it (at most
+// one). A warp takes one column (128 dimensions, 4 per lane); with 2 or 4 columns
+// the 8 warps share each column's pieces.
+constexpr int CMB_WARPS = 8;
+__global__ void __launch_bounds__(CMB_WARPS * 32) kv8_combine_kernel(const Kv8AttnArgs p, const Lay lay, int n_max) {
+    __shared__ float red[CMB_WARPS][KV8_HD + 1];
     dep_wait();
     dep_launch();
-    const int c = blockIdx.x, n = gridDim.x + 1;               // n runs, n - 1 inner borders
+    const int c = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     Cur cur{};
     long long u0 = 0, u1 = 0;
-    const long long total = locate(p, lay, [&](long long t) {
-        u0 = run_start(t, c, n);
-        u1 = run_start(t, c + 1, n);
+    int n = 0;
+    long long tot = 0;
+    locate(p, lay, [&](long long total) {
+        const Cut cut(total, n_max);
+        tot = total;
+        u0 = u1 = total;
+        n = cut.n;
+        if (c < cut.n - 1) {
+            u0 = cut.start(c);
+            u1 = cut.start(c + 1);
+        }
         return u1;
     }, &cur);
-    if (u0 == u1 || u1 >= total) return;
+    if (c >= n - 1) return;
     const int kvh = (int)(cur.x / cur.upp), j = (int)(cur.x % cur.upp);
-    const long long first = u1 - j, last = first + cur.upp;    // the pair's units
+    const long long first = u1 - j;                            // the pair's first unit
     if (j == 0 || first < u0) return;                          // no pair crosses, or it began earlier
-    const int n_col = 2 * p.L;
+    const int pieces = Cut(tot, n_max).run_of(first + cur.upp - 1) - c + 1;
+    const int n_col = 2 * p.L, wpc = max(1, CMB_WARPS / n_col), sub = warp % wpc;
     const size_t stride = (size_t)n_col * (KV8_HD + 2);
-    // its pieces: run c, then whole runs up to the one that holds unit last - 1
-    const int c_end = (int)((last * n - 1) / total);           // largest run that starts before `last`
-    const float *head = p.part + (2 * (size_t)c + (first > u0)) * stride;
-    for (int i = threadIdx.x; i < n_col * KV8_HD; i += blockDim.x) {
-        const int col = i >> 7;
+    const float *own = p.part + 2 * (size_t)c * stride;        // piece k: slot 2 (c + k), the first 2 c or 2 c + 1
+    const size_t own_off = first > u0 ? stride : 0;
+    for (int col = warp / wpc; col < n_col; col += CMB_WARPS / wpc) {
         const size_t ml = (size_t)n_col * KV8_HD + 2 * col;
-        float M = head[ml];
-        for (int x = c + 1; x <= c_end; x++)
-            if (run_start(total, x, n) < run_start(total, x + 1, n)) M = fmaxf(M, p.part[2 * x * stride + ml]);
-        float f = head[ml] == M ? 1.f : ex2(head[ml] - M);
-        float L = head[ml + 1] * f, O = head[i] * f;
-        for (int x = c + 1; x <= c_end; x++) {
-            if (run_start(total, x, n) == run_start(total, x + 1, n)) continue;
-            const float *q = p.part + 2 * x * stride;
-            f = q[ml] == M ? 1.f : ex2(q[ml] - M);
-            L += q[ml + 1] * f;
-            O += q[i] * f;
+        float M = -INFINITY;
+        for (int k = lane; k < pieces; k += 32) M = fmaxf(M, __ldcg(own + 2 * k * stride + (k ? 0 : own_off) + ml));
+#pragma unroll
+        for (int x = 16; x > 0; x >>= 1) M = fmaxf(M, __shfl_xor_sync(0xFFFFFFFFu, M, x));
+        float L = 0.f;
+        float4 O = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int k0 = 0; k0 < pieces; k0 += 32 * wpc) {        // lane i of this batch: piece k0 + wpc i + sub
+            const int k = k0 + wpc * lane + sub;
+            float f = 0.f;
+            if (k < pieces) {
+                const float2 v = __ldcg((const float2 *)(own + 2 * k * stride + (k ? 0 : own_off) + ml));
+                f = v.x == M ? 1.f : ex2(v.x - M);
+                L += v.y * f;
+            }
+            const int take = min(32, (pieces - k0 - sub + wpc - 1) / wpc);
+#pragma unroll 8
+            for (int i = 0; i < take; i++) {
+                const int ki = k0 + wpc * i + sub;
+                const float w = __shfl_sync(0xFFFFFFFFu, f, i);
+                const float4 v = __ldcg((const float4 *)(own + 2 * ki * stride + (ki ? 0 : own_off) + col * KV8_HD) + lane);
+                O.x += v.x * w; O.y += v.y * w; O.z += v.z * w; O.w += v.w * w;
+            }
+        }
+#pragma unroll
+        for (int x = 16; x > 0; x >>= 1) L += __shfl_xor_sync(0xFFFFFFFFu, L, x);
+        if (wpc > 1) {                                         // one round: every warp comes here once
+            float *d = red[warp] + 4 * lane;
+            d[0] = O.x; d[1] = O.y; d[2] = O.z; d[3] = O.w;
+            if (lane == 0) red[warp][KV8_HD] = L;
+            __syncthreads();
+            if (sub) continue;
+            for (int w = 1; w < wpc; w++) {
+                const float *q = red[warp + w] + 4 * lane;
+                O.x += q[0]; O.y += q[1]; O.z += q[2]; O.w += q[3];
+                L += red[warp + w][KV8_HD];
+            }
         }
         const size_t row = (size_t)cur.s * p.L + (col >> 1);
-        p.out[row * p.ldo + (2 * kvh + (col & 1)) * KV8_HD + (i & 127)] = f32_to_bf16_rne(L == 0.f ? 0.f : O / L);
+        const float inv = L == 0.f ? 0.f : 1.f / L;
+        uint2 *dst = (uint2 *)(p.out + row * p.ldo + (2 * kvh + (col & 1)) * KV8_HD) + lane;
+        *dst = make_uint2(pack_bf16x2(O.x * inv, O.y * inv), pack_bf16x2(O.z * inv, O.w * inv));
     }
 }
 
@@ -601,13 +661,13 @@ int launch(cudaStream_t st, const CUtensorMap &tk, const CUtensorMap &tv, const 
         lay.kind = LAY_EVEN;
         lay.upp = (a.pos0 + a.L + KV8_BLOCK - 1) / KV8_BLOCK;
     }
-    // no more runs than there can be units
-    const long long most = pairs * (lay.kind == LAY_EVEN ? lay.upp : a.c.nb);
+    // no more runs than there can be (the kernels cut by the units there are)
+    const long long most = (pairs * (lay.kind == LAY_EVEN ? lay.upp : a.c.nb) + kMinRun - 1) / kMinRun;
     const int n = (int)(most < ctas<NT>(a.L) ? most : ctas<NT>(a.L));
     N550_CUDA_TRY(launch_k(kv8_attn_kernel<NT>, dim3(n), THREADS, smem, st, tk, tv, a, lay));
     N550_LAUNCH_CHECK();
     if (n > 1) {
-        N550_CUDA_TRY(launch_k(kv8_combine_kernel, dim3(n - 1), 256, 0, st, a, lay));
+        N550_CUDA_TRY(launch_k(kv8_combine_kernel, dim3(n - 1), CMB_WARPS * 32, 0, st, a, lay, n));
         N550_LAUNCH_CHECK();
     }
     return N550_OK;
