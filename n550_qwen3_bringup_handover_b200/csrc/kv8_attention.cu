@@ -10,15 +10,26 @@
 // the SMs evenly, where one CTA per pair waits for the longest. A run that ends
 // inside a pair leaves a partial (max, sum, out) that the combine kernel merges.
 //
-// In a CTA one warp reads block lists and scales and streams K and V blocks (8
-// KB each) through a ring of TMA loads, and four warps take 16 positions of every
-// block each. Codes become FP16 in registers, exactly (e4m3 is a subset), on
-// their way from shared memory into mma.sync fragments with the positions (for
-// q . k) and the dimensions (for P . v) as the 16-row side and the query columns
-// as the 8-column side: 2 heads x 4 tokens fill a tile that a decode leaves 3/4
-// empty, at a tenth of the tensor rate either way. The 128-byte swizzle and the
-// row permutation tok_of() let every shared-memory access read 8 different
-// 16-byte columns per phase.
+// The codes are tensor-core operands as they lie in the cache: tiles of 128
+// positions (two blocks) go from HBM by TMA into shared memory and from there
+// into tcgen05.mma kind::f8f6f4, K as the 128-row side of S^T = K q^T, V (MN-major)
+// as the 128-row side of O^T = V^T P^T. No code passes through a register; the
+// mma.sync form of this kernel, which turned codes into FP16 there, issued about
+// 390 instructions per warp and 16 positions and stopped at 4.7 TB/s (256
+// sequences x 1152 positions, 114 us). The 8-column side has room for queries and
+// weights in e4m3 parts, four bits a part:
+//   q = 2^a (h + l / 16): two parts hold a BF16 value whole, down to 2^-21 of the
+//       row's largest;
+//   w = 2^-8 (w1 + w2 / 16 + w3 / 256): three parts hold a softmax weight to 12
+//       bits (2^-13 half a step), or 2^-26 of the largest for the small ones.
+// Sums, scores and the softmax state are FP32.
+//
+//   warp 0     producer: walks the run, 32 blocks a batch (one per lane: list entry,
+//              slot, scales), and fills a ring of 32 KB stages
+//   warp 1     issues the MMAs, S of the next tile before P.V of this one
+//   warp 6     splits the queries of each new pair
+//   warps 2-5  softmax, a thread per position, and the output, a thread per
+//              dimension; they agree on a tile's maximum through shared memory
 #include <cuda.h>
 
 #include "kv8.h"
@@ -28,18 +39,17 @@
 namespace n550 {
 namespace {
 
-constexpr int CW = 4;                           // consumer warps
-constexpr int THREADS = (CW + 1) * 32;
-constexpr int TILE = KV8_BLOCK * KV8_HD;        // 8 KB of K or V codes
-constexpr float kLazy = 8.0f;                   // a maximum may be 8 (a factor 256) stale
+constexpr int THREADS = 224;                    // 7 warps
+constexpr int BLK = KV8_BLOCK * KV8_HD;         // 8 KB of K or V codes
+constexpr int STAGE = 4 * BLK;                  // K of two blocks | V of two blocks
 
-// What the producer says about a ring stage: one block of one pair.
-struct Rec {
-    int s, kvh, blk, ctx;                       // blk < 0: nothing to read
-    float ks, vs;
-    int flags, slot;                            // partial slot, or -1: the whole pair
+// What the producer says about a ring stage: one or two blocks of one pair.
+struct __align__(16) Rec {
+    int s, kvh, blk[2], ctx;                    // blk[0] < 0: nothing to read, blk[1] < 0: one block
+    float ks[2], vs[2];
+    int flags, slot, pad;                       // partial slot, or -1: the whole pair
 };
-enum { R_FIRST = 1, R_LAST = 2, R_END = 4 };
+enum { R_FIRST = 1, R_LAST = 2, R_END = 4, R_Q = 8 };   // of a piece, of the run; the piece's first tile
 
 // How the blocks are laid out along the run axis.
 enum { LAY_RAGGED = 0, LAY_EVEN = 1, LAY_PAIR = 2 };
@@ -48,40 +58,104 @@ struct Lay {
     int upp;                                    // LAY_EVEN: units per pair
 };
 
-template <int NT> constexpr int stages() { return NT == 1 ? 4 : 3; }
-
-__device__ __forceinline__ int tok_of(int g) { return (g & 1) ? (g & 6) ^ 5 : g; }
+// LT: most query tokens (2 heads each) of an instance. S has 4 columns a token,
+// O (and P) 6; the MMA's column side is a multiple of 16.
+template <int LT> constexpr int s_cols() { return LT == 1 ? 16 : 4 * LT; }
+template <int LT> constexpr int p_cols() { return (6 * LT + 15) / 16 * 16; }
+template <int LT> constexpr int tmem_cols() {
+    return 2 * (s_cols<LT>() + p_cols<LT>()) <= 64 ? 64 : 2 * (s_cols<LT>() + p_cols<LT>()) <= 128 ? 128 : 256;
+}
+template <int LT> constexpr int op_bytes() { return 2 * 128 * (s_cols<LT>() + p_cols<LT>()); }
+template <int LT> constexpr int smem_bytes(int L, int st) { return st * (STAGE + L * 512) + op_bytes<LT>() + 1024; }
+template <int LT> constexpr int stages() { return LT == 1 ? 2 : 5; }
 
 __device__ __forceinline__ float ex2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
-__device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
-    uint32_t r;
-    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
-    return r;
+
+// D[tmem] (+)= A[smem] . B[smem]^T, e4m3 x e4m3 -> FP32, M = 128, K = 32.
+__device__ __forceinline__ void umma_e4m3(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
+                                          uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}"
+        ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+        : "memory");
 }
-// Transposes an 8 x 8 matrix of 16-bit values held one row per four lanes.
-__device__ __forceinline__ uint32_t transpose8(uint32_t x) {
-    uint32_t y;
-    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+// Instruction descriptor: D FP32, A and B e4m3 (format 0), M = 128; a_mn: A is MN-major.
+__host__ __device__ constexpr uint32_t idesc_e4m3(int N, int a_mn) {
+    return (1u << 4) | ((uint32_t)a_mn << 15) | ((uint32_t)(N >> 3) << 17) | ((128u >> 4) << 24);
+}
+
+__device__ __forceinline__ void tmem_ld_x4(uint32_t taddr, uint32_t *r) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x4.b32 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_ld_x8(uint32_t taddr, uint32_t *r) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+                 : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_st_x8(uint32_t taddr, const uint32_t *r) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};"
+                 ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+                 : "memory");
+}
+// The S columns (4 LT) and O columns (6 LT, rounded up to whole loads) of this
+// thread's TMEM lane.
+template <int LT>
+__device__ __forceinline__ void load_s(uint32_t t, uint32_t (&r)[4 * LT]) {
+    if constexpr (LT == 1) tmem_ld_x4(t, r);
+    else if constexpr (LT == 4) tmem_ld_32x32b_x16(t, r);
+    else tmem_ld_32x32b_x32(t, r);
+    tmem_ld_wait();
+}
+template <int LT> constexpr int o_regs() { return LT == 1 ? 8 : LT == 4 ? 32 : 48; }
+template <int LT>
+__device__ __forceinline__ void load_o(uint32_t t, uint32_t (&r)[o_regs<LT>()]) {
+    if constexpr (LT == 1) tmem_ld_x8(t, r);
+    else if constexpr (LT == 4) tmem_ld_32x32b_x32(t, r);
+    else {
+        tmem_ld_32x32b_x32(t, *reinterpret_cast<uint32_t(*)[32]>(&r[0]));
+        tmem_ld_32x32b_x16(t + 32, *reinterpret_cast<uint32_t(*)[16]>(&r[32]));
+    }
+    tmem_ld_wait();
+}
+template <int LT>
+__device__ __forceinline__ void store_o(uint32_t t, const uint32_t (&r)[o_regs<LT>()]) {
+    if constexpr (LT == 1) tmem_st_x8(t, r);
+    else if constexpr (LT == 4) tmem_st_32x32b_x32(t, r);
+    else {
+        tmem_st_32x32b_x32(t, *reinterpret_cast<const uint32_t(*)[32]>(&r[0]));
+        tmem_st_32x32b_x16(t + 32, *reinterpret_cast<const uint32_t(*)[16]>(&r[32]));
+    }
+    tmem_st_wait();
+}
+
+// Maximum over the warp; a NaN counts as nothing.
+__device__ __forceinline__ float warp_max(float x) {
+    float y;
+    asm volatile("redux.sync.max.f32 %0, %1, 0xFFFFFFFF;" : "=f"(y) : "f"(x));
     return y;
 }
-// D (16 x 8, FP32) += A (16 x 16 FP16) . B (16 x 8 FP16)
-__device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
-                                        uint32_t b0, uint32_t b1) {
+// Whether the phase has completed, without waiting (try_wait may suspend the thread).
+__device__ __forceinline__ bool mbar_test(uint64_t *bar, uint32_t parity) {
+    uint32_t ok;
     asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
-        "{%0,%1,%2,%3};"
-        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok) : "r"(smem_u32(bar)), "r"(parity) : "memory");
+    return ok != 0;
 }
-__device__ __forceinline__ uint4 lds128(uint32_t addr) {
-    uint4 v;
-    asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr));
-    return v;
+__device__ __forceinline__ bool warp_wait(uint64_t *bar, uint32_t parity) {
+    return __all_sync(0xFFFFFFFFu, mbar_wait(bar, parity));
 }
+// Byte offset of byte k of row n in an operand of 128-byte rows, 128-byte swizzle.
+__device__ __forceinline__ uint32_t sw(int n, int k) { return n * 128 + ((((k >> 4) ^ n) & 7) << 4) + (k & 15); }
 
 // Units (blocks; one empty unit for an empty context) of a pair of sequence s.
 __device__ __forceinline__ int seq_ctx(const Kv8AttnArgs &p, int s) {
@@ -93,8 +167,7 @@ __device__ __forceinline__ int ctx_blocks(int ctx) { return max(1, (ctx + KV8_BL
 
 // Cursor into the run axis: sequence s, unit x of its 8 pairs, upp units per pair.
 struct Cur {
-    int s, upp, ctx;
-    long long x;
+    int s, upp, ctx, x;
 };
 
 // All threads of the CTA. Returns the total number of units and places *cur at
@@ -106,17 +179,22 @@ __device__ __forceinline__ long long locate(const Kv8AttnArgs &p, const Lay lay,
         const long long total = (long long)lay.upp * KV8_NKV * p.n_seqs, u = first(total);
         if (u >= total) return total;
         cur->s = (int)(u / ((long long)lay.upp * KV8_NKV));
-        cur->x = u - (long long)cur->s * lay.upp * KV8_NKV;
+        cur->x = (int)(u - (long long)cur->s * lay.upp * KV8_NKV);
         cur->upp = lay.upp;
         return total;
     }
+    constexpr int KEEP = 4;                      // contexts a thread keeps in registers (else it reads them again)
     __shared__ long long wsum[32];
-    __shared__ int found_s;
-    __shared__ long long found_x;
+    __shared__ Cur found;
     const int nt = blockDim.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int per = (p.n_seqs + nt - 1) / nt, s0 = min(tid * per, p.n_seqs), s1 = min(s0 + per, p.n_seqs);
+    int kept[KEEP];
     long long mine = 0;
-    for (int s = s0; s < s1; s++) mine += (long long)ctx_blocks(seq_ctx(p, s)) * KV8_NKV;
+#pragma unroll
+    for (int i = 0; i < KEEP; i++) kept[i] = s0 + i < s1 ? seq_ctx(p, s0 + i) : 0;
+#pragma unroll
+    for (int i = 0; i < KEEP; i++) mine += s0 + i < s1 ? ctx_blocks(kept[i]) * KV8_NKV : 0;
+    for (int s = s0 + KEEP; s < s1; s++) mine += (long long)ctx_blocks(seq_ctx(p, s)) * KV8_NKV;
     long long pre = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -133,23 +211,27 @@ __device__ __forceinline__ long long locate(const Kv8AttnArgs &p, const Lay lay,
     const long long u = first(total);
     pre += base - mine;                          // units before this thread's sequences
     if (u >= pre && u < pre + mine) {
-        int s = s0;
         long long x = u - pre;
-        for (;; s++) {
-            const long long n = (long long)ctx_blocks(seq_ctx(p, s)) * KV8_NKV;
-            if (x < n) break;
-            x -= n;
+        int s = s0, ctx = 0, n = 0;
+        bool hit = false;
+#pragma unroll
+        for (int i = 0; i < KEEP; i++)
+            if (!hit && s < s1) {
+                ctx = kept[i];
+                n = ctx_blocks(ctx);
+                hit = x < (long long)n * KV8_NKV;
+                if (!hit) { x -= (long long)n * KV8_NKV; s++; }
+            }
+        while (!hit) {
+            ctx = seq_ctx(p, s);
+            n = ctx_blocks(ctx);
+            hit = x < (long long)n * KV8_NKV;
+            if (!hit) { x -= (long long)n * KV8_NKV; s++; }
         }
-        found_s = s;
-        found_x = x;
+        found.s = s; found.upp = n; found.ctx = ctx; found.x = (int)x;
     }
     __syncthreads();
-    if (u < total) {
-        cur->s = found_s;
-        cur->x = found_x;
-        cur->ctx = seq_ctx(p, found_s);
-        cur->upp = ctx_blocks(cur->ctx);
-    }
+    if (u < total) *cur = found;
     return total;
 }
 
@@ -173,43 +255,56 @@ struct Cut {
     }
 };
 
-// NT column tiles of 8: column 8 i + c is query token (8 i + c) / 2 and head
-// 2 kvh + (c & 1).
-template <int NT>
+template <int LT, int ST>
 __global__ void __launch_bounds__(THREADS)
 kv8_attn_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
                 const Kv8AttnArgs p, const Lay lay) {
-    constexpr int ST = stages<NT>();
+    constexpr int NS = s_cols<LT>(), NP = p_cols<LT>(), NC = 2 * LT;
     extern __shared__ uint8_t dsm[];
-    uint8_t *ring = (uint8_t *)(((uintptr_t)dsm + 1023) & ~(uintptr_t)1023);     // [ST][K | V]
-    const int q_stride = p.L * 512;                                               // 2 heads x 128 BF16 per token
-    uint8_t *sq = ring + ST * 2 * TILE;                                           // [ST][L][256]
-    float *wo = (float *)(sq + ST * q_stride);                                    // [CW][2 L][128]
-    __shared__ __align__(16) Rec rec[ST];
-    __shared__ __align__(8) uint64_t full[ST], empty[ST], merge[2];
-    __shared__ float wm[CW][8 * NT], wl[CW][8 * NT], wscale[CW];
+    uint8_t *ring = (uint8_t *)(((uintptr_t)dsm + 1023) & ~(uintptr_t)1023);      // [ST][STAGE]
+    uint8_t *sQ = ring + ST * STAGE;                                               // [2][NS][128]
+    uint8_t *sP = sQ + 2 * NS * 128;                                               // [2][NP][128]
+    uint8_t *sraw = sP + 2 * NP * 128;                                             // [ST][L][2 heads x 128 BF16]
+    __shared__ Rec rec[ST];
+    __shared__ __align__(8) uint64_t full[ST], empty[ST], q_ready[4], q_free[2], s_full[2], p_full[2], pv_done[2], o_free[2], done;
+    __shared__ float q_scale[4][NC];            // power of two of each query row, by piece modulo 4
+    __shared__ float xmax[2][4][NC], xsum[2][4][NC];
+    __shared__ int xdead[2][4];
+    __shared__ uint32_t tmem_slot;
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
-        for (int i = 0; i < ST; i++) { mbar_init(&full[i], 1); mbar_init(&empty[i], CW); }
-        mbar_init(&merge[0], CW);
-        mbar_init(&merge[1], CW);
+        for (int i = 0; i < ST; i++) { mbar_init(&full[i], 1); mbar_init(&empty[i], 6); }
+        for (int i = 0; i < 2; i++) {
+            mbar_init(&q_ready[i], 1);
+            mbar_init(&q_ready[2 + i], 1);
+            mbar_init(&q_free[i], 1);
+            mbar_init(&s_full[i], 1);
+            mbar_init(&p_full[i], 4);
+            mbar_init(&pv_done[i], 1);
+            mbar_init(&o_free[i], 4);
+        }
+        mbar_init(&done, 1);
         fence_mbar_init();
         tma_prefetch_desc(&tmK);
         tma_prefetch_desc(&tmV);
     }
+    if (warp == 1) { tmem_alloc(&tmem_slot, tmem_cols<LT>()); tmem_relinquish(); }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = tmem_slot, tS = tmem, tO = tmem + 2 * NS;
     // block lists, positions, scales, codes and queries all come from earlier kernels
-    dep_wait();
     dep_launch();
+    dep_wait();
     Cur cur{};
     int n_units;
     if (lay.kind == LAY_PAIR) {
         cur.s = blockIdx.x / KV8_NKV;
         cur.ctx = seq_ctx(p, cur.s);
         cur.upp = p.n_select >= 0 ? max(1, p.n_select) : ctx_blocks(cur.ctx);
-        cur.x = (long long)(blockIdx.x % KV8_NKV) * cur.upp;
+        cur.x = (int)(blockIdx.x % KV8_NKV) * cur.upp;
         n_units = cur.upp;
-        __syncthreads();
     } else {
         long long u0 = 0, u1 = 0;
         locate(p, lay, [&](long long total) {
@@ -222,24 +317,24 @@ kv8_attn_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
             return u0;
         }, &cur);
         n_units = (int)(u1 - u0);
-        if (lay.kind == LAY_EVEN) __syncthreads();
     }
-    if (n_units == 0) return;
 
-    if (warp == CW) {
+    if (n_units > 0 && warp == 0) {
         // ---------------- producer: lane i takes unit 32 k + i ----------------
-        int r = 0;                                                 // records issued
-        bool ok = true;
-        for (int base = 0; base < n_units && ok; base += 32) {
+        bool seen = false;                       // the piece that reaches into this batch had a tile
+        // The records of the batch of 32 units at `base` (the next one is read while the
+        // ring still takes this one: its loads depend on one another three deep).
+        auto batch = [&](int base, Rec &me, int &plane, uint32_t &sends) {
             const int i = base + lane;
-            Rec me{};
+            me = Rec{};
             bool send = false;
+            int ps = i;                          // the run's unit with which the piece begins
             // walk to this lane's unit: whole sequences first
             Cur c = cur;
             if (base + 31 < n_units || i < n_units) {
                 c.x += lane;
-                while (c.x >= (long long)c.upp * KV8_NKV && c.s + 1 < p.n_seqs) {
-                    c.x -= (long long)c.upp * KV8_NKV;
+                while (c.x >= c.upp * KV8_NKV && c.s + 1 < p.n_seqs) {
+                    c.x -= c.upp * KV8_NKV;
                     c.s++;
                     if (lay.kind == LAY_RAGGED) {
                         c.ctx = seq_ctx(p, c.s);
@@ -247,298 +342,402 @@ kv8_attn_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
                     }
                 }
             }
+            me.blk[0] = me.blk[1] = -1;
+            plane = 0;
             if (i < n_units) {
+                const int slot = __ldcg(p.seq_ids + c.s);
                 if (lay.kind == LAY_EVEN) c.ctx = seq_ctx(p, c.s);
-                const int kvh = (int)(c.x / c.upp), j = (int)(c.x % c.upp);
+                const int kvh = c.x / c.upp, j = c.x - kvh * c.upp;
                 int b = j;
                 if (p.n_select >= 0)
                     b = p.n_select > 0 ? __ldcg(p.blocks + ((size_t)c.s * KV8_NKV + kvh) * p.n_select + j) : -1;
                 if (b < 0 || b > (c.ctx - 1) >> 6) b = -1;      // ctx 0: -1 >> 6 = -1
-                me.s = c.s; me.kvh = kvh; me.blk = b; me.ctx = c.ctx;
+                me.s = c.s; me.kvh = kvh; me.blk[0] = b; me.ctx = c.ctx;
                 me.flags = (i == 0 || j == 0 ? R_FIRST : 0) | (i == n_units - 1 || j == c.upp - 1 ? R_LAST : 0) |
                            (i == n_units - 1 ? R_END : 0);
                 // a piece [first unit here .. last unit here] that is not the whole pair
                 // is a partial; the one that begins this CTA's run takes slot 2 c
+                ps = max(0, i - j);
                 const bool head = i - j < 0;                     // the pair begins before this run
                 const bool tail = i - j + c.upp > n_units;       // and here ends behind it
                 me.slot = head || tail ? 2 * (int)blockIdx.x + (i - j > 0) : -1;
                 if (b >= 0) {
-                    const size_t o = p.c.plane(__ldcg(p.seq_ids + c.s), kvh) * p.c.nb + b;
-                    me.ks = __ldcg(p.c.ks + o);
-                    me.vs = __ldcg(p.c.vs + o);
+                    plane = (int)p.c.plane(slot, kvh);
+                    me.ks[0] = __ldcg(p.c.ks + (size_t)plane * p.c.nb + b);
+                    me.vs[0] = __ldcg(p.c.vs + (size_t)plane * p.c.nb + b);
                 }
                 // an unlisted block needs no stage unless its pair begins or ends with it
                 send = b >= 0 || (me.flags & (R_FIRST | R_LAST));
             }
-            const int n = min(32, n_units - base);
-            const uint32_t sends = __ballot_sync(0xFFFFFFFFu, send);
-            for (int l = 0; l < n; l++) {
-                if (!(sends >> l & 1)) continue;
-                const int st = r % ST;
-                if (lane == l) {
-                    ok = mbar_wait(&empty[st], ((r / ST) & 1) ^ 1);
-                    if (ok) {
-                        rec[st] = me;
-                        const int qn = me.flags & R_FIRST ? p.L : 0;
-                        const uint32_t tx = (me.blk >= 0 ? 2 * TILE : 0) + qn * 512;
-                        if (tx) mbar_arrive_expect_tx(&full[st], tx);
-                        else mbar_arrive(&full[st]);
-                        if (me.blk >= 0) {
-                            const int plane = (int)p.c.plane(__ldcg(p.seq_ids + me.s), me.kvh);
-                            uint8_t *t = ring + st * 2 * TILE;
-                            tma_load_3d(t, &tmK, &full[st], 0, me.blk * KV8_BLOCK, plane);
-                            tma_load_3d(t + TILE, &tmV, &full[st], 0, me.blk * KV8_BLOCK, plane);
-                        }
-                        for (int j = 0; j < qn; j++)
-                            bulk_load(sq + st * q_stride + j * 512,
-                                      p.q + ((size_t)me.s * p.L + j) * p.ldq + me.kvh * 2 * KV8_HD, 512, &full[st]);
-                    }
-                }
-                ok = __shfl_sync(0xFFFFFFFFu, ok, l);
-                if (!ok) break;
-                r++;
+            // the queries travel with the piece's first tile
+            {
+                const bool tile = me.blk[0] >= 0;
+                const uint32_t before = __ballot_sync(0xFFFFFFFFu, tile) & ((1u << lane) - 1u) & ~0u << max(0, ps - base);
+                const bool earlier = before != 0 || (ps < base && seen);
+                if (tile && !earlier) me.flags |= R_Q;
+                seen = __shfl_sync(0xFFFFFFFFu, earlier || tile, 31);
             }
+            // Lanes 2 i and 2 i + 1 share a stage where both hold a block of one piece
+            // and V's scales are near enough for weights in one scale (2^6: the
+            // smaller block's weights keep 2^-20 of their own largest).
+            const int blk = __shfl_down_sync(0xFFFFFFFFu, me.blk[0], 1), fl = __shfl_down_sync(0xFFFFFFFFu, me.flags, 1);
+            const float ks = __shfl_down_sync(0xFFFFFFFFu, me.ks[0], 1), vs = __shfl_down_sync(0xFFFFFFFFu, me.vs[0], 1);
+            bool two = false;
+            if (!(lane & 1) && i + 1 < n_units && me.blk[0] >= 0 && blk >= 0 && !(fl & R_FIRST) &&
+                fmaxf(vs, me.vs[0]) <= 64.f * fminf(vs, me.vs[0])) {
+                two = true;
+                me.blk[1] = blk;
+                me.ks[1] = ks;
+                me.vs[1] = vs;
+                me.flags |= fl;
+            }
+            if (__shfl_up_sync(0xFFFFFFFFu, (int)two, 1) && (lane & 1)) send = false;
+            sends = __ballot_sync(0xFFFFFFFFu, send);
             // the next batch starts behind lane 31's unit
             cur.s = __shfl_sync(0xFFFFFFFFu, c.s, 31);
             cur.upp = __shfl_sync(0xFFFFFFFFu, c.upp, 31);
             cur.ctx = __shfl_sync(0xFFFFFFFFu, c.ctx, 31);
             cur.x = __shfl_sync(0xFFFFFFFFu, c.x, 31) + 1;
+        };
+        Rec me, nxt;
+        int plane, nplane;
+        uint32_t sends, nsends;
+        batch(0, me, plane, sends);
+        int r = 0;                               // records issued
+        bool ok = true;
+        for (int base = 0; base < n_units && ok; base += 32) {
+            bool more = false;
+            for (; sends; sends &= sends - 1) {
+                const int l = __ffs(sends) - 1, st = r % ST;
+                if (lane == l) {
+                    ok = mbar_wait(&empty[st], ((r / ST) & 1) ^ 1);
+                    if (ok) {
+                        rec[st] = me;
+                        const int qn = me.flags & R_Q ? p.L : 0;
+                        const uint32_t tx = (me.blk[0] >= 0 ? 2 * BLK : 0) + (me.blk[1] >= 0 ? 2 * BLK : 0) + qn * 512;
+                        if (tx) mbar_arrive_expect_tx(&full[st], tx);
+                        else mbar_arrive(&full[st]);
+                        uint8_t *t = ring + st * STAGE;
+                        for (int j = 0; j < qn; j++)
+                            bulk_load(sraw + (st * p.L + j) * 512,
+                                      p.q + ((size_t)me.s * p.L + j) * p.ldq + me.kvh * 2 * KV8_HD, 512, &full[st]);
+                        for (int j = 0; j < 2; j++)
+                            if (me.blk[j] >= 0) {
+                                tma_load_3d(t + j * BLK, &tmK, &full[st], 0, me.blk[j] * KV8_BLOCK, plane);
+                                tma_load_3d(t + (2 + j) * BLK, &tmV, &full[st], 0, me.blk[j] * KV8_BLOCK, plane);
+                            }
+                    }
+                }
+                ok = __shfl_sync(0xFFFFFFFFu, ok, l);
+                if (!ok) break;
+                r++;
+                if (!more && base + 32 < n_units) {   // once the batch's first records are on their way
+                    more = true;
+                    batch(base + 32, nxt, nplane, nsends);
+                }
+            }
+            if (!ok || base + 32 >= n_units) break;
+            if (!more) batch(base + 32, nxt, nplane, nsends);
+            me = nxt;
+            plane = nplane;
+            sends = nsends;
         }
         // every load must have landed before the CTA exits: the last ST records
         if (lane == 0)
             for (int i = max(0, r - ST); i < r; i++) mbar_wait(&full[i % ST], (i / ST) & 1);
         __syncwarp();
-        return;
-    }
-
-    // ---------------- consumers: positions 16 warp .. 16 warp + 15 of every block ----------------
-    const int g = lane >> 2, tq = lane & 3, p0 = warp * 16;
-    const int n_col = 2 * p.L;
-    uint32_t qa[NT][16];                        // q of column g: dims 16 tq + 2 e (+1), then 64 + 16 tq ..
-    float qs[NT][2];                            // score factor of columns 2 tq, 2 tq + 1
-    float m[NT][2], l[NT][2], o[NT][8][4], vref = 0.f, vinv = INFINITY;
-    int jlim[NT][2];                            // last position of the columns' queries
-    int merged = 0;
-    // addresses of this lane's 16-byte chunks in a tile (row r at 128 r, chunk c at c ^ (r & 7))
-    const int kr = p0 + tok_of(g), va = p0 + 2 * tq, vb = p0 + ((2 * tq) ^ 5);
-    const uint32_t k_off[2] = {(uint32_t)(kr * 128 + ((tq ^ (kr & 7)) << 4)),
-                               (uint32_t)(kr * 128 + (((tq + 4) ^ (kr & 7)) << 4))};
-    const uint32_t v_off[2] = {(uint32_t)(va * 128 + ((g ^ (va & 7)) << 4)),
-                               (uint32_t)(vb * 128 + ((g ^ (vb & 7)) << 4))};
-    for (int r = 0;; r++) {
-        const int st = r % ST;
-        if (!__all_sync(0xFFFFFFFFu, mbar_wait(&full[st], (r / ST) & 1))) return;
-        const Rec w = rec[st];
-        if (w.flags & R_FIRST) {
-            // queries: FP16 with the column's largest magnitude brought into [1, 2) by
-            // a power of two, which BF16 values survive whole (down to 2^-14 of it)
-            const uint32_t qb = smem_u32(sq + st * q_stride);
-#pragma unroll
-            for (int i = 0; i < NT; i++) {
-                const int col = 8 * i + g;
-                uint32_t x[16];
-#pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    uint4 t = make_uint4(0u, 0u, 0u, 0u);
-                    if (col < n_col)
-                        t = lds128(qb + col * 256 + (e >> 1) * 128 + tq * 32 + (e & 1) * 16);
-                    x[4 * e] = t.x; x[4 * e + 1] = t.y; x[4 * e + 2] = t.z; x[4 * e + 3] = t.w;
-                }
-                uint32_t am = 0;
-#pragma unroll
-                for (int e = 0; e < 16; e++) am = max(am, max(x[e] & 0x7FFFu, x[e] >> 16 & 0x7FFFu));
-                am = max(am, __shfl_xor_sync(0xFFFFFFFFu, am, 1));
-                am = max(am, __shfl_xor_sync(0xFFFFFFFFu, am, 2));
-                const int e2 = min(max((int)(am >> 7) - 127, -126), 126);
-                const float inv = __uint_as_float((uint32_t)(127 - e2) << 23);
-                const float up = __uint_as_float((uint32_t)(127 + e2) << 23);
-#pragma unroll
-                for (int e = 0; e < 16; e++)
-                    qa[i][e] = pack_f16x2(__uint_as_float(x[e] << 16) * inv,
-                                          __uint_as_float(x[e] & 0xFFFF0000u) * inv);
-                qs[i][0] = __shfl_sync(0xFFFFFFFFu, up, 8 * tq);
-                qs[i][1] = __shfl_sync(0xFFFFFFFFu, up, 8 * tq + 4);
-#pragma unroll
-                for (int c = 0; c < 2; c++) {
-                    m[i][c] = -INFINITY;
-                    l[i][c] = 0.f;
-                    // both columns of a lane are heads of one token
-                    jlim[i][c] = w.ctx - p.L + 4 * i + tq;
-                }
-#pragma unroll
-                for (int d = 0; d < 8; d++) o[i][d][0] = o[i][d][1] = o[i][d][2] = o[i][d][3] = 0.f;
+    } else if (n_units > 0 && warp == 1) {
+        // ---------------- MMAs ----------------
+        constexpr uint32_t id_s = idesc_e4m3(NS, 0), id_o = idesc_e4m3(NP, 1);
+        const uint32_t aR = smem_u32(ring), aQ = smem_u32(sQ), aP = smem_u32(sP);
+        int t = 0, piece = -1;                   // tiles whose S was issued; this piece with tiles
+        int w_st = 0, w_half = 0, w_first = 0, w_piece = 0;       // the tile whose P.V is due
+        bool due = false, ok = true;
+        auto issue_pv = [&]() -> bool {
+            const int u = t - 1, b = u & 1;
+            due = false;
+            if (!warp_wait(&p_full[b], (u >> 1) & 1)) return false;
+            // the first P.V of a piece overwrites O: its buffer must have been read out
+            if (w_first && !warp_wait(&o_free[w_piece & 1], ((w_piece >> 1) & 1) ^ 1)) return false;
+            tc_fence_after();
+            const uint32_t v = aR + w_st * STAGE + 2 * BLK, pp = aP + b * NP * 128, d = tO + (w_piece & 1) * NP;
+            const int steps = w_half ? 2 : 4;
+            for (int k = 0; k < steps; k++)
+                if (elect_one_sync())
+                    umma_e4m3(d, umma_desc_sw128_mn(v + k * 4096, 0), umma_desc_sw128(pp + k * 32), id_o,
+                              (w_first && k == 0) ? 0u : 1u);
+            if (elect_one_sync()) { umma_commit(&empty[w_st]); umma_commit(&pv_done[b]); }
+            __syncwarp();
+            return true;
+        };
+        bool first = false;                      // no tile of this piece yet
+        for (int r = 0;; r++) {
+            const int st = r % ST;
+            // nothing to issue S for yet: the due P.V frees its stage
+            if (due && !__all_sync(0xFFFFFFFFu, mbar_test(&full[st], (r / ST) & 1)) && !(ok = issue_pv())) break;
+            if (!(ok = warp_wait(&full[st], (r / ST) & 1))) break;
+            const Rec w = rec[st];
+            if (w.flags & R_Q) {
+                // every S of the piece before has been issued
+                if (piece >= 0 && elect_one_sync()) umma_commit(&q_free[piece & 1]);
+                __syncwarp();
+                piece++;
+                first = true;
+                if (!(ok = warp_wait(&q_ready[piece & 3], (piece >> 2) & 1))) break;
             }
-            vref = 0.f;                            // O is zero: the first block sets the scale
-            vinv = INFINITY;
-        }
-        if (w.blk >= 0) {
-            const uint32_t kb = smem_u32(ring + st * 2 * TILE), vbase = kb + TILE;
-            const int t0 = w.blk * KV8_BLOCK + p0;                 // this warp's first position
-            // S (positions x columns): 16 dims per thread and load, 4 steps each
-            float s[NT][4];
-#pragma unroll
-            for (int i = 0; i < NT; i++) s[i][0] = s[i][1] = s[i][2] = s[i][3] = 0.f;
-#pragma unroll
-            for (int h = 0; h < 2; h++) {
-                const uint4 ra = lds128(kb + k_off[h]), rb = lds128(kb + k_off[h] + 8 * 128);
-                const uint32_t a[4] = {ra.x, ra.y, ra.z, ra.w}, b[4] = {rb.x, rb.y, rb.z, rb.w};
-#pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    const uint32_t a0 = e4m3x2_to_f16x2(a[e] & 0xFFFFu), a2 = e4m3x2_to_f16x2(a[e] >> 16);
-                    const uint32_t a1 = e4m3x2_to_f16x2(b[e] & 0xFFFFu), a3 = e4m3x2_to_f16x2(b[e] >> 16);
-#pragma unroll
-                    for (int i = 0; i < NT; i++)
-                        mma_f16(s[i], a0, a1, a2, a3, qa[i][8 * h + 2 * e], qa[i][8 * h + 2 * e + 1]);
-                }
-            }
-            // online softmax; position of s[.][0], [1]: row g, of [2], [3]: row g + 8
-            const int ta = t0 + tok_of(g), tb = ta + 8;
-            bool grow = false;
-            const float kf = w.ks * kKv8ScaleLog2;
-#pragma unroll
-            for (int i = 0; i < NT; i++)
-#pragma unroll
-                for (int c = 0; c < 2; c++) {
-                    const float f = qs[i][c] * kf;
-                    s[i][c] = ta <= jlim[i][c] ? s[i][c] * f : -INFINITY;
-                    s[i][2 + c] = tb <= jlim[i][c] ? s[i][2 + c] * f : -INFINITY;
-                    grow |= s[i][c] > m[i][c] + kLazy || s[i][2 + c] > m[i][c] + kLazy;
-                }
-            if (__any_sync(0xFFFFFFFFu, grow)) {
-#pragma unroll
-                for (int i = 0; i < NT; i++)
-#pragma unroll
-                    for (int c = 0; c < 2; c++) {
-                        float x = fmaxf(m[i][c], fmaxf(s[i][c], s[i][2 + c]));
-                        x = fmaxf(x, __shfl_xor_sync(0xFFFFFFFFu, x, 4));
-                        x = fmaxf(x, __shfl_xor_sync(0xFFFFFFFFu, x, 8));
-                        x = fmaxf(x, __shfl_xor_sync(0xFFFFFFFFu, x, 16));
-                        const float corr = m[i][c] == x ? 1.f : ex2(m[i][c] - x);
-                        m[i][c] = x;
-                        l[i][c] *= corr;
-#pragma unroll
-                        for (int d = 0; d < 8; d++) { o[i][d][c] *= corr; o[i][d][2 + c] *= corr; }
-                    }
-            }
-            // V's block scale joins the weights as a ratio to the scale O is held in;
-            // O moves to the new scale when the ratio leaves [2^-6, 2^6] (FP16 weights
-            // reach 2^8 * 2^6)
-            float ratio = w.vs * vinv;
-            if (!(ratio >= 0.015625f && ratio <= 64.f)) {
-                const float move = vref / w.vs;
-#pragma unroll
-                for (int i = 0; i < NT; i++)
-#pragma unroll
-                    for (int d = 0; d < 8; d++)
-#pragma unroll
-                        for (int c = 0; c < 4; c++) o[i][d][c] *= move;
-                vref = w.vs;
-                vinv = 1.f / vref;
-                ratio = 1.f;
-            }
-            uint32_t pb[NT][2];
-#pragma unroll
-            for (int i = 0; i < NT; i++) {
-                float e[4];
-#pragma unroll
-                for (int c = 0; c < 4; c++) {
-                    const float mm = m[i][c & 1] == -INFINITY ? 0.f : m[i][c & 1];
-                    e[c] = ex2(s[i][c] - mm);
-                    l[i][c & 1] += e[c];
-                    e[c] *= ratio;
-                }
-                // rows g / g + 8 of P become the k pairs of the B fragment of column g
-                pb[i][0] = transpose8(pack_f16x2(e[0], e[1]));
-                pb[i][1] = transpose8(pack_f16x2(e[2], e[3]));
-            }
-            // O (dimensions x columns) += V^T P^T: positions va, vb (k = 2 tq, 2 tq + 1) and + 8
-            uint4 q4[4];
-            q4[0] = lds128(vbase + v_off[0]);
-            q4[1] = lds128(vbase + v_off[1]);
-            q4[2] = lds128(vbase + v_off[0] + 8 * 128);
-            q4[3] = lds128(vbase + v_off[1] + 8 * 128);
-            if (t0 + 16 > w.ctx) {
-                // codes behind the context may be anything, NaN too: a weight of 0 needs a 0
-                const int pv[4] = {va - p0, vb - p0, va - p0 + 8, vb - p0 + 8};
-#pragma unroll
-                for (int e = 0; e < 4; e++)
-                    if (t0 + pv[e] >= w.ctx) q4[e] = make_uint4(0u, 0u, 0u, 0u);
-            }
-#pragma unroll
-            for (int e = 0; e < 4; e++) {
-                const uint32_t x0 = e == 0 ? q4[0].x : e == 1 ? q4[0].y : e == 2 ? q4[0].z : q4[0].w;
-                const uint32_t x1 = e == 0 ? q4[1].x : e == 1 ? q4[1].y : e == 2 ? q4[1].z : q4[1].w;
-                const uint32_t x2 = e == 0 ? q4[2].x : e == 1 ? q4[2].y : e == 2 ? q4[2].z : q4[2].w;
-                const uint32_t x3 = e == 0 ? q4[3].x : e == 1 ? q4[3].y : e == 2 ? q4[3].z : q4[3].w;
-                const uint32_t lo = __byte_perm(x0, x1, 0x5140), hi = __byte_perm(x0, x1, 0x7362);
-                const uint32_t lo8 = __byte_perm(x2, x3, 0x5140), hi8 = __byte_perm(x2, x3, 0x7362);
-#pragma unroll
-                for (int half = 0; half < 2; half++) {
-                    const uint32_t u = half ? hi : lo, v = half ? hi8 : lo8;
-                    const uint32_t a0 = e4m3x2_to_f16x2(u & 0xFFFFu), a1 = e4m3x2_to_f16x2(u >> 16);
-                    const uint32_t a2 = e4m3x2_to_f16x2(v & 0xFFFFu), a3 = e4m3x2_to_f16x2(v >> 16);
-#pragma unroll
-                    for (int i = 0; i < NT; i++)
-                        mma_f16(o[i][2 * e + half], a0, a1, a2, a3, pb[i][0], pb[i][1]);
-                }
-            }
-        }
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&empty[st]);
-        if (!(w.flags & R_LAST)) continue;
-
-        // ---------------- the piece ends: merge the four warps ----------------
-#pragma unroll
-        for (int i = 0; i < NT; i++)
-#pragma unroll
-            for (int c = 0; c < 2; c++) {
-#pragma unroll
-                for (int x = 4; x < 32; x <<= 1) l[i][c] += __shfl_xor_sync(0xFFFFFFFFu, l[i][c], x);
-                const int col = 8 * i + 2 * tq + c;
-                if (g == 0) { wm[warp][col] = m[i][c]; wl[warp][col] = l[i][c]; }
-                if (col < n_col) {
-                    float *d = wo + ((size_t)warp * n_col + col) * KV8_HD + 16 * g;
-#pragma unroll
-                    for (int x = 0; x < 8; x++)
-                        *(float2 *)(d + 2 * x) = make_float2(o[i][x][c], o[i][x][2 + c]);
-                }
-            }
-        if (lane == 0) wscale[warp] = vref;
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&merge[0]);
-        if (!__all_sync(0xFFFFFFFFu, mbar_wait(&merge[0], merged & 1))) return;
-        for (int i = threadIdx.x; i < n_col * KV8_HD; i += CW * 32) {
-            const int col = i >> 7, d = i & 127;
-            float M = -INFINITY;
-#pragma unroll
-            for (int x = 0; x < CW; x++) M = fmaxf(M, wm[x][col]);
-            float L = 0.f, O = 0.f;
-#pragma unroll
-            for (int x = 0; x < CW; x++) {
-                // a warp without positions has m = -inf and l = 0; NaN scores leave m and make l NaN
-                const float f = wm[x][col] == M ? 1.f : ex2(wm[x][col] - M);
-                L += wl[x][col] * f;
-                O += wo[((size_t)x * n_col + col) * KV8_HD + d] * (f * wscale[x]);
-            }
-            if (w.slot < 0) {
-                const size_t row = (size_t)w.s * p.L + (col >> 1);
-                // no position at all: zero
-                p.out[row * p.ldo + (2 * w.kvh + (col & 1)) * KV8_HD + d] =
-                    f32_to_bf16_rne(L == 0.f ? 0.f : O * (1.f / L));
+            if (w.blk[0] < 0) {
+                if (lane == 0) mbar_arrive(&empty[st]);
             } else {
-                float *part = p.part + (size_t)w.slot * n_col * (KV8_HD + 2);
-                part[col * KV8_HD + d] = O;
-                if (d == 0) {
-                    part[n_col * KV8_HD + 2 * col] = M;
-                    part[n_col * KV8_HD + 2 * col + 1] = L;
+                tc_fence_after();
+                const uint32_t q = aQ + (piece & 1) * NS * 128, k = aR + st * STAGE, d = tS + (t & 1) * NS;
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+                    if (elect_one_sync())
+                        umma_e4m3(d, umma_desc_sw128(k + i * 32), umma_desc_sw128(q + i * 32), id_s, i > 0 ? 1u : 0u);
+                if (elect_one_sync()) umma_commit(&s_full[t & 1]);
+                __syncwarp();
+                // P.V of the tile before, then this one is due
+                if (due && !(ok = issue_pv())) break;
+                t++;
+                due = true;
+                w_st = st;
+                w_half = w.blk[1] < 0;
+                w_first = first;
+                w_piece = piece;
+                first = false;
+            }
+            if (w.flags & R_END) break;
+        }
+        if (ok && due) issue_pv();
+        // all MMAs of this warp are done before TMEM is released
+        if (elect_one_sync()) umma_commit(&done);
+        __syncwarp();
+        warp_wait(&done, 0);
+    } else if (n_units > 0 && warp == 6) {
+        // ---------------- query parts: lane i takes dimensions 4 i .. 4 i + 3 ----------------
+        int piece = -1;
+        for (int r = 0;; r++) {
+            const int st = r % ST;
+            if (!warp_wait(&full[st], (r / ST) & 1)) break;
+            const int flags = rec[st].flags;
+            if (flags & R_Q) {
+                piece++;
+                // the buffer's last piece but one has been multiplied
+                if (piece >= 2 && !warp_wait(&q_free[piece & 1], ((piece >> 1) - 1) & 1)) break;
+                uint8_t *dst = sQ + (piece & 1) * NS * 128;
+#pragma unroll 2
+                for (int c = 0; c < 2 * p.L; c++) {
+                    const uint2 x2 = *(const uint2 *)(sraw + (st * p.L) * 512 + c * 256 + lane * 8);
+                    uint32_t am = max(max(x2.x & 0x7FFFu, x2.x >> 16 & 0x7FFFu), max(x2.y & 0x7FFFu, x2.y >> 16 & 0x7FFFu));
+                    am = __reduce_max_sync(0xFFFFFFFFu, am);
+                    // the row's largest magnitude to [128, 256)
+                    const int e = min(max((int)(am >> 7), 8), 254);
+                    const float f = __uint_as_float((uint32_t)(261 - e) << 23);
+                    float x[4] = {__uint_as_float(x2.x << 16), __uint_as_float(x2.x & 0xFFFF0000u),
+                                  __uint_as_float(x2.y << 16), __uint_as_float(x2.y & 0xFFFF0000u)};
+                    uint32_t hi[2], lo[2];
+#pragma unroll
+                    for (int k = 0; k < 4; k++) x[k] = fabsf(x[k]) == INFINITY ? NAN : x[k] * f;   // e4m3 has no infinity
+#pragma unroll
+                    for (int k = 0; k < 2; k++) {
+                        hi[k] = f32x2_to_e4m3x2(x[2 * k], x[2 * k + 1]);
+                        const float2 h = e4m3x2_to_f32x2(hi[k]);
+                        lo[k] = f32x2_to_e4m3x2((x[2 * k] - h.x) * 16.f, (x[2 * k + 1] - h.y) * 16.f);
+                    }
+                    *(uint32_t *)(dst + sw(2 * c, 4 * lane)) = hi[0] | hi[1] << 16;
+                    *(uint32_t *)(dst + sw(2 * c + 1, 4 * lane)) = lo[0] | lo[1] << 16;
+                    if (lane == 0) q_scale[piece & 3][c] = __uint_as_float((uint32_t)max(e - 7, 1) << 23);
+                }
+                fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&q_ready[piece & 3]);
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&empty[st]);
+            if (flags & R_END) break;
+        }
+    } else if (n_units > 0) {
+        // ---------------- softmax and output (warps 2-5) ----------------
+        const int qw = warp & 3, row = qw * 32 + lane, half = row >> 6;
+        const uint32_t lane_off = (uint32_t)(qw * 32) << 16;
+        int t = 0, piece = -1, tiles = 0, bars = 0, ends = 0;      // tiles done; pieces with tiles; this piece's tiles
+        float m[NC], l[NC], qf[NC] = {}, vref = 0.f;
+        bool dead = false;
+        // All four warps pass here together, also when one's wait ran out: then all leave.
+        auto meet = [&](bool mine) -> bool {
+            if (lane == 0) xdead[bars & 1][qw] = mine;
+            named_bar_sync(1, 128);
+            const int *d = xdead[bars & 1];
+            bars++;
+            return d[0] | d[1] | d[2] | d[3];
+        };
+        for (int r = 0;; r++) {
+            const int st = r % ST;
+            dead = dead || !warp_wait(&full[st], (r / ST) & 1);
+            const Rec w = rec[st];
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&empty[st]);
+            if (w.flags & R_FIRST) {
+                tiles = 0;
+                vref = 0.f;
+                ends++;
+#pragma unroll
+                for (int c = 0; c < NC; c++) { m[c] = -INFINITY; l[c] = 0.f; }
+            }
+            if (!dead && (w.flags & R_Q)) {
+                piece++;
+                dead = !warp_wait(&q_ready[piece & 3], (piece >> 2) & 1);
+#pragma unroll
+                for (int c = 0; c < NC; c++) qf[c] = c < 2 * p.L ? q_scale[piece & 3][c] : 0.f;
+            }
+            if (dead || w.blk[0] >= 0) {
+                const uint32_t ts = tS + lane_off + (t & 1) * NS, to = tO + lane_off + (piece & 1) * NP;
+                const int blk = half ? w.blk[1] : w.blk[0], pos = blk * KV8_BLOCK + (row & 63);
+                const float kf = (half ? w.ks[1] : w.ks[0]) * kKv8ScaleLog2;
+                float s[NC];
+                if (!dead) dead = !warp_wait(&s_full[t & 1], (t >> 1) & 1);
+                if (!dead) {
+                    uint32_t v[4 * LT];
+                    tc_fence_after();
+                    load_s<LT>(ts, v);
+                    const int lim = blk < 0 ? -1 : w.ctx - p.L;     // last position of token j: lim + j
+#pragma unroll
+                    for (int c = 0; c < NC; c++) {
+                        const float x = fmaf(__uint_as_float(v[2 * c + 1]), 0.0625f, __uint_as_float(v[2 * c]));
+                        const bool see = blk >= 0 && pos <= lim + c / 2 && c < 2 * p.L;
+                        s[c] = see ? x * qf[c] * kf : -INFINITY;
+                        const float mx = warp_max(s[c]);
+                        if (lane == 0) xmax[bars & 1][qw][c] = mx;
+                    }
+                }
+                const float (*xm)[NC] = xmax[bars & 1];
+                if (meet(dead)) break;
+                // the tile's maximum, and V's scale: O moves when either changes
+                const float vmax = w.blk[1] < 0 ? w.vs[0] : fmaxf(w.vs[0], w.vs[1]);
+                const bool moved = !(vmax <= vref && vmax * 16.f >= vref);
+                const float vmove = moved && tiles ? vref / vmax : 1.f;
+                float corr[NC];
+                bool grow = moved;
+#pragma unroll
+                for (int c = 0; c < NC; c++) {
+                    const float x = fmaxf(fmaxf(xm[0][c], xm[1][c]), fmaxf(xm[2][c], xm[3][c]));
+                    corr[c] = 1.f;
+                    if (x > m[c]) {
+                        corr[c] = ex2(m[c] - x);
+                        m[c] = x;
+                        l[c] *= corr[c];
+                        grow = true;
+                    }
+                }
+                if (moved) vref = vmax;
+                bool alive = true;
+                if (grow && tiles) {                               // warp-uniform
+                    // O holds the tiles before: P.V of the last one must have ended
+                    alive = warp_wait(&pv_done[(t - 1) & 1], ((t - 1) >> 1) & 1);
+                    if (alive) {
+                        uint32_t o[o_regs<LT>()];
+                        tc_fence_after();
+                        load_o<LT>(to, o);
+#pragma unroll
+                        for (int c = 0; c < NC; c++)
+#pragma unroll
+                            for (int k = 0; k < 3; k++)
+                                o[3 * c + k] = __float_as_uint(__uint_as_float(o[3 * c + k]) * (corr[c] * vmove));
+                        store_o<LT>(to, o);
+                    }
+                }
+                // this buffer of P was read by P.V of two tiles ago
+                if (alive && t >= 2) alive = warp_wait(&pv_done[t & 1], ((t - 2) >> 1) & 1);
+                if (alive) {
+                    uint8_t *dst = sP + (t & 1) * NP * 128;
+                    const float ratio = 256.f * ((half ? w.vs[1] : w.vs[0]) / vref);
+#pragma unroll
+                    for (int c = 0; c < NC; c += 2) {
+                        float a = ex2(s[c] - (m[c] == -INFINITY ? 0.f : m[c]));
+                        float b = ex2(s[c + 1] - (m[c + 1] == -INFINITY ? 0.f : m[c + 1]));
+                        l[c] += a;
+                        l[c + 1] += b;
+                        a = blk < 0 ? 0.f : a * ratio;
+                        b = blk < 0 ? 0.f : b * ratio;
+#pragma unroll
+                        for (int k = 0; k < 3; k++) {
+                            const uint32_t e = f32x2_to_e4m3x2(a, b);
+                            dst[sw(3 * c + k, row)] = (uint8_t)e;
+                            dst[sw(3 * c + 3 + k, row)] = (uint8_t)(e >> 8);
+                            const float2 f = e4m3x2_to_f32x2(e);
+                            a = (a - f.x) * 16.f;
+                            b = (b - f.y) * 16.f;
+                        }
+                    }
+                    // codes of V behind the context may be anything, NaN too: a weight of 0 needs a 0
+                    if (blk >= 0 && pos >= w.ctx) {
+                        uint4 *z = (uint4 *)(ring + st * STAGE + 2 * BLK + row * 128);
+#pragma unroll
+                        for (int k = 0; k < 8; k++) z[k] = make_uint4(0u, 0u, 0u, 0u);
+                    }
+                    fence_proxy_async_smem();
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&p_full[t & 1]);
+                }
+                dead = !alive;                                     // leaves at the next meeting
+                t++;
+                tiles++;
+            }
+            if (!(w.flags & R_LAST)) continue;
+
+            // ---------------- the piece ends ----------------
+            const uint32_t to = tO + lane_off + (piece & 1) * NP;
+            uint32_t o[o_regs<LT>()];
+#pragma unroll
+            for (int c = 0; c < o_regs<LT>(); c++) o[c] = 0u;
+#pragma unroll
+            for (int c = 0; c < NC; c++) {
+                float x = l[c];
+#pragma unroll
+                for (int k = 16; k > 0; k >>= 1) x += __shfl_xor_sync(0xFFFFFFFFu, x, k);
+                if (lane == 0) xsum[ends & 1][qw][c] = x;
+            }
+            if (tiles && !dead) {
+                dead = !warp_wait(&pv_done[(t - 1) & 1], ((t - 1) >> 1) & 1);
+                if (!dead) {
+                    tc_fence_after();
+                    load_o<LT>(to, o);
+                    tc_fence_before();
                 }
             }
+            __syncwarp();
+            if (tiles && lane == 0) mbar_arrive(&o_free[piece & 1]);
+            if (meet(dead)) break;
+            const float (*xs)[NC] = xsum[ends & 1];
+#pragma unroll
+            for (int c = 0; c < NC; c++) {
+                if (c >= 2 * p.L) break;
+                const float L = (xs[0][c] + xs[1][c]) + (xs[2][c] + xs[3][c]);
+                const float O = fmaf(fmaf(__uint_as_float(o[3 * c + 2]), 0.0625f, __uint_as_float(o[3 * c + 1])), 0.0625f,
+                                     __uint_as_float(o[3 * c])) * (vref * 0.00390625f);
+                if (w.slot < 0) {
+                    const size_t orow = (size_t)w.s * p.L + (c >> 1);
+                    // no position at all: zero
+                    p.out[orow * p.ldo + (2 * w.kvh + (c & 1)) * KV8_HD + row] =
+                        f32_to_bf16_rne(L == 0.f ? 0.f : O * (1.f / L));
+                } else {
+                    float *part = p.part + (size_t)w.slot * (2 * p.L) * (KV8_HD + 2);
+                    part[c * KV8_HD + row] = O;
+                    if (row == 0) {
+                        part[2 * p.L * KV8_HD + 2 * c] = m[c];
+                        part[2 * p.L * KV8_HD + 2 * c + 1] = L;
+                    }
+                }
+            }
+            if (w.flags & R_END) break;
         }
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&merge[1]);
-        if (!__all_sync(0xFFFFFFFFu, mbar_wait(&merge[1], merged & 1))) return;
-        merged++;
-        if (w.flags & R_END) return;
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 1) {
+        tc_fence_after();
+        tmem_dealloc(tmem, tmem_cols<LT>());
     }
 }
 
@@ -567,7 +766,7 @@ __global__ void __launch_bounds__(CMB_WARPS * 32) kv8_combine_kernel(const Kv8At
         return u1;
     }, &cur);
     if (c >= n - 1) return;
-    const int kvh = (int)(cur.x / cur.upp), j = (int)(cur.x % cur.upp);
+    const int kvh = cur.x / cur.upp, j = cur.x - kvh * cur.upp;
     const long long first = u1 - j;                            // the pair's first unit
     if (j == 0 || first < u0) return;                          // no pair crosses, or it began earlier
     const int pieces = Cut(tot, n_max).run_of(first + cur.upp - 1) - c + 1;
@@ -621,36 +820,34 @@ __global__ void __launch_bounds__(CMB_WARPS * 32) kv8_combine_kernel(const Kv8At
     }
 }
 
-template <int NT>
-constexpr int smem_bytes(int L) {
-    return stages<NT>() * (2 * TILE + L * 512) + CW * 2 * L * KV8_HD * 4 + 1024;
-}
-
 constexpr int kSms = 148;
-// CTAs that share an SM: shared memory (227 KB, 1 KB of it taken per CTA and about 1 KB static)
-template <int NT>
+// CTAs that share an SM: by shared memory (228 KB, 2 KB a CTA of it reserved or
+// static) and TMEM (512 columns)
+template <int LT>
 int ctas(int L) {
-    const int per_sm = 232448 / (smem_bytes<NT>(L) + 2560);
-    return kSms * (per_sm < 1 ? 1 : per_sm > 3 ? 3 : per_sm);
+    const int per_sm = 233472 / (smem_bytes<LT>(L, stages<LT>()) + 2048);
+    const int by_tmem = 512 / tmem_cols<LT>();
+    return kSms * (per_sm < 1 ? 1 : per_sm < by_tmem ? per_sm : by_tmem);
 }
-int max_ctas(int L) { return L <= 4 ? ctas<1>(L) : ctas<2>(L); }
+int max_ctas(int L) { return L == 1 ? ctas<1>(L) : L <= 4 ? ctas<4>(L) : ctas<8>(L); }
 
-template <int NT>
+template <int LT>
 int launch(cudaStream_t st, const CUtensorMap &tk, const CUtensorMap &tv, const Kv8AttnArgs &a) {
+    constexpr int ST = stages<LT>();
     static bool attr[64];
     int dev = 0;
     N550_CUDA_TRY(cudaGetDevice(&dev));
     if (dev >= 0 && dev < 64 && !attr[dev]) {
-        N550_CUDA_TRY(cudaFuncSetAttribute(kv8_attn_kernel<NT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                           smem_bytes<NT>(4 * NT)));
+        N550_CUDA_TRY(cudaFuncSetAttribute(kv8_attn_kernel<LT, ST>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                           smem_bytes<LT>(LT, ST)));
         attr[dev] = true;
     }
-    const size_t smem = smem_bytes<NT>(a.L);
+    const size_t smem = smem_bytes<LT>(a.L, ST);
     Lay lay{};
     const long long pairs = (long long)a.n_seqs * KV8_NKV;
     if (!a.part) {
         lay.kind = LAY_PAIR;
-        N550_CUDA_TRY(launch_k(kv8_attn_kernel<NT>, dim3((unsigned)pairs), THREADS, smem, st, tk, tv, a, lay));
+        N550_CUDA_TRY(launch_k(kv8_attn_kernel<LT, ST>, dim3((unsigned)pairs), THREADS, smem, st, tk, tv, a, lay));
         N550_LAUNCH_CHECK();
         return N550_OK;
     }
@@ -663,8 +860,8 @@ int launch(cudaStream_t st, const CUtensorMap &tk, const CUtensorMap &tv, const 
     }
     // no more runs than there can be (the kernels cut by the units there are)
     const long long most = (pairs * (lay.kind == LAY_EVEN ? lay.upp : a.c.nb) + kMinRun - 1) / kMinRun;
-    const int n = (int)(most < ctas<NT>(a.L) ? most : ctas<NT>(a.L));
-    N550_CUDA_TRY(launch_k(kv8_attn_kernel<NT>, dim3(n), THREADS, smem, st, tk, tv, a, lay));
+    const int n = (int)(most < ctas<LT>(a.L) ? most : ctas<LT>(a.L));
+    N550_CUDA_TRY(launch_k(kv8_attn_kernel<LT, ST>, dim3(n), THREADS, smem, st, tk, tv, a, lay));
     N550_LAUNCH_CHECK();
     if (n > 1) {
         N550_CUDA_TRY(launch_k(kv8_combine_kernel, dim3(n - 1), CMB_WARPS * 32, 0, st, a, lay, n));
@@ -687,7 +884,7 @@ int launch_kv8_attn(cudaStream_t st, const Kv8AttnArgs &a) {
     int rc = tmap_bf16_sw128_3d(&tk, a.c.k, a.c.max_len, 64, 64, KV8_BLOCK, planes, (uint64_t)a.c.max_len * 64);
     if (!rc) rc = tmap_bf16_sw128_3d(&tv, a.c.v, a.c.max_len, 64, 64, KV8_BLOCK, planes, (uint64_t)a.c.max_len * 64);
     if (rc) return rc;
-    return a.L <= 4 ? launch<1>(st, tk, tv, a) : launch<2>(st, tk, tv, a);
+    return a.L == 1 ? launch<1>(st, tk, tv, a) : a.L <= 4 ? launch<4>(st, tk, tv, a) : launch<8>(st, tk, tv, a);
 }
 
 }  // namespace n550
