@@ -27,9 +27,10 @@
 //   warp 0     producer: walks the run, 32 blocks a batch (one per lane: list entry,
 //              slot, scales), and fills a ring of 32 KB stages
 //   warp 1     issues the MMAs, S of the next tile before P.V of this one
-//   warp 6     splits the queries of each new pair
 //   warps 2-5  softmax, a thread per position, and the output, a thread per
-//              dimension; they agree on a tile's maximum through shared memory
+//              dimension; they agree on a tile's maximum through shared memory.
+//              With more query tokens more such groups share the columns.
+//   last warp  splits the queries of each new pair
 #include <cuda.h>
 
 #include "kv8.h"
@@ -39,7 +40,6 @@
 namespace n550 {
 namespace {
 
-constexpr int THREADS = 224;                    // 7 warps
 constexpr int BLK = KV8_BLOCK * KV8_HD;         // 8 KB of K or V codes
 constexpr int STAGE = 4 * BLK;                  // K of two blocks | V of two blocks
 
@@ -66,8 +66,20 @@ template <int LT> constexpr int tmem_cols() {
     return 2 * (s_cols<LT>() + p_cols<LT>()) <= 64 ? 64 : 2 * (s_cols<LT>() + p_cols<LT>()) <= 128 ? 128 : 256;
 }
 template <int LT> constexpr int op_bytes() { return 2 * 128 * (s_cols<LT>() + p_cols<LT>()); }
-template <int LT> constexpr int smem_bytes(int L, int st) { return st * (STAGE + L * 512) + op_bytes<LT>() + 1024; }
-template <int LT> constexpr int stages() { return LT == 1 ? 2 : 5; }
+// Ring stages and CTAs per SM: HBM latency takes about 4000 cycles under load and a
+// tile's way from full to empty about 2000, so an SM needs some 150 KB of ring; 3 x 2
+// stages beat 2 x 3 (256 x 1152 decode 107 against 113 us), because the softmax of
+// one CTA alone keeps 13 bytes per cycle of the 23 that HBM gives an SM.
+template <int LT> constexpr int stages() { return LT == 8 ? 4 : 2; }
+template <int LT> constexpr int per_sm() { return LT == 1 ? 3 : LT == 4 ? 2 : 1; }
+template <int LT> constexpr int smem_bytes(int L) { return stages<LT>() * (STAGE + L * 512) + op_bytes<LT>() + 1024; }
+template <int LT> constexpr int groups() { return LT == 1 ? 1 : LT / 2; }       // of four softmax warps
+template <int LT> constexpr int threads() { return (3 + 4 * groups<LT>()) * 32; }
+
+// The pair that a run leaves to the merge: its pieces are in runs c .. c + n - 1.
+struct Cross {
+    int s, kvh, n, slot;                        // n = 0: none; slot: the first piece's (2 c or 2 c + 1)
+};
 
 __device__ __forceinline__ float ex2(float x) {
     float y;
@@ -104,34 +116,25 @@ __device__ __forceinline__ void tmem_st_x8(uint32_t taddr, const uint32_t *r) {
                  ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
                  : "memory");
 }
-// The S columns (4 LT) and O columns (6 LT, rounded up to whole loads) of this
-// thread's TMEM lane.
-template <int LT>
-__device__ __forceinline__ void load_s(uint32_t t, uint32_t (&r)[4 * LT]) {
-    if constexpr (LT == 1) tmem_ld_x4(t, r);
-    else if constexpr (LT == 4) tmem_ld_32x32b_x16(t, r);
-    else tmem_ld_32x32b_x32(t, r);
+__device__ __forceinline__ void tmem_st_x4(uint32_t taddr, const uint32_t *r) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1,%2,%3,%4};"
+                 ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]) : "memory");
+}
+// N columns (2 to 24, loads rounded up to a multiple of 4) of this thread's TMEM lane.
+template <int N>
+__device__ __forceinline__ void load_cols(uint32_t t, uint32_t (&r)[(N + 3) / 4 * 4]) {
+    int at = 0;
+    if constexpr (N >= 16) { tmem_ld_32x32b_x16(t, *reinterpret_cast<uint32_t(*)[16]>(&r[0])); at = 16; }
+    if constexpr (N % 16 > 4) { tmem_ld_x8(t + at, r + at); at += 8; }
+    if constexpr (N % 8 > 0 && N % 8 <= 4) tmem_ld_x4(t + at, r + at);
     tmem_ld_wait();
 }
-template <int LT> constexpr int o_regs() { return LT == 1 ? 8 : LT == 4 ? 32 : 48; }
-template <int LT>
-__device__ __forceinline__ void load_o(uint32_t t, uint32_t (&r)[o_regs<LT>()]) {
-    if constexpr (LT == 1) tmem_ld_x8(t, r);
-    else if constexpr (LT == 4) tmem_ld_32x32b_x32(t, r);
-    else {
-        tmem_ld_32x32b_x32(t, *reinterpret_cast<uint32_t(*)[32]>(&r[0]));
-        tmem_ld_32x32b_x16(t + 32, *reinterpret_cast<uint32_t(*)[16]>(&r[32]));
-    }
-    tmem_ld_wait();
-}
-template <int LT>
-__device__ __forceinline__ void store_o(uint32_t t, const uint32_t (&r)[o_regs<LT>()]) {
-    if constexpr (LT == 1) tmem_st_x8(t, r);
-    else if constexpr (LT == 4) tmem_st_32x32b_x32(t, r);
-    else {
-        tmem_st_32x32b_x32(t, *reinterpret_cast<const uint32_t(*)[32]>(&r[0]));
-        tmem_st_32x32b_x16(t + 32, *reinterpret_cast<const uint32_t(*)[16]>(&r[32]));
-    }
+template <int N>
+__device__ __forceinline__ void store_cols(uint32_t t, const uint32_t (&r)[(N + 3) / 4 * 4]) {
+    int at = 0;
+    if constexpr (N >= 16) { tmem_st_32x32b_x16(t, *reinterpret_cast<const uint32_t(*)[16]>(&r[0])); at = 16; }
+    if constexpr (N % 16 > 4) { tmem_st_x8(t + at, r + at); at += 8; }
+    if constexpr (N % 8 > 0 && N % 8 <= 4) tmem_st_x4(t + at, r + at);
     tmem_st_wait();
 }
 
@@ -159,9 +162,8 @@ __device__ __forceinline__ uint32_t sw(int n, int k) { return n * 128 + ((((k >>
 
 // Units (blocks; one empty unit for an empty context) of a pair of sequence s.
 __device__ __forceinline__ int seq_ctx(const Kv8AttnArgs &p, int s) {
-    const int slot = __ldcg(p.seq_ids + s);
-    if (!p.pos) return kv8_ctx(p.c, slot, p.pos0 + p.L - 1);
-    return kv8_ctx(p.c, slot, __ldcg(p.pos + s));
+    const int slot = p.seq_ids[s], pos = p.pos ? p.pos[s] : p.pos0 + p.L - 1;   // through L1: every CTA reads them all
+    return kv8_ctx(p.c, slot, pos);
 }
 __device__ __forceinline__ int ctx_blocks(int ctx) { return max(1, (ctx + KV8_BLOCK - 1) / KV8_BLOCK); }
 
@@ -170,70 +172,76 @@ struct Cur {
     int s, upp, ctx, x;
 };
 
-// All threads of the CTA. Returns the total number of units and places *cur at
-// unit first(total): LAY_RAGGED needs the prefix sums of the sequences' block
-// counts, which every CTA forms itself (n_seqs loads, two barriers).
+// One converged warp. Returns the total number of units and places *cur at unit
+// first(total). LAY_RAGGED needs the prefix sums of the sequences' block counts,
+// which every CTA forms itself: 256 sequences take one round of loads.
 template <class First>
 __device__ __forceinline__ long long locate(const Kv8AttnArgs &p, const Lay lay, First first, Cur *cur) {
     if (lay.kind == LAY_EVEN) {
-        const long long total = (long long)lay.upp * KV8_NKV * p.n_seqs, u = first(total);
+        const long long per = (long long)lay.upp * KV8_NKV, total = per * p.n_seqs, u = first(total);
         if (u >= total) return total;
-        cur->s = (int)(u / ((long long)lay.upp * KV8_NKV));
-        cur->x = (int)(u - (long long)cur->s * lay.upp * KV8_NKV);
+        cur->s = total >> 31 ? (int)(u / per) : (int)((uint32_t)u / (uint32_t)per);
+        cur->x = (int)(u - cur->s * per);
         cur->upp = lay.upp;
         return total;
     }
-    constexpr int KEEP = 4;                      // contexts a thread keeps in registers (else it reads them again)
-    __shared__ long long wsum[32];
-    __shared__ Cur found;
-    const int nt = blockDim.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int per = (p.n_seqs + nt - 1) / nt, s0 = min(tid * per, p.n_seqs), s1 = min(s0 + per, p.n_seqs);
-    int kept[KEEP];
-    long long mine = 0;
+    // Rounds of 256 sequences, lane l holds l, 32 + l, .. of them: their sums by 32 find the
+    // group of 32 that holds the unit, a scan of that group the sequence. (The code
+    // runs once, from a cold instruction cache: eight unrolled scans cost 2000 cycles
+    // more, and a lane's loads from 8 consecutive sequences 3000.)
+    constexpr int ROUND = 8;
+    const int lane = threadIdx.x & 31;
+    int ctx[ROUND], sum[ROUND];
+    auto round = [&](int s0) -> int {            // returns the round's units
+        int all = 0;
 #pragma unroll
-    for (int i = 0; i < KEEP; i++) kept[i] = s0 + i < s1 ? seq_ctx(p, s0 + i) : 0;
+        for (int i = 0; i < ROUND; i++) ctx[i] = s0 + 32 * i + lane < p.n_seqs ? seq_ctx(p, s0 + 32 * i + lane) : -KV8_BLOCK;
 #pragma unroll
-    for (int i = 0; i < KEEP; i++) mine += s0 + i < s1 ? ctx_blocks(kept[i]) * KV8_NKV : 0;
-    for (int s = s0 + KEEP; s < s1; s++) mine += (long long)ctx_blocks(seq_ctx(p, s)) * KV8_NKV;
-    long long pre = mine;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const long long t = __shfl_up_sync(0xFFFFFFFFu, pre, o);
-        if (lane >= o) pre += t;
-    }
-    if (lane == 31) wsum[warp] = pre;
-    __syncthreads();
-    long long base = 0, total = 0;
-    for (int w = 0; w < nt / 32; w++) {
-        if (w < warp) base += wsum[w];
-        total += wsum[w];
-    }
-    const long long u = first(total);
-    pre += base - mine;                          // units before this thread's sequences
-    if (u >= pre && u < pre + mine) {
-        long long x = u - pre;
-        int s = s0, ctx = 0, n = 0;
-        bool hit = false;
-#pragma unroll
-        for (int i = 0; i < KEEP; i++)
-            if (!hit && s < s1) {
-                ctx = kept[i];
-                n = ctx_blocks(ctx);
-                hit = x < (long long)n * KV8_NKV;
-                if (!hit) { x -= (long long)n * KV8_NKV; s++; }
-            }
-        while (!hit) {
-            ctx = seq_ctx(p, s);
-            n = ctx_blocks(ctx);
-            hit = x < (long long)n * KV8_NKV;
-            if (!hit) { x -= (long long)n * KV8_NKV; s++; }
+        for (int i = 0; i < ROUND; i++) {
+            sum[i] = s0 + 32 * i < p.n_seqs ? __reduce_add_sync(0xFFFFFFFFu, ctx[i] < 0 ? 0 : ctx_blocks(ctx[i])) * KV8_NKV : 0;
+            all += sum[i];
         }
-        found.s = s; found.upp = n; found.ctx = ctx; found.x = (int)x;
+        return all;
+    };
+    long long total = 0;
+    for (int s0 = 0; s0 < p.n_seqs; s0 += 32 * ROUND) total += round(s0);
+    const long long u = first(total);
+    if (u >= total) return total;
+    int s0 = 0;
+    long long base = 0;                          // units before the round that holds u
+    if (p.n_seqs > 32 * ROUND)
+        for (;; s0 += 32 * ROUND) {
+            const int n = round(s0);
+            if (u < base + n) break;
+            base += n;
+        }
+    int x = (int)(u - base), mine = ctx[0];
+    bool found = x < sum[0];
+#pragma unroll
+    for (int i = 1; i < ROUND; i++)
+        if (!found) {
+            x -= sum[i - 1];
+            s0 += 32;
+            mine = ctx[i];
+            found = x < sum[i];
+        }
+    const int n = mine < 0 ? 0 : ctx_blocks(mine) * KV8_NKV;
+    int end = n;
+#pragma unroll 1
+    for (int o = 1; o < 32; o <<= 1) {
+        const int t = __shfl_up_sync(0xFFFFFFFFu, end, o);
+        if (lane >= o) end += t;
     }
-    __syncthreads();
-    if (u < total) *cur = found;
+    const int l = __ffs(__ballot_sync(0xFFFFFFFFu, x < end)) - 1;
+    cur->s = s0 + l;
+    cur->ctx = __shfl_sync(0xFFFFFFFFu, mine, l);
+    cur->x = x - __shfl_sync(0xFFFFFFFFu, end - n, l);
+    cur->upp = ctx_blocks(cur->ctx);
     return total;
 }
+
+// Floats before the partials of n runs: the runs' Cross records.
+__host__ __device__ __forceinline__ size_t part_base(int n) { return (size_t)n * (sizeof(Cross) / sizeof(float)); }
 
 // `total` units cut into n runs that differ by at most one unit: as many runs as
 // CTAs, but none shorter than kMinRun units (a run's blocks are in flight
@@ -245,7 +253,7 @@ struct Cut {
     __device__ __forceinline__ Cut(long long total, int n_max) {
         const long long most = (total + kMinRun - 1) / kMinRun;
         n = most < n_max ? (int)most : n_max;
-        q = total / n;
+        q = total >> 31 ? total / n : (long long)((uint32_t)total / (uint32_t)n);
         r = (int)(total - q * n);
     }
     __device__ __forceinline__ long long start(int c) const { return q * c + min(c, r); }
@@ -255,11 +263,11 @@ struct Cut {
     }
 };
 
-template <int LT, int ST>
-__global__ void __launch_bounds__(THREADS)
+template <int LT>
+__global__ void __launch_bounds__(threads<LT>(), per_sm<LT>())
 kv8_attn_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
                 const Kv8AttnArgs p, const Lay lay) {
-    constexpr int NS = s_cols<LT>(), NP = p_cols<LT>(), NC = 2 * LT;
+    constexpr int NS = s_cols<LT>(), NP = p_cols<LT>(), NC = 2 * LT, G = groups<LT>(), ST = stages<LT>();
     extern __shared__ uint8_t dsm[];
     uint8_t *ring = (uint8_t *)(((uintptr_t)dsm + 1023) & ~(uintptr_t)1023);      // [ST][STAGE]
     uint8_t *sQ = ring + ST * STAGE;                                               // [2][NS][128]
@@ -269,20 +277,20 @@ kv8_attn_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
     __shared__ __align__(8) uint64_t full[ST], empty[ST], q_ready[4], q_free[2], s_full[2], p_full[2], pv_done[2], o_free[2], done;
     __shared__ float q_scale[4][NC];            // power of two of each query row, by piece modulo 4
     __shared__ float xmax[2][4][NC], xsum[2][4][NC];
-    __shared__ int xdead[2][4];
+    __shared__ int xdead[G][2][4];
     __shared__ uint32_t tmem_slot;
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
-        for (int i = 0; i < ST; i++) { mbar_init(&full[i], 1); mbar_init(&empty[i], 6); }
+        for (int i = 0; i < ST; i++) { mbar_init(&full[i], 1); mbar_init(&empty[i], 2 + 4 * G); }
         for (int i = 0; i < 2; i++) {
             mbar_init(&q_ready[i], 1);
             mbar_init(&q_ready[2 + i], 1);
             mbar_init(&q_free[i], 1);
             mbar_init(&s_full[i], 1);
-            mbar_init(&p_full[i], 4);
+            mbar_init(&p_full[i], 4 * G);
             mbar_init(&pv_done[i], 1);
-            mbar_init(&o_free[i], 4);
+            mbar_init(&o_free[i], 4 * G);
         }
         mbar_init(&done, 1);
         fence_mbar_init();
@@ -294,32 +302,37 @@ kv8_attn_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = tmem_slot, tS = tmem, tO = tmem + 2 * NS;
-    // block lists, positions, scales, codes and queries all come from earlier kernels
     dep_launch();
-    dep_wait();
-    Cur cur{};
-    int n_units;
-    if (lay.kind == LAY_PAIR) {
-        cur.s = blockIdx.x / KV8_NKV;
-        cur.ctx = seq_ctx(p, cur.s);
-        cur.upp = p.n_select >= 0 ? max(1, p.n_select) : ctx_blocks(cur.ctx);
-        cur.x = (int)(blockIdx.x % KV8_NKV) * cur.upp;
-        n_units = cur.upp;
-    } else {
-        long long u0 = 0, u1 = 0;
-        locate(p, lay, [&](long long total) {
-            const Cut cut(total, gridDim.x);
-            u0 = u1 = total;
-            if ((int)blockIdx.x < cut.n) {
-                u0 = cut.start(blockIdx.x);
-                u1 = cut.start(blockIdx.x + 1);
-            }
-            return u0;
-        }, &cur);
-        n_units = (int)(u1 - u0);
-    }
-
-    if (n_units > 0 && warp == 0) {
+    if (warp == 0) {
+        // Block lists, positions, scales, codes and queries all come from earlier kernels;
+        // what every CTA reads first may be on its way to L2 before they end.
+        if (lay.kind == LAY_RAGGED && lane * 32 < p.n_seqs) {
+            asm volatile("prefetch.global.L2 [%0];" ::"l"(p.pos + lane * 32));
+            asm volatile("prefetch.global.L2 [%0];" ::"l"(p.seq_ids + lane * 32));
+        }
+        dep_wait();
+        Cur cur{};
+        int n_units;
+        long long u0 = 0, total = 0;
+        if (lay.kind == LAY_PAIR) {
+            cur.s = blockIdx.x / KV8_NKV;
+            cur.ctx = seq_ctx(p, cur.s);
+            cur.upp = p.n_select >= 0 ? max(1, p.n_select) : ctx_blocks(cur.ctx);
+            cur.x = (int)(blockIdx.x % KV8_NKV) * cur.upp;
+            n_units = cur.upp;
+        } else {
+            long long u1 = 0;
+            total = locate(p, lay, [&](long long all) {
+                const Cut cut(all, gridDim.x);
+                u0 = u1 = all;
+                if ((int)blockIdx.x < cut.n) {
+                    u0 = cut.start(blockIdx.x);
+                    u1 = cut.start(blockIdx.x + 1);
+                }
+                return u0;
+            }, &cur);
+            n_units = (int)(u1 - u0);
+        }
         // ---------------- producer: lane i takes unit 32 k + i ----------------
         bool seen = false;                       // the piece that reaches into this batch had a tile
         // The records of the batch of 32 units at `base` (the next one is read while the
@@ -345,7 +358,7 @@ kv8_attn_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
             me.blk[0] = me.blk[1] = -1;
             plane = 0;
             if (i < n_units) {
-                const int slot = __ldcg(p.seq_ids + c.s);
+                const int slot = p.seq_ids[c.s];
                 if (lay.kind == LAY_EVEN) c.ctx = seq_ctx(p, c.s);
                 const int kvh = c.x / c.upp, j = c.x - kvh * c.upp;
                 int b = j;
@@ -361,8 +374,24 @@ kv8_attn_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
                 const bool head = i - j < 0;                     // the pair begins before this run
                 const bool tail = i - j + c.upp > n_units;       // and here ends behind it
                 me.slot = head || tail ? 2 * (int)blockIdx.x + (i - j > 0) : -1;
+                // tell the merge about the pair that crosses this run's end, if it begins in it
+                if (i == n_units - 1 && lay.kind != LAY_PAIR) {
+                    Cross x{};
+                    if (tail && !head) {
+                        x.s = c.s;
+                        x.kvh = kvh;
+                        x.n = Cut(total, gridDim.x).run_of(u0 + (i - j) + c.upp - 1) - (int)blockIdx.x + 1;
+                        x.slot = me.slot;
+                    }
+                    ((Cross *)p.part)[blockIdx.x] = x;
+                }
                 if (b >= 0) {
                     plane = (int)p.c.plane(slot, kvh);
+                    // the ring's first blocks need not wait for the scales
+                    if (i < 2 * ST) {
+                        tma_prefetch_3d(&tmK, 0, b * KV8_BLOCK, plane);
+                        tma_prefetch_3d(&tmV, 0, b * KV8_BLOCK, plane);
+                    }
                     me.ks[0] = __ldcg(p.c.ks + (size_t)plane * p.c.nb + b);
                     me.vs[0] = __ldcg(p.c.vs + (size_t)plane * p.c.nb + b);
                 }
@@ -402,10 +431,19 @@ kv8_attn_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
         Rec me, nxt;
         int plane, nplane;
         uint32_t sends, nsends;
-        batch(0, me, plane, sends);
+        if (n_units > 0) {
+            batch(0, me, plane, sends);
+        } else {                                 // an empty run: one record says so
+            me = Rec{};
+            me.blk[0] = me.blk[1] = -1;
+            me.flags = R_END;
+            sends = 1;
+            plane = 0;
+            if (lane == 0) ((Cross *)p.part)[blockIdx.x] = Cross{};
+        }
         int r = 0;                               // records issued
         bool ok = true;
-        for (int base = 0; base < n_units && ok; base += 32) {
+        for (int base = 0; ok; base += 32) {
             bool more = false;
             for (; sends; sends &= sends - 1) {
                 const int l = __ffs(sends) - 1, st = r % ST;
@@ -446,7 +484,7 @@ kv8_attn_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
         if (lane == 0)
             for (int i = max(0, r - ST); i < r; i++) mbar_wait(&full[i % ST], (i / ST) & 1);
         __syncwarp();
-    } else if (n_units > 0 && warp == 1) {
+    } else if (warp == 1) {
         // ---------------- MMAs ----------------
         constexpr uint32_t id_s = idesc_e4m3(NS, 0), id_o = idesc_e4m3(NP, 1);
         const uint32_t aR = smem_u32(ring), aQ = smem_u32(sQ), aP = smem_u32(sP);
@@ -513,7 +551,7 @@ kv8_attn_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
         if (elect_one_sync()) umma_commit(&done);
         __syncwarp();
         warp_wait(&done, 0);
-    } else if (n_units > 0 && warp == 6) {
+    } else if (warp == 2 + 4 * G) {
         // ---------------- query parts: lane i takes dimensions 4 i .. 4 i + 3 ----------------
         int piece = -1;
         for (int r = 0;; r++) {
@@ -556,18 +594,21 @@ kv8_attn_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
             if (lane == 0) mbar_arrive(&empty[st]);
             if (flags & R_END) break;
         }
-    } else if (n_units > 0) {
-        // ---------------- softmax and output (warps 2-5) ----------------
+    } else {
+        dep_wait();                              // out and the workspace may be in use by earlier kernels
+        // ---------------- softmax and output: a group's columns c0 .. c0 + NG - 1 ----------------
+        constexpr int NG = NC / G;
+        const int grp = (warp - 2) >> 2, c0 = grp * NG, ng = min(NG, 2 * p.L - c0);     // ng <= 0: nothing to do but keep step
         const int qw = warp & 3, row = qw * 32 + lane, half = row >> 6;
         const uint32_t lane_off = (uint32_t)(qw * 32) << 16;
         int t = 0, piece = -1, tiles = 0, bars = 0, ends = 0;      // tiles done; pieces with tiles; this piece's tiles
-        float m[NC], l[NC], qf[NC] = {}, vref = 0.f;
+        float m[NG], l[NG], qf[NG] = {}, vref = 0.f;
         bool dead = false;
-        // All four warps pass here together, also when one's wait ran out: then all leave.
+        // A group's four warps pass here together, also when one's wait ran out: then all leave.
         auto meet = [&](bool mine) -> bool {
-            if (lane == 0) xdead[bars & 1][qw] = mine;
-            named_bar_sync(1, 128);
-            const int *d = xdead[bars & 1];
+            int *d = xdead[grp][bars & 1];
+            if (lane == 0) d[qw] = mine;
+            named_bar_sync(1 + grp, 128);
             bars++;
             return d[0] | d[1] | d[2] | d[3];
         };
@@ -582,32 +623,34 @@ kv8_attn_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
                 vref = 0.f;
                 ends++;
 #pragma unroll
-                for (int c = 0; c < NC; c++) { m[c] = -INFINITY; l[c] = 0.f; }
+                for (int c = 0; c < NG; c++) { m[c] = -INFINITY; l[c] = 0.f; }
             }
             if (!dead && (w.flags & R_Q)) {
                 piece++;
                 dead = !warp_wait(&q_ready[piece & 3], (piece >> 2) & 1);
 #pragma unroll
-                for (int c = 0; c < NC; c++) qf[c] = c < 2 * p.L ? q_scale[piece & 3][c] : 0.f;
+                for (int c = 0; c < NG; c++) qf[c] = c < ng ? q_scale[piece & 3][c0 + c] : 0.f;
             }
             if (dead || w.blk[0] >= 0) {
-                const uint32_t ts = tS + lane_off + (t & 1) * NS, to = tO + lane_off + (piece & 1) * NP;
+                const uint32_t ts = tS + lane_off + (t & 1) * NS + 2 * c0, to = tO + lane_off + (piece & 1) * NP + 3 * c0;
                 const int blk = half ? w.blk[1] : w.blk[0], pos = blk * KV8_BLOCK + (row & 63);
                 const float kf = (half ? w.ks[1] : w.ks[0]) * kKv8ScaleLog2;
-                float s[NC];
+                float s[NG];
                 if (!dead) dead = !warp_wait(&s_full[t & 1], (t >> 1) & 1);
                 if (!dead) {
-                    uint32_t v[4 * LT];
+                    uint32_t v[(2 * NG + 3) / 4 * 4];
                     tc_fence_after();
-                    load_s<LT>(ts, v);
-                    const int lim = blk < 0 ? -1 : w.ctx - p.L;     // last position of token j: lim + j
+                    load_cols<2 * NG>(ts, v);
+                    const int lim = blk < 0 ? -1 : w.ctx - p.L + c0 / 2;   // last position of this group's token j: lim + j
 #pragma unroll
-                    for (int c = 0; c < NC; c++) {
-                        const float x = fmaf(__uint_as_float(v[2 * c + 1]), 0.0625f, __uint_as_float(v[2 * c]));
-                        const bool see = blk >= 0 && pos <= lim + c / 2 && c < 2 * p.L;
-                        s[c] = see ? x * qf[c] * kf : -INFINITY;
-                        const float mx = warp_max(s[c]);
-                        if (lane == 0) xmax[bars & 1][qw][c] = mx;
+                    for (int c = 0; c < NG; c++) {
+                        s[c] = -INFINITY;
+                        if (c < ng) {
+                            const float x = fmaf(__uint_as_float(v[2 * c + 1]), 0.0625f, __uint_as_float(v[2 * c]));
+                            if (blk >= 0 && pos <= lim + c / 2) s[c] = x * qf[c] * kf;
+                            const float mx = warp_max(s[c]);
+                            if (lane == 0) xmax[bars & 1][qw][c0 + c] = mx;
+                        }
                     }
                 }
                 const float (*xm)[NC] = xmax[bars & 1];
@@ -616,17 +659,19 @@ kv8_attn_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
                 const float vmax = w.blk[1] < 0 ? w.vs[0] : fmaxf(w.vs[0], w.vs[1]);
                 const bool moved = !(vmax <= vref && vmax * 16.f >= vref);
                 const float vmove = moved && tiles ? vref / vmax : 1.f;
-                float corr[NC];
+                float corr[NG];
                 bool grow = moved;
 #pragma unroll
-                for (int c = 0; c < NC; c++) {
-                    const float x = fmaxf(fmaxf(xm[0][c], xm[1][c]), fmaxf(xm[2][c], xm[3][c]));
+                for (int c = 0; c < NG; c++) {
                     corr[c] = 1.f;
-                    if (x > m[c]) {
-                        corr[c] = ex2(m[c] - x);
-                        m[c] = x;
-                        l[c] *= corr[c];
-                        grow = true;
+                    if (c < ng) {
+                        const float x = fmaxf(fmaxf(xm[0][c0 + c], xm[1][c0 + c]), fmaxf(xm[2][c0 + c], xm[3][c0 + c]));
+                        if (x > m[c]) {
+                            corr[c] = ex2(m[c] - x);
+                            m[c] = x;
+                            l[c] *= corr[c];
+                            grow = true;
+                        }
                     }
                 }
                 if (moved) vref = vmax;
@@ -635,42 +680,43 @@ kv8_attn_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
                     // O holds the tiles before: P.V of the last one must have ended
                     alive = warp_wait(&pv_done[(t - 1) & 1], ((t - 1) >> 1) & 1);
                     if (alive) {
-                        uint32_t o[o_regs<LT>()];
+                        uint32_t o[(3 * NG + 3) / 4 * 4];
                         tc_fence_after();
-                        load_o<LT>(to, o);
+                        load_cols<3 * NG>(to, o);
 #pragma unroll
-                        for (int c = 0; c < NC; c++)
+                        for (int c = 0; c < NG; c++)
 #pragma unroll
                             for (int k = 0; k < 3; k++)
                                 o[3 * c + k] = __float_as_uint(__uint_as_float(o[3 * c + k]) * (corr[c] * vmove));
-                        store_o<LT>(to, o);
+                        store_cols<3 * NG>(to, o);
                     }
                 }
                 // this buffer of P was read by P.V of two tiles ago
                 if (alive && t >= 2) alive = warp_wait(&pv_done[t & 1], ((t - 2) >> 1) & 1);
                 if (alive) {
                     uint8_t *dst = sP + (t & 1) * NP * 128;
-                    const float ratio = 256.f * ((half ? w.vs[1] : w.vs[0]) / vref);
+                    const float ratio = blk < 0 ? 0.f : 256.f * ((half ? w.vs[1] : w.vs[0]) / vref);
 #pragma unroll
-                    for (int c = 0; c < NC; c += 2) {
+                    for (int c = 0; c < NG; c += 2) {
+                        if (c >= ng) break;
                         float a = ex2(s[c] - (m[c] == -INFINITY ? 0.f : m[c]));
                         float b = ex2(s[c + 1] - (m[c + 1] == -INFINITY ? 0.f : m[c + 1]));
                         l[c] += a;
                         l[c + 1] += b;
-                        a = blk < 0 ? 0.f : a * ratio;
-                        b = blk < 0 ? 0.f : b * ratio;
+                        a *= ratio;
+                        b *= ratio;
 #pragma unroll
                         for (int k = 0; k < 3; k++) {
                             const uint32_t e = f32x2_to_e4m3x2(a, b);
-                            dst[sw(3 * c + k, row)] = (uint8_t)e;
-                            dst[sw(3 * c + 3 + k, row)] = (uint8_t)(e >> 8);
+                            dst[sw(3 * (c0 + c) + k, row)] = (uint8_t)e;
+                            dst[sw(3 * (c0 + c) + 3 + k, row)] = (uint8_t)(e >> 8);
                             const float2 f = e4m3x2_to_f32x2(e);
                             a = (a - f.x) * 16.f;
                             b = (b - f.y) * 16.f;
                         }
                     }
                     // codes of V behind the context may be anything, NaN too: a weight of 0 needs a 0
-                    if (blk >= 0 && pos >= w.ctx) {
+                    if (grp == 0 && blk >= 0 && pos >= w.ctx) {
                         uint4 *z = (uint4 *)(ring + st * STAGE + 2 * BLK + row * 128);
 #pragma unroll
                         for (int k = 0; k < 8; k++) z[k] = make_uint4(0u, 0u, 0u, 0u);
@@ -684,25 +730,28 @@ kv8_attn_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
                 t++;
                 tiles++;
             }
-            if (!(w.flags & R_LAST)) continue;
+            if (!(w.flags & R_LAST)) {
+                if (dead ? meet(dead) : (w.flags & R_END) != 0) break;
+                continue;
+            }
 
             // ---------------- the piece ends ----------------
-            const uint32_t to = tO + lane_off + (piece & 1) * NP;
-            uint32_t o[o_regs<LT>()];
+            const uint32_t to = tO + lane_off + (piece & 1) * NP + 3 * c0;
+            uint32_t o[(3 * NG + 3) / 4 * 4];
 #pragma unroll
-            for (int c = 0; c < o_regs<LT>(); c++) o[c] = 0u;
+            for (int c = 0; c < (3 * NG + 3) / 4 * 4; c++) o[c] = 0u;
 #pragma unroll
-            for (int c = 0; c < NC; c++) {
+            for (int c = 0; c < NG; c++) {
                 float x = l[c];
 #pragma unroll
                 for (int k = 16; k > 0; k >>= 1) x += __shfl_xor_sync(0xFFFFFFFFu, x, k);
-                if (lane == 0) xsum[ends & 1][qw][c] = x;
+                if (lane == 0) xsum[ends & 1][qw][c0 + c] = x;
             }
             if (tiles && !dead) {
                 dead = !warp_wait(&pv_done[(t - 1) & 1], ((t - 1) >> 1) & 1);
                 if (!dead) {
                     tc_fence_after();
-                    load_o<LT>(to, o);
+                    load_cols<3 * NG>(to, o);
                     tc_fence_before();
                 }
             }
@@ -711,22 +760,23 @@ kv8_attn_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
             if (meet(dead)) break;
             const float (*xs)[NC] = xsum[ends & 1];
 #pragma unroll
-            for (int c = 0; c < NC; c++) {
-                if (c >= 2 * p.L) break;
-                const float L = (xs[0][c] + xs[1][c]) + (xs[2][c] + xs[3][c]);
+            for (int c = 0; c < NG; c++) {
+                if (c >= ng) break;
+                const int col = c0 + c;
+                const float L = (xs[0][col] + xs[1][col]) + (xs[2][col] + xs[3][col]);
                 const float O = fmaf(fmaf(__uint_as_float(o[3 * c + 2]), 0.0625f, __uint_as_float(o[3 * c + 1])), 0.0625f,
                                      __uint_as_float(o[3 * c])) * (vref * 0.00390625f);
                 if (w.slot < 0) {
-                    const size_t orow = (size_t)w.s * p.L + (c >> 1);
+                    const size_t orow = (size_t)w.s * p.L + (col >> 1);
                     // no position at all: zero
-                    p.out[orow * p.ldo + (2 * w.kvh + (c & 1)) * KV8_HD + row] =
+                    p.out[orow * p.ldo + (2 * w.kvh + (col & 1)) * KV8_HD + row] =
                         f32_to_bf16_rne(L == 0.f ? 0.f : O * (1.f / L));
                 } else {
-                    float *part = p.part + (size_t)w.slot * (2 * p.L) * (KV8_HD + 2);
-                    part[c * KV8_HD + row] = O;
+                    float *part = p.part + part_base(gridDim.x) + (size_t)w.slot * (2 * p.L) * (KV8_HD + 2);
+                    part[col * KV8_HD + row] = O;
                     if (row == 0) {
-                        part[2 * p.L * KV8_HD + 2 * c] = m[c];
-                        part[2 * p.L * KV8_HD + 2 * c + 1] = L;
+                        part[2 * p.L * KV8_HD + 2 * col] = m[c];
+                        part[2 * p.L * KV8_HD + 2 * col + 1] = L;
                     }
                 }
             }
@@ -745,62 +795,44 @@ kv8_attn_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
 // one). A warp takes one column (128 dimensions, 4 per lane); with 2 or 4 columns
 // the 8 warps share each column's pieces.
 constexpr int CMB_WARPS = 8;
-__global__ void __launch_bounds__(CMB_WARPS * 32) kv8_combine_kernel(const Kv8AttnArgs p, const Lay lay, int n_max) {
+__global__ void __launch_bounds__(CMB_WARPS * 32) kv8_combine_kernel(const Kv8AttnArgs p, int n_runs) {
     __shared__ float red[CMB_WARPS][KV8_HD + 1];
     dep_wait();
     dep_launch();
-    const int c = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    Cur cur{};
-    long long u0 = 0, u1 = 0;
-    int n = 0;
-    long long tot = 0;
-    locate(p, lay, [&](long long total) {
-        const Cut cut(total, n_max);
-        tot = total;
-        u0 = u1 = total;
-        n = cut.n;
-        if (c < cut.n - 1) {
-            u0 = cut.start(c);
-            u1 = cut.start(c + 1);
-        }
-        return u1;
-    }, &cur);
-    if (c >= n - 1) return;
-    const int kvh = cur.x / cur.upp, j = cur.x - kvh * cur.upp;
-    const long long first = u1 - j;                            // the pair's first unit
-    if (j == 0 || first < u0) return;                          // no pair crosses, or it began earlier
-    const int pieces = Cut(tot, n_max).run_of(first + cur.upp - 1) - c + 1;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int4 x4 = __ldcg((const int4 *)p.part + blockIdx.x);
+    const Cross x = *(const Cross *)&x4;
+    const int pieces = x.n;
+    if (!pieces) return;
     const int n_col = 2 * p.L, wpc = max(1, CMB_WARPS / n_col), sub = warp % wpc;
     const size_t stride = (size_t)n_col * (KV8_HD + 2);
-    const float *own = p.part + 2 * (size_t)c * stride;        // piece k: slot 2 (c + k), the first 2 c or 2 c + 1
-    const size_t own_off = first > u0 ? stride : 0;
+    // piece k: slot 2 (c + k), but the first one's is given
+    const float *own = p.part + part_base(n_runs) + 2 * (size_t)blockIdx.x * stride;
+    const size_t own_off = (x.slot & 1) * stride;
     for (int col = warp / wpc; col < n_col; col += CMB_WARPS / wpc) {
         const size_t ml = (size_t)n_col * KV8_HD + 2 * col;
-        float M = -INFINITY;
-        for (int k = lane; k < pieces; k += 32) M = fmaxf(M, __ldcg(own + 2 * k * stride + (k ? 0 : own_off) + ml));
-#pragma unroll
-        for (int x = 16; x > 0; x >>= 1) M = fmaxf(M, __shfl_xor_sync(0xFFFFFFFFu, M, x));
+        auto state = [&](int k) { return __ldcg((const float2 *)(own + 2 * k * stride + (k ? 0 : own_off) + ml)); };
+        // lane i holds piece i's (max, sum); pieces beyond 32 are read again below
+        const float2 mine = lane < pieces ? state(lane) : make_float2(-INFINITY, 0.f);
+        float M = mine.x;
+        for (int k = lane + 32; k < pieces; k += 32) M = fmaxf(M, state(k).x);
+        M = warp_max(M);
         float L = 0.f;
         float4 O = make_float4(0.f, 0.f, 0.f, 0.f);
-        for (int k0 = 0; k0 < pieces; k0 += 32 * wpc) {        // lane i of this batch: piece k0 + wpc i + sub
-            const int k = k0 + wpc * lane + sub;
-            float f = 0.f;
-            if (k < pieces) {
-                const float2 v = __ldcg((const float2 *)(own + 2 * k * stride + (k ? 0 : own_off) + ml));
-                f = v.x == M ? 1.f : ex2(v.x - M);
-                L += v.y * f;
-            }
-            const int take = min(32, (pieces - k0 - sub + wpc - 1) / wpc);
+        for (int k0 = 0; k0 < pieces; k0 += 32) {
+            const float2 v = k0 == 0 ? mine : k0 + lane < pieces ? state(k0 + lane) : make_float2(-INFINITY, 0.f);
+            const float f = v.x == M ? 1.f : ex2(v.x - M);
+            if (lane % wpc == sub) L += v.y * f;
+            const int n = min(32, pieces - k0);
 #pragma unroll 8
-            for (int i = 0; i < take; i++) {
-                const int ki = k0 + wpc * i + sub;
+            for (int i = sub; i < n; i += wpc) {
                 const float w = __shfl_sync(0xFFFFFFFFu, f, i);
-                const float4 v = __ldcg((const float4 *)(own + 2 * ki * stride + (ki ? 0 : own_off) + col * KV8_HD) + lane);
-                O.x += v.x * w; O.y += v.y * w; O.z += v.z * w; O.w += v.w * w;
+                const float4 o = __ldcg((const float4 *)(own + 2 * (k0 + i) * stride + (k0 + i ? 0 : own_off) + col * KV8_HD) + lane);
+                O.x += o.x * w; O.y += o.y * w; O.z += o.z * w; O.w += o.w * w;
             }
         }
 #pragma unroll
-        for (int x = 16; x > 0; x >>= 1) L += __shfl_xor_sync(0xFFFFFFFFu, L, x);
+        for (int o = 16; o > 0; o >>= 1) L += __shfl_xor_sync(0xFFFFFFFFu, L, o);
         if (wpc > 1) {                                         // one round: every warp comes here once
             float *d = red[warp] + 4 * lane;
             d[0] = O.x; d[1] = O.y; d[2] = O.z; d[3] = O.w;
@@ -813,41 +845,38 @@ __global__ void __launch_bounds__(CMB_WARPS * 32) kv8_combine_kernel(const Kv8At
                 L += red[warp + w][KV8_HD];
             }
         }
-        const size_t row = (size_t)cur.s * p.L + (col >> 1);
+        const size_t row = (size_t)x.s * p.L + (col >> 1);
         const float inv = L == 0.f ? 0.f : 1.f / L;
-        uint2 *dst = (uint2 *)(p.out + row * p.ldo + (2 * kvh + (col & 1)) * KV8_HD) + lane;
+        uint2 *dst = (uint2 *)(p.out + row * p.ldo + (2 * x.kvh + (col & 1)) * KV8_HD) + lane;
         *dst = make_uint2(pack_bf16x2(O.x * inv, O.y * inv), pack_bf16x2(O.z * inv, O.w * inv));
     }
 }
 
 constexpr int kSms = 148;
-// CTAs that share an SM: by shared memory (228 KB, 2 KB a CTA of it reserved or
-// static) and TMEM (512 columns)
 template <int LT>
-int ctas(int L) {
-    const int per_sm = 233472 / (smem_bytes<LT>(L, stages<LT>()) + 2048);
-    const int by_tmem = 512 / tmem_cols<LT>();
-    return kSms * (per_sm < 1 ? 1 : per_sm < by_tmem ? per_sm : by_tmem);
-}
-int max_ctas(int L) { return L == 1 ? ctas<1>(L) : L <= 4 ? ctas<4>(L) : ctas<8>(L); }
+int ctas() { return kSms * per_sm<LT>(); }
+static_assert(3 * (smem_bytes<1>(1) + 2048) <= 233472 && 2 * (smem_bytes<4>(4) + 2560) <= 233472 &&
+                  smem_bytes<8>(8) + 3072 <= 233472,
+              "shared memory of an SM: 228 KB, 1 KB a CTA reserved, the rest of the sum static");
+static_assert(3 * tmem_cols<1>() <= 512 && 2 * tmem_cols<4>() <= 512 && tmem_cols<8>() <= 512, "TMEM of an SM");
+int max_ctas(int L) { return L == 1 ? ctas<1>() : L <= 4 ? ctas<4>() : ctas<8>(); }
 
 template <int LT>
 int launch(cudaStream_t st, const CUtensorMap &tk, const CUtensorMap &tv, const Kv8AttnArgs &a) {
-    constexpr int ST = stages<LT>();
     static bool attr[64];
     int dev = 0;
     N550_CUDA_TRY(cudaGetDevice(&dev));
     if (dev >= 0 && dev < 64 && !attr[dev]) {
-        N550_CUDA_TRY(cudaFuncSetAttribute(kv8_attn_kernel<LT, ST>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                           smem_bytes<LT>(LT, ST)));
+        N550_CUDA_TRY(cudaFuncSetAttribute(kv8_attn_kernel<LT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                           smem_bytes<LT>(LT)));
         attr[dev] = true;
     }
-    const size_t smem = smem_bytes<LT>(a.L, ST);
+    const size_t smem = smem_bytes<LT>(a.L);
     Lay lay{};
     const long long pairs = (long long)a.n_seqs * KV8_NKV;
     if (!a.part) {
         lay.kind = LAY_PAIR;
-        N550_CUDA_TRY(launch_k(kv8_attn_kernel<LT, ST>, dim3((unsigned)pairs), THREADS, smem, st, tk, tv, a, lay));
+        N550_CUDA_TRY(launch_k(kv8_attn_kernel<LT>, dim3((unsigned)pairs), threads<LT>(), smem, st, tk, tv, a, lay));
         N550_LAUNCH_CHECK();
         return N550_OK;
     }
@@ -860,11 +889,11 @@ int launch(cudaStream_t st, const CUtensorMap &tk, const CUtensorMap &tv, const 
     }
     // no more runs than there can be (the kernels cut by the units there are)
     const long long most = (pairs * (lay.kind == LAY_EVEN ? lay.upp : a.c.nb) + kMinRun - 1) / kMinRun;
-    const int n = (int)(most < ctas<LT>(a.L) ? most : ctas<LT>(a.L));
-    N550_CUDA_TRY(launch_k(kv8_attn_kernel<LT, ST>, dim3(n), THREADS, smem, st, tk, tv, a, lay));
+    const int n = (int)(most < ctas<LT>() ? most : ctas<LT>());
+    N550_CUDA_TRY(launch_k(kv8_attn_kernel<LT>, dim3(n), threads<LT>(), smem, st, tk, tv, a, lay));
     N550_LAUNCH_CHECK();
     if (n > 1) {
-        N550_CUDA_TRY(launch_k(kv8_combine_kernel, dim3(n - 1), CMB_WARPS * 32, 0, st, a, lay, n));
+        N550_CUDA_TRY(launch_k(kv8_combine_kernel, dim3(n - 1), CMB_WARPS * 32, 0, st, a, n));
         N550_LAUNCH_CHECK();
     }
     return N550_OK;
@@ -874,7 +903,8 @@ int launch(cudaStream_t st, const CUtensorMap &tk, const CUtensorMap &tv, const 
 
 size_t kv8_attn_workspace(int n_seqs, int L) {
     if (n_seqs <= 0 || L <= 0) return 0;
-    return (size_t)max_ctas(L) * 2 * (2 * L) * (KV8_HD + 2) * sizeof(float);
+    const size_t n = max_ctas(L);
+    return n * sizeof(Cross) + n * 2 * (2 * L) * (KV8_HD + 2) * sizeof(float);
 }
 
 int launch_kv8_attn(cudaStream_t st, const Kv8AttnArgs &a) {
