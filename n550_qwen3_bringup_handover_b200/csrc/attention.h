@@ -15,6 +15,7 @@ struct AttnPrefillArgs {
     const int32_t *seq_ids;   // [n_seqs] KV slots
     int ldq, ldo, L, pos0, layer, max_len;
     int kv_planes;            // slots x 28 layers x 8 KV heads in the cache
+    bool packed;              // sequence s, KV head h is plane 8 s + h (seq_ids and layer unused)
 };
 
 // Decode: one query per sequence at position pos[s] (attends 0..pos[s]).

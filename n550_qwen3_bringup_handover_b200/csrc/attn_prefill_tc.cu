@@ -116,7 +116,7 @@ __device__ __forceinline__ Item decode_item(const PfParams &p, int k, bool with_
     const int q_last = min(p.L, it.q0 + BQ) - 1;
     it.nblk = (p.pos0 + q_last) / BKV + 1;                      // key blocks 0..nblk-1
     // (slot, layer, kv head); only the producer needs it (a global load)
-    it.plane = with_plane ? (p.seq_ids[it.s] * NL + p.layer) * NKV + it.kvh : 0;
+    it.plane = !with_plane ? 0 : p.seq_ids ? (p.seq_ids[it.s] * NL + p.layer) * NKV + it.kvh : it.s * NKV + it.kvh;
     return it;
 }
 
@@ -510,7 +510,7 @@ bool g_attr[64];
 
 int launch_attn_prefill(cudaStream_t st, const AttnPrefillArgs &a, int n_seqs) {
     if (n_seqs <= 0 || a.L <= 0) return N550_OK;
-    if (!a.q || !a.kc || !a.vc || !a.out || !a.seq_ids || a.pos0 < 0 || a.layer < 0 ||
+    if (!a.q || !a.kc || !a.vc || !a.out || (!a.seq_ids && !a.packed) || a.pos0 < 0 || a.layer < 0 ||
         a.layer >= NL || a.max_len < a.pos0 + a.L || (a.ldq % 8) || (a.ldo % 8) ||
         a.ldq < 16 * HD || a.ldo < 16 * HD || ((uintptr_t)a.out & 15) || a.kv_planes <= 0 ||
         (long long)a.kv_planes * a.max_len * HD > (1LL << 40))
@@ -536,7 +536,7 @@ int launch_attn_prefill(cudaStream_t st, const AttnPrefillArgs &a, int n_seqs) {
     }
     PfParams p;
     p.out = a.out;
-    p.seq_ids = a.seq_ids;
+    p.seq_ids = a.packed ? nullptr : a.seq_ids;
     p.ldo = a.ldo;
     p.L = a.L;
     p.pos0 = a.pos0;

@@ -28,6 +28,9 @@ float *split_ws(void *ws, size_t bytes, size_t need) {
 // gridDim.y and .z end at 65535
 constexpr int kMaxSeqs = 65535;
 
+// a pair's list and its eight heads are counted in 32 bits
+constexpr int kMaxSelect = 1 << 24;
+
 bool rows_ok(const void *p, int ld, int esz) {
     return p && ((uintptr_t)p & 15) == 0 && ld >= KV8_NH * KV8_HD && (long long)ld * esz % 16 == 0;
 }
@@ -65,7 +68,7 @@ int n550_attention_decode_kv8(void *stream, const uint16_t *q, int ldq, const n5
     if (!rows_ok(q, ldq, 2) || !rows_ok(out, ldo, 2) || !seq_ids || !pos || n_seqs > kMaxSeqs)
         return N550_ERR_ARG;
     a.q = q; a.ldq = ldq; a.out = out; a.ldo = ldo; a.seq_ids = seq_ids; a.pos = pos;
-    a.L = 1; a.n_seqs = n_seqs; a.n_select = -1;
+    a.L = a.rows = 1; a.n_seqs = n_seqs; a.n_select = -1;
     a.part = split_ws(workspace, workspace_bytes, kv8_attn_workspace(n_seqs, 1));
     return launch_kv8_attn((cudaStream_t)stream, a);
 }
@@ -79,17 +82,18 @@ int n550_attention_sparse_kv8(void *stream, const uint16_t *q, int ldq, const n5
     if (n_seqs < 0 || n_select < 0) return N550_ERR_ARG;
     if (n_seqs == 0) return N550_OK;
     if (!rows_ok(q, ldq, 2) || !rows_ok(out, ldo, 2) || !seq_ids || !pos ||
-        (!blocks && n_select) || n_seqs > kMaxSeqs)
+        (!blocks && n_select) || n_select > kMaxSelect || n_seqs > kMaxSeqs)
         return N550_ERR_ARG;
     a.q = q; a.ldq = ldq; a.out = out; a.ldo = ldo; a.seq_ids = seq_ids; a.pos = pos;
     a.blocks = blocks; a.n_select = n_select;
-    a.L = 1; a.n_seqs = n_seqs;
+    a.L = a.rows = 1; a.n_seqs = n_seqs;
     a.part = split_ws(workspace, workspace_bytes, kv8_attn_workspace(n_seqs, 1));
     return launch_kv8_attn((cudaStream_t)stream, a);
 }
 
 size_t n550_attention_prefill_kv8_workspace(int n_seqs, int L, int pos0) {
-    return n_seqs > 0 && L > 0 && L <= KV8_FEW && pos0 >= 0 ? kv8_attn_workspace(n_seqs, L) : 0;
+    if (n_seqs <= 0 || L <= 0 || pos0 < 0) return 0;
+    return L <= KV8_FEW ? kv8_attn_workspace(n_seqs, L) : kv8_prefill_workspace(n_seqs, L, pos0);
 }
 
 int n550_attention_prefill_kv8(void *stream, const uint16_t *q, int ldq, const n550_kv8_cache *c,
@@ -104,9 +108,19 @@ int n550_attention_prefill_kv8(void *stream, const uint16_t *q, int ldq, const n
         return N550_ERR_ARG;
     a.q = q; a.ldq = ldq; a.out = out; a.ldo = ldo; a.seq_ids = seq_ids;
     a.L = L; a.pos0 = pos0; a.n_seqs = n_seqs; a.n_select = -1;
-    if (L > KV8_FEW) return launch_kv8_prefill((cudaStream_t)stream, a);
-    a.part = split_ws(workspace, workspace_bytes, kv8_attn_workspace(n_seqs, L));
-    return launch_kv8_attn((cudaStream_t)stream, a);
+    a.rows = L;
+    const size_t need = n550_attention_prefill_kv8_workspace(n_seqs, L, pos0);
+    float *ws = split_ws(workspace, workspace_bytes, need);
+    if (L > KV8_FEW && ws) return launch_kv8_prefill((cudaStream_t)stream, a, ws);
+    // few queries, or no workspace: the streaming kernel, KV8_FEW queries a pass
+    if (L <= KV8_FEW) a.part = ws;
+    for (int j = 0; j < L; j += KV8_FEW) {
+        a.row0 = j;
+        a.pos0 = pos0 + j;
+        a.L = L - j < KV8_FEW ? L - j : KV8_FEW;
+        if (int rc = launch_kv8_attn((cudaStream_t)stream, a)) return rc;
+    }
+    return N550_OK;
 }
 
 int n550_kv8_select_blocks(void *stream, const uint16_t *q, int ldq, const n550_kv8_cache *c, int layer,

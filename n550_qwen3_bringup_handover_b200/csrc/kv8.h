@@ -74,12 +74,16 @@ struct Kv8AttnArgs {
     const int32_t *blocks;     // [n_seqs][8][n_select]
     int n_select;              // < 0: no list, the whole context
     int ldq, ldo, L, pos0, n_seqs;
+    int rows, row0;            // a sequence's rows in q and out, and the first of these L among them
     float *part;               // split partials, or NULL
 };
 
 int launch_kv8_append(cudaStream_t st, const Kv8AppendArgs &a, bool f32, int n_seqs);
 constexpr int KV8_FEW = 8;     // most queries per sequence of launch_kv8_attn
-int launch_kv8_prefill(cudaStream_t st, const Kv8AttnArgs &a);
+// Many queries: codes written out as BF16 to `ws` (kv8_prefill_workspace bytes), then
+// the BF16 prefill kernel.
+int launch_kv8_prefill(cudaStream_t st, const Kv8AttnArgs &a, void *ws);
+size_t kv8_prefill_workspace(int n_seqs, int L, int pos0);
 int launch_kv8_attn(cudaStream_t st, const Kv8AttnArgs &a);
 size_t kv8_attn_workspace(int n_seqs, int L);
 

@@ -458,7 +458,7 @@ kv8_attn_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
                         uint8_t *t = ring + st * STAGE;
                         for (int j = 0; j < qn; j++)
                             bulk_load(sraw + (st * p.L + j) * 512,
-                                      p.q + ((size_t)me.s * p.L + j) * p.ldq + me.kvh * 2 * KV8_HD, 512, &full[st]);
+                                      p.q + ((size_t)me.s * p.rows + p.row0 + j) * p.ldq + me.kvh * 2 * KV8_HD, 512, &full[st]);
                         for (int j = 0; j < 2; j++)
                             if (me.blk[j] >= 0) {
                                 tma_load_3d(t + j * BLK, &tmK, &full[st], 0, me.blk[j] * KV8_BLOCK, plane);
@@ -767,7 +767,7 @@ kv8_attn_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
                 const float O = fmaf(fmaf(__uint_as_float(o[3 * c + 2]), 0.0625f, __uint_as_float(o[3 * c + 1])), 0.0625f,
                                      __uint_as_float(o[3 * c])) * (vref * 0.00390625f);
                 if (w.slot < 0) {
-                    const size_t orow = (size_t)w.s * p.L + (col >> 1);
+                    const size_t orow = (size_t)w.s * p.rows + p.row0 + (col >> 1);
                     // no position at all: zero
                     p.out[orow * p.ldo + (2 * w.kvh + (col & 1)) * KV8_HD + row] =
                         f32_to_bf16_rne(L == 0.f ? 0.f : O * (1.f / L));
@@ -845,7 +845,7 @@ __global__ void __launch_bounds__(CMB_WARPS * 32) kv8_combine_kernel(const Kv8At
                 L += red[warp + w][KV8_HD];
             }
         }
-        const size_t row = (size_t)x.s * p.L + (col >> 1);
+        const size_t row = (size_t)x.s * p.rows + p.row0 + (col >> 1);
         const float inv = L == 0.f ? 0.f : 1.f / L;
         uint2 *dst = (uint2 *)(p.out + row * p.ldo + (2 * x.kvh + (col & 1)) * KV8_HD) + lane;
         *dst = make_uint2(pack_bf16x2(O.x * inv, O.y * inv), pack_bf16x2(O.z * inv, O.w * inv));

@@ -9,14 +9,17 @@ from . import BF16, F32, KV8_BLOCK, KV8CacheStruct, check, lib
 _LAYERS, _NKV, _HD, _NH = 28, 8, 128, 16
 
 
-def _on_current(*tensors):
-    """The current CUDA device's stream; the tensors must live on that device."""
+def _stream(cache, *tensors):
+    """The raw current stream of the cache's device, which must be the current one
+    and hold the tensors."""
     import torch
-    dev = torch.cuda.current_device()
+    dev = cache.device_index
     for t in tensors:
-        if t.device.type != "cuda" or t.device.index != dev:
-            raise ValueError(f"tensor on {t.device}, but the current CUDA device is cuda:{dev}")
-    return torch.cuda.current_stream().cuda_stream
+        if t.get_device() != dev:
+            raise ValueError(f"tensor on {t.device}, but the cache is on cuda:{dev}")
+    if torch.cuda.current_device() != dev:
+        raise ValueError(f"the cache is on cuda:{dev}, the current device is cuda:{torch.cuda.current_device()}")
+    return torch._C._cuda_getCurrentRawStream(dev)
 
 
 class KV8Cache:
@@ -61,34 +64,40 @@ class KV8Cache:
                 raise ValueError("the cache's tensors must be on one CUDA device")
         self.k, self.v, self.k_scale, self.v_scale, self.k_bounds = k, v, k_scale, v_scale, k_bounds
         self.n_slots, self.n_layers, self.max_len, self.n_blocks = k.shape[0], k.shape[1], k.shape[3], nb
+        self.device_index = k.get_device()
         self._c = KV8CacheStruct(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
                                  k_bounds.data_ptr() if k_bounds is not None else None,
                                  self.n_slots, self.n_layers, self.max_len)
         self._ref = C.byref(self._c)
 
 
-def _ids(name, t, n=None):
+def _ids(seq_ids, pos=None):
+    """Number of sequences; both must be contiguous int32 vectors of that length."""
     import torch
-    if t.dtype != torch.int32 or t.dim() != 1 or not t.is_contiguous() or (n is not None and t.numel() != n):
-        raise ValueError(f"{name} must be a contiguous int32 vector" + (f" of {n}" if n is not None else ""))
-    return t.numel()
+    for name, t in (("seq_ids", seq_ids), ("pos", pos)):
+        if t is not None and (t.dtype != torch.int32 or t.dim() != 1 or not t.is_contiguous()):
+            raise ValueError(f"{name} must be a contiguous int32 vector")
+    n = seq_ids.shape[0]
+    if pos is not None and pos.shape[0] != n:
+        raise ValueError(f"pos must hold {n} positions")
+    return n
 
 
 def _rows(name, t, rows, cols, dtypes):
-    if t.dim() != 2 or t.shape[0] != rows or t.shape[1] < cols or t.dtype not in dtypes or \
-            (t.stride(1) != 1 and rows > 0):
+    shape, stride = t.shape, t.stride()
+    if len(shape) != 2 or shape[0] != rows or shape[1] < cols or t.dtype not in dtypes or \
+            (stride[1] != 1 and rows > 0):
         raise ValueError(f"{name} must be [{rows}, >= {cols}] with contiguous rows of {dtypes}")
     # the stride of a single row is never used; torch reports any number there
-    return t.stride(0) if rows > 1 else t.shape[1]
+    return stride[0] if rows > 1 else cols
 
 
 def kv8_append(cache, k, v, seq_ids, pos, L, layer):
     """Quantise len(seq_ids) x L rows of k and v ([n_seqs*L, >= 1024] float32 or
     bfloat16) into positions pos[s] .. pos[s]+L-1 of slot seq_ids[s]."""
     import torch
-    st = _on_current(cache.k, k, v, seq_ids, pos)
-    n = _ids("seq_ids", seq_ids)
-    _ids("pos", pos, n)
+    st = _stream(cache, k, v, seq_ids, pos)
+    n = _ids(seq_ids, pos)
     if L < 0:
         raise ValueError("L must not be negative")
     ld = _rows("k", k, n * L, _NKV * _HD, (torch.float32, torch.bfloat16))
@@ -103,28 +112,27 @@ def _q_out(q, rows, out):
     import torch
     ldq = _rows("q", q, rows, _NH * _HD, (torch.bfloat16,))
     if out is None:
-        out = torch.empty((rows, _NH * _HD), dtype=torch.bfloat16, device=q.device)
+        return ldq, q.new_empty((rows, _NH * _HD)), _NH * _HD
     return ldq, out, _rows("out", out, rows, _NH * _HD, (torch.bfloat16,))
 
 
 def _workspace(nbytes, device):
     import torch
-    return torch.empty(max(nbytes, 16), dtype=torch.uint8, device=device)
+    return torch.empty(nbytes, dtype=torch.uint8, device=device)
 
 
 def attention_decode_kv8(q, cache, seq_ids, pos, layer, out=None, split=True):
     """One query per sequence (rows of q, BF16) at position pos[s] over the 8-bit
     cache; split=True passes a split-KV workspace, split=False runs one CTA per
     (sequence, KV head)."""
-    n = _ids("seq_ids", seq_ids)
-    _ids("pos", pos, n)
+    n = _ids(seq_ids, pos)
     ldq, out, ldo = _q_out(q, n, out)
-    st = _on_current(cache.k, q, seq_ids, pos, out)
+    st = _stream(cache, q, seq_ids, pos, out)
     L = lib()
     nbytes = L.n550_attention_kv8_workspace(n) if split else 0
-    ws = _workspace(nbytes, q.device).data_ptr() if nbytes else None
+    ws = _workspace(nbytes, q.device) if nbytes else None
     check(L.n550_attention_decode_kv8(st, q.data_ptr(), ldq, cache._ref, layer, seq_ids.data_ptr(),
-                                      pos.data_ptr(), n, out.data_ptr(), ldo, ws, nbytes),
+                                      pos.data_ptr(), n, out.data_ptr(), ldo, ws.data_ptr() if nbytes else None, nbytes),
           "n550_attention_decode_kv8")
     return out
 
@@ -133,35 +141,34 @@ def attention_sparse_kv8(q, cache, seq_ids, pos, blocks, layer, out=None, split=
     """attention_decode_kv8 over the positions <= pos[s] of the listed blocks only:
     blocks int32 [n_seqs, 8, n_select], entries outside the context skipped."""
     import torch
-    n = _ids("seq_ids", seq_ids)
-    _ids("pos", pos, n)
+    n = _ids(seq_ids, pos)
     if blocks.dtype != torch.int32 or blocks.dim() != 3 or tuple(blocks.shape[:2]) != (n, _NKV) or \
             not blocks.is_contiguous():
         raise ValueError(f"blocks must be a contiguous int32 tensor [{n}, 8, n_select]")
     ldq, out, ldo = _q_out(q, n, out)
-    st = _on_current(cache.k, q, seq_ids, pos, blocks, out)
+    st = _stream(cache, q, seq_ids, pos, blocks, out)
     L = lib()
     nbytes = L.n550_attention_kv8_workspace(n) if split else 0
-    ws = _workspace(nbytes, q.device).data_ptr() if nbytes else None
+    ws = _workspace(nbytes, q.device) if nbytes else None
     check(L.n550_attention_sparse_kv8(st, q.data_ptr(), ldq, cache._ref, layer, seq_ids.data_ptr(),
                                       pos.data_ptr(), blocks.data_ptr(), blocks.shape[2], n,
-                                      out.data_ptr(), ldo, ws, nbytes), "n550_attention_sparse_kv8")
+                                      out.data_ptr(), ldo, ws.data_ptr() if nbytes else None, nbytes), "n550_attention_sparse_kv8")
     return out
 
 
 def attention_prefill_kv8(q, cache, seq_ids, L, pos0, layer, out=None, workspace=True):
     """Causal attention of len(seq_ids) sequences x L queries (rows of q, BF16) at
     positions pos0.. over the 8-bit cache, which holds their K/V already."""
-    n = _ids("seq_ids", seq_ids)
+    n = _ids(seq_ids)
     if L < 0:
         raise ValueError("L must not be negative")
     ldq, out, ldo = _q_out(q, n * L, out)
-    st = _on_current(cache.k, q, seq_ids, out)
+    st = _stream(cache, q, seq_ids, out)
     lb = lib()
     nbytes = lb.n550_attention_prefill_kv8_workspace(n, L, pos0) if workspace else 0
-    ws = _workspace(nbytes, q.device).data_ptr() if nbytes else None
+    ws = _workspace(nbytes, q.device) if nbytes else None
     check(lb.n550_attention_prefill_kv8(st, q.data_ptr(), ldq, cache._ref, layer, seq_ids.data_ptr(), n,
-                                        L, pos0, out.data_ptr(), ldo, ws, nbytes),
+                                        L, pos0, out.data_ptr(), ldo, ws.data_ptr() if nbytes else None, nbytes),
           "n550_attention_prefill_kv8")
     return out
 
@@ -171,14 +178,13 @@ def kv8_select_blocks(q, cache, seq_ids, pos, layer, n_select, n_sink=1, n_recen
     for the sequence's query, per KV head: int32 [n_seqs, 8, n_select], ascending,
     -1 behind the last."""
     import torch
-    n = _ids("seq_ids", seq_ids)
-    _ids("pos", pos, n)
+    n = _ids(seq_ids, pos)
     ldq = _rows("q", q, n, _NH * _HD, (torch.bfloat16,))
     if out is None:
         out = torch.empty((n, _NKV, max(n_select, 0)), dtype=torch.int32, device=q.device)
     elif tuple(out.shape) != (n, _NKV, n_select) or out.dtype != torch.int32 or not out.is_contiguous():
         raise ValueError(f"out must be a contiguous int32 tensor [{n}, 8, {n_select}]")
-    st = _on_current(cache.k, q, seq_ids, pos, out)
+    st = _stream(cache, q, seq_ids, pos, out)
     check(lib().n550_kv8_select_blocks(st, q.data_ptr(), ldq, cache._ref, layer, seq_ids.data_ptr(),
                                        pos.data_ptr(), n, n_select, n_sink, n_recent, out.data_ptr()),
           "n550_kv8_select_blocks")
