@@ -16,40 +16,187 @@
 namespace n550 {
 namespace {
 
-constexpr int AP_THREADS = 256;
-constexpr int AP_ROWS = AP_THREADS / 16;                  // rows in flight: 16 threads x 8 dims each
-constexpr int AP_ITER = KV8_BLOCK / AP_ROWS;
-
-template <bool F32>
-__device__ __forceinline__ void load8(const void *base, size_t off, float (&x)[8]) {
-    if constexpr (F32) {
-        const float4 *p = (const float4 *)((const float *)base + off);
-        const float4 a = p[0], b = p[1];
-        x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
-        x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
-    } else {
-        const uint4 a = *(const uint4 *)((const uint16_t *)base + off);
-        const uint32_t w[4] = {a.x, a.y, a.z, a.w};
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            x[2 * i] = __uint_as_float(w[i] << 16);
-            x[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
-        }
-    }
-}
-
 // Exponent e of the smallest power of two 2^e with amax <= 448 * 2^e, at least
 // -126 (so that the scale and its reciprocal are normal numbers).
 __device__ __forceinline__ int scale_exp(uint32_t amax_bits) {
     const int e = (int)(amax_bits >> 23) - 127 - 8 + ((amax_bits & 0x7FFFFFu) > 0x600000u);
     return max(e, -126);
 }
+__device__ __forceinline__ float pow2(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
+// 1 / s of a power of two with exponent in [-126, 120]
+__device__ __forceinline__ float inv_pow2(float s) { return __uint_as_float((254u << 23) - __float_as_uint(s)); }
 
-// One CTA per (block the rows reach, K or V of a KV head, sequence).
+// FP32 bits of the largest finite magnitude of N words (FP32, or pairs of BF16).
+__device__ __forceinline__ uint32_t finite_only(uint32_t a) { return a < 0x7F800000u ? a : 0u; }
+template <bool F32, int N>
+__device__ __forceinline__ uint32_t abs_max(const uint32_t (&w)[N]) {
+    uint32_t m = 0;
+    if constexpr (F32) {
+#pragma unroll
+        for (int i = 0; i < N; i++) m = max(m, w[i] & 0x7FFFFFFFu);
+        if (m >= 0x7F800000u) {                              // an infinity or a NaN: look again
+            m = 0;
+#pragma unroll
+            for (int i = 0; i < N; i++) m = max(m, finite_only(w[i] & 0x7FFFFFFFu));
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; i++) m = __vmaxu2(m, w[i] & 0x7FFF7FFFu);
+        m = max(m << 16, m & 0xFFFF0000u);
+        if (m >= 0x7F800000u) {
+            m = 0;
+#pragma unroll
+            for (int i = 0; i < N; i++) {
+                m = max(m, finite_only(w[i] << 16 & 0x7FFF0000u));
+                m = max(m, finite_only(w[i] & 0x7FFF0000u));
+            }
+        }
+    }
+    return m;
+}
+// Four codes of four values (2 words of BF16 pairs, or 4 of FP32) times inv.
 template <bool F32>
-__global__ void __launch_bounds__(AP_THREADS) kv8_append_kernel(const Kv8AppendArgs p) {
+__device__ __forceinline__ uint32_t codes4(const uint32_t *w, float inv) {
+    float x[4];
+    if constexpr (F32) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) x[i] = __uint_as_float(w[i]) * inv;
+    } else {
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+            x[2 * i] = __uint_as_float(w[i] << 16) * inv;
+            x[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u) * inv;
+        }
+    }
+    return f32x2_to_e4m3x2(x[0], x[1]) | f32x2_to_e4m3x2(x[2], x[3]) << 16;
+}
+// Four held codes at a scale 1 / shrink times larger.
+__device__ __forceinline__ uint32_t shrink4(uint32_t c, float shrink) {
+    const float2 a = e4m3x2_to_f32x2(c & 0xFFFFu), b = e4m3x2_to_f32x2(c >> 16);
+    return f32x2_to_e4m3x2(a.x * shrink, a.y * shrink) | f32x2_to_e4m3x2(b.x * shrink, b.y * shrink) << 16;
+}
+// Codes with each NaN (0x7F, 0xFF) replaced by 0: what a NaN counts as in the bounds.
+__device__ __forceinline__ uint32_t nan_to_zero(uint32_t c) {
+    const uint32_t n = ((c & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u;     // 0x80 at each NaN
+    return n ? c & ~((n >> 7) * 0xFFu) : c;
+}
+__device__ __forceinline__ uint32_t hmin2(uint32_t a, uint32_t b) {
+    uint32_t r;
+    asm("min.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+}
+__device__ __forceinline__ uint32_t hmax2(uint32_t a, uint32_t b) {
+    uint32_t r;
+    asm("max.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+}
+// FP16 pair that holds e4m3 values -> its two codes (exact).
+__device__ __forceinline__ uint32_t f16x2_to_e4m3x2(uint32_t h) {
+    uint16_t r;
+    asm("cvt.rn.satfinite.e4m3x2.f16x2 %0, %1;" : "=h"(r) : "r"(h));
+    return r;
+}
+constexpr uint32_t kHInf = 0x7C007C00u, kHNegInf = 0xFC00FC00u;
+
+// ---------------------------------------------------------------------------
+// A few rows per sequence (a decode step, drafted tokens): one warp per (block the
+// rows reach, KV head, sequence) does K and V, lane l the dimensions 4 l .. 4 l + 3.
+// Bound: latency. All it reads besides ids and positions is requested at once. One
+// CTA of 256 threads per (block, K or V head, sequence) took 19 us for 256 rows.
+// ---------------------------------------------------------------------------
+constexpr int FEW = 8;                                        // most rows per sequence
+constexpr int FEW_WARPS = 4;
+
+template <bool F32>
+__global__ void __launch_bounds__(FEW_WARPS * 32) kv8_append_few_kernel(const Kv8AppendArgs p, int n_blk, int n_items) {
+    constexpr int W = F32 ? 4 : 2;                            // words of a lane's four dimensions
+    const int item = blockIdx.x * FEW_WARPS + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+    dep_wait();
+    dep_launch();
+    if (item >= n_items) return;
+    const int kvh = item & 7, s = (item >> 3) / n_blk, nth = (item >> 3) % n_blk;
+    const int slot = p.seq_ids[s], p0 = p.pos[s];
+    if (slot < 0 || slot >= p.c.n_slots || p0 < 0 || p0 > p.c.max_len - p.L) return;
+    const int b = p0 / KV8_BLOCK + nth, t_blk = b * KV8_BLOCK;
+    const int lo = max(p0, t_blk), hi = min(p0 + p.L, t_blk + KV8_BLOCK), n = hi - lo;
+    if (n <= 0) return;
+    const bool has_old = p0 > t_blk;
+    const size_t plane = p.c.plane(slot, kvh), blk = plane * p.c.nb + b;
+    uint32_t *bound = p.c.kb ? (uint32_t *)(p.c.kb + blk * 2 * KV8_HD) + lane : nullptr;
+    float s_old[2] = {0.f, 0.f};
+    uint32_t old_lo = 0, old_hi = 0;
+    if (has_old) {
+        s_old[0] = p.c.ks[blk];
+        s_old[1] = p.c.vs[blk];
+        if (bound) { old_lo = bound[0]; old_hi = bound[32]; }
+    }
+#pragma unroll
+    for (int w = 0; w < 2; w++) {
+        const void *src = w ? p.v : p.k;
+        uint32_t x[FEW][W], all[FEW * W];
+#pragma unroll
+        for (int i = 0; i < FEW; i++) {
+            const size_t o = ((size_t)s * p.L + (lo - p0) + i) * p.ld + kvh * KV8_HD + 4 * lane;
+#pragma unroll
+            for (int j = 0; j < W; j++) x[i][j] = 0u;
+            if (i < n) {
+                if constexpr (F32) {
+                    const uint4 q = *(const uint4 *)((const float *)src + o);
+                    x[i][0] = q.x; x[i][1] = q.y; x[i][2] = q.z; x[i][3] = q.w;
+                } else {
+                    const uint2 q = *(const uint2 *)((const uint16_t *)src + o);
+                    x[i][0] = q.x; x[i][1] = q.y;
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < W; j++) all[i * W + j] = x[i][j];
+        }
+        const uint32_t am = __reduce_max_sync(0xFFFFFFFFu, abs_max<F32>(all));
+        const float sc = fmaxf(s_old[w], pow2(scale_exp(am))), inv = inv_pow2(sc), shrink = s_old[w] * inv;
+        uint32_t *codes = (uint32_t *)((w ? p.c.v : p.c.k) + (plane * p.c.max_len + t_blk) * KV8_HD) + lane;
+        if (has_old && shrink != 1.f)                         // the scale grew
+#pragma unroll 8
+            for (int r = 0; r < p0 - t_blk; r++) codes[r * 32] = shrink4(codes[r * 32], shrink);
+        uint32_t mn[2] = {kHInf, kHInf}, mx[2] = {kHNegInf, kHNegInf};
+#pragma unroll
+        for (int i = 0; i < FEW; i++) {
+            if (i >= n) continue;
+            const uint32_t c = codes4<F32>(x[i], inv);
+            codes[(lo - t_blk + i) * 32] = c;
+            if (w == 0) {
+                const uint32_t z = nan_to_zero(c), h0 = e4m3x2_to_f16x2(z & 0xFFFFu), h1 = e4m3x2_to_f16x2(z >> 16);
+                mn[0] = hmin2(mn[0], h0); mx[0] = hmax2(mx[0], h0);
+                mn[1] = hmin2(mn[1], h1); mx[1] = hmax2(mx[1], h1);
+            }
+        }
+        if (lane == 0) (w ? p.c.vs : p.c.ks)[blk] = sc;
+        if (w == 0 && bound) {
+            if (has_old) {
+                const uint32_t l = shrink4(old_lo, shrink), h = shrink4(old_hi, shrink);
+                mn[0] = hmin2(mn[0], e4m3x2_to_f16x2(l & 0xFFFFu)); mn[1] = hmin2(mn[1], e4m3x2_to_f16x2(l >> 16));
+                mx[0] = hmax2(mx[0], e4m3x2_to_f16x2(h & 0xFFFFu)); mx[1] = hmax2(mx[1], e4m3x2_to_f16x2(h >> 16));
+            }
+            bound[0] = f16x2_to_e4m3x2(mn[0]) | f16x2_to_e4m3x2(mn[1]) << 16;
+            bound[32] = f16x2_to_e4m3x2(mx[0]) | f16x2_to_e4m3x2(mx[1]) << 16;
+        }
+    }
+}
+
+// ---------------------------------------------------------------------------
+// Prompts: one CTA per (block the rows reach, K or V of a KV head, sequence), the
+// block's rows in registers between the maximum and the rounding. Bound: HBM.
+// Thread t takes 8 dimensions (t % 16) of rows t / 16, + 16, ..; bounds are minima
+// and maxima of FP16 pairs.
+// ---------------------------------------------------------------------------
+constexpr int AP_THREADS = 256;
+constexpr int AP_ROWS = AP_THREADS / 16;
+constexpr int AP_ITER = KV8_BLOCK / AP_ROWS;
+
+template <bool F32>
+__global__ void __launch_bounds__(AP_THREADS, F32 ? 4 : 6) kv8_append_kernel(const Kv8AppendArgs p) {
+    constexpr int W = F32 ? 8 : 4;                            // words of a thread's eight dimensions
     __shared__ uint32_t wmax[AP_THREADS / 32];
-    __shared__ float blo[AP_THREADS / 32][KV8_HD], bhi[AP_THREADS / 32][KV8_HD];
+    __shared__ uint32_t blo[AP_THREADS / 32][KV8_HD / 2], bhi[AP_THREADS / 32][KV8_HD / 2];
     dep_wait();
     dep_launch();
     const int s = blockIdx.z, kvh = blockIdx.y & 7;
@@ -59,108 +206,109 @@ __global__ void __launch_bounds__(AP_THREADS) kv8_append_kernel(const Kv8AppendA
     const int b = p0 / KV8_BLOCK + blockIdx.x, t_blk = b * KV8_BLOCK;
     const int lo = max(p0, t_blk), hi = min(p0 + p.L, t_blk + KV8_BLOCK);
     if (lo >= hi) return;
-    const size_t plane = p.c.plane(slot, kvh);
+    const size_t plane = p.c.plane(slot, kvh), blk = plane * p.c.nb + b;
     uint8_t *codes = (is_v ? p.c.v : p.c.k) + (plane * p.c.max_len + t_blk) * KV8_HD;
-    float *scale = (is_v ? p.c.vs : p.c.ks) + plane * p.c.nb + b;
+    float *scale = (is_v ? p.c.vs : p.c.ks) + blk;
     const void *src = is_v ? p.v : p.k;
-    const int c8 = (threadIdx.x & 15) * 8, r0 = threadIdx.x >> 4, warp = threadIdx.x >> 5;
+    const int c16 = threadIdx.x & 15, r0 = threadIdx.x >> 4, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
-    float x[AP_ITER][8];
-    uint32_t am = 0;
+    uint32_t x[AP_ITER][W];
 #pragma unroll
     for (int i = 0; i < AP_ITER; i++) {
         const int t = t_blk + r0 + i * AP_ROWS;
-        if (t < lo || t >= hi) continue;
-        load8<F32>(src, ((size_t)s * p.L + (t - p0)) * p.ld + kvh * KV8_HD + c8, x[i]);
+        const size_t o = ((size_t)s * p.L + (t - p0)) * p.ld + kvh * KV8_HD + 8 * c16;
 #pragma unroll
-        for (int j = 0; j < 8; j++) {
-            const uint32_t a = __float_as_uint(x[i][j]) & 0x7FFFFFFFu;
-            am = a < 0x7F800000u ? max(am, a) : am;
+        for (int j = 0; j < W; j++) x[i][j] = 0u;
+        if (t < lo || t >= hi) continue;
+        const uint4 *q = F32 ? (const uint4 *)((const float *)src + o) : (const uint4 *)((const uint16_t *)src + o);
+        const uint4 a = __ldcs(q);
+        x[i][0] = a.x; x[i][1] = a.y; x[i][2] = a.z; x[i][3] = a.w;
+        if constexpr (F32) {
+            const uint4 d = __ldcs(q + 1);
+            x[i][4] = d.x; x[i][5] = d.y; x[i][6] = d.z; x[i][7] = d.w;
         }
     }
-    am = __reduce_max_sync(0xFFFFFFFFu, am);
-    if ((threadIdx.x & 31) == 0) wmax[warp] = am;
     const bool has_old = p0 > t_blk;
     const float s_old = has_old ? *scale : 0.f;
+    uint32_t am = 0;
+#pragma unroll
+    for (int i = 0; i < AP_ITER; i++) am = max(am, abs_max<F32>(x[i]));
+    am = __reduce_max_sync(0xFFFFFFFFu, am);
+    if (lane == 0) wmax[warp] = am;
     __syncthreads();
 #pragma unroll
     for (int w = 0; w < AP_THREADS / 32; w++) am = max(am, wmax[w]);
-    const float s_new = __uint_as_float((uint32_t)(scale_exp(am) + 127) << 23);
-    const float sc = fmaxf(s_old, s_new);
-    const float inv = __uint_as_float((254u << 23) - __float_as_uint(sc));   // 1 / 2^e
-    const float shrink = s_old * inv;
-
-    float mn[8], mx[8];
-#pragma unroll
-    for (int j = 0; j < 8; j++) { mn[j] = INFINITY; mx[j] = -INFINITY; }
+    const float sc = fmaxf(s_old, pow2(scale_exp(am))), inv = inv_pow2(sc), shrink = s_old * inv;
+    const bool want = !is_v && p.c.kb;
+    uint32_t mn[4] = {kHInf, kHInf, kHInf, kHInf}, mx[4] = {kHNegInf, kHNegInf, kHNegInf, kHNegInf};
 #pragma unroll
     for (int i = 0; i < AP_ITER; i++) {
         const int r = r0 + i * AP_ROWS, t = t_blk + r;
-        uint8_t *dst = codes + (size_t)r * KV8_HD + c8;
+        uint2 *dst = (uint2 *)(codes + r * KV8_HD) + c16;
         if (t >= lo && t < hi) {
-            uint32_t w[4];
+            const uint32_t c[2] = {codes4<F32>(x[i], inv), codes4<F32>(x[i] + W / 2, inv)};
+            *dst = make_uint2(c[0], c[1]);
+            if (want)
 #pragma unroll
-            for (int j = 0; j < 4; j++) {
-                w[j] = f32x2_to_e4m3x2(x[i][2 * j] * inv, x[i][2 * j + 1] * inv);
-                const float2 f = e4m3x2_to_f32x2(w[j]);
-                const float a = f.x == f.x ? f.x : 0.f, c = f.y == f.y ? f.y : 0.f;   // NaN counts as 0
-                mn[2 * j] = fminf(mn[2 * j], a);
-                mx[2 * j] = fmaxf(mx[2 * j], a);
-                mn[2 * j + 1] = fminf(mn[2 * j + 1], c);
-                mx[2 * j + 1] = fmaxf(mx[2 * j + 1], c);
-            }
-            *(uint2 *)dst = make_uint2(w[0] | (w[1] << 16), w[2] | (w[3] << 16));
-        } else if (t < lo && has_old && shrink != 1.f) {
-            const uint2 o = *(const uint2 *)dst;
-            uint32_t w[4] = {o.x & 0xFFFFu, o.x >> 16, o.y & 0xFFFFu, o.y >> 16};
-#pragma unroll
-            for (int j = 0; j < 4; j++) {
-                const float2 f = e4m3x2_to_f32x2(w[j]);
-                w[j] = f32x2_to_e4m3x2(f.x * shrink, f.y * shrink);
-            }
-            *(uint2 *)dst = make_uint2(w[0] | (w[1] << 16), w[2] | (w[3] << 16));
+                for (int j = 0; j < 2; j++) {
+                    const uint32_t z = nan_to_zero(c[j]), h0 = e4m3x2_to_f16x2(z & 0xFFFFu), h1 = e4m3x2_to_f16x2(z >> 16);
+                    mn[2 * j] = hmin2(mn[2 * j], h0); mx[2 * j] = hmax2(mx[2 * j], h0);
+                    mn[2 * j + 1] = hmin2(mn[2 * j + 1], h1); mx[2 * j + 1] = hmax2(mx[2 * j + 1], h1);
+                }
+        } else if (t < lo && shrink != 1.f) {                 // (t < lo: the block held positions)
+            const uint2 o = *dst;
+            *dst = make_uint2(shrink4(o.x, shrink), shrink4(o.y, shrink));
         }
     }
     if (threadIdx.x == 0) *scale = sc;
-    if (is_v || !p.c.kb) return;
-    // bounds: over the warp's two rows per pass, then over the warps
+    if (!want) return;
+    // over the warp's two rows per step, then over the warps
 #pragma unroll
-    for (int j = 0; j < 8; j++) {
-        mn[j] = fminf(mn[j], __shfl_xor_sync(0xFFFFFFFFu, mn[j], 16));
-        mx[j] = fmaxf(mx[j], __shfl_xor_sync(0xFFFFFFFFu, mx[j], 16));
-        if ((threadIdx.x & 31) < 16) { blo[warp][c8 + j] = mn[j]; bhi[warp][c8 + j] = mx[j]; }
+    for (int j = 0; j < 4; j++) {
+        mn[j] = hmin2(mn[j], __shfl_xor_sync(0xFFFFFFFFu, mn[j], 16));
+        mx[j] = hmax2(mx[j], __shfl_xor_sync(0xFFFFFFFFu, mx[j], 16));
+    }
+    if (lane < 16) {
+        *(uint4 *)&blo[warp][4 * lane] = make_uint4(mn[0], mn[1], mn[2], mn[3]);
+        *(uint4 *)&bhi[warp][4 * lane] = make_uint4(mx[0], mx[1], mx[2], mx[3]);
     }
     __syncthreads();
-    if (threadIdx.x < KV8_HD) {
+    if (threadIdx.x < KV8_HD / 2) {
         const int d = threadIdx.x;
-        float l = blo[0][d], h = bhi[0][d];
+        uint32_t l = blo[0][d], h = bhi[0][d];
 #pragma unroll
         for (int w = 1; w < AP_THREADS / 32; w++) {
-            l = fminf(l, blo[w][d]);
-            h = fmaxf(h, bhi[w][d]);
+            l = hmin2(l, blo[w][d]);
+            h = hmax2(h, bhi[w][d]);
         }
-        uint8_t *kb = p.c.kb + (plane * p.c.nb + b) * 2 * KV8_HD + d;
+        uint16_t *kb = (uint16_t *)(p.c.kb + blk * 2 * KV8_HD) + d;
         if (has_old) {
-            const float2 o = e4m3x2_to_f32x2((uint32_t)kb[0] | ((uint32_t)kb[KV8_HD] << 8));
-            const uint32_t r = f32x2_to_e4m3x2(o.x * shrink, o.y * shrink);
-            const float2 q = e4m3x2_to_f32x2(r);
-            l = fminf(l, q.x);
-            h = fmaxf(h, q.y);
+            l = hmin2(l, e4m3x2_to_f16x2(shrink4(kb[0], shrink) & 0xFFFFu));
+            h = hmax2(h, e4m3x2_to_f16x2(shrink4(kb[KV8_HD / 2], shrink) & 0xFFFFu));
         }
-        const uint32_t r = f32x2_to_e4m3x2(l, h);
-        kb[0] = (uint8_t)r;
-        kb[KV8_HD] = (uint8_t)(r >> 8);
+        kb[0] = (uint16_t)f16x2_to_e4m3x2(l);
+        kb[KV8_HD / 2] = (uint16_t)f16x2_to_e4m3x2(h);
     }
 }
 
 }  // namespace
 
 int launch_kv8_append(cudaStream_t st, const Kv8AppendArgs &a, bool f32, int n_seqs) {
-    const dim3 grid((a.L + KV8_BLOCK - 2) / KV8_BLOCK + 1, 2 * KV8_NKV, n_seqs);
-    if (f32)
-        N550_CUDA_TRY(launch_k(kv8_append_kernel<true>, grid, AP_THREADS, 0, st, a));
-    else
-        N550_CUDA_TRY(launch_k(kv8_append_kernel<false>, grid, AP_THREADS, 0, st, a));
+    const int n_blk = (a.L + KV8_BLOCK - 2) / KV8_BLOCK + 1;  // blocks that L rows can touch
+    if (a.L <= FEW) {
+        const int items = n_blk * KV8_NKV * n_seqs;
+        const dim3 grid((items + FEW_WARPS - 1) / FEW_WARPS);
+        if (f32)
+            N550_CUDA_TRY(launch_k(kv8_append_few_kernel<true>, grid, FEW_WARPS * 32, 0, st, a, n_blk, items));
+        else
+            N550_CUDA_TRY(launch_k(kv8_append_few_kernel<false>, grid, FEW_WARPS * 32, 0, st, a, n_blk, items));
+    } else {
+        const dim3 grid(n_blk, 2 * KV8_NKV, n_seqs);
+        if (f32)
+            N550_CUDA_TRY(launch_k(kv8_append_kernel<true>, grid, AP_THREADS, 0, st, a));
+        else
+            N550_CUDA_TRY(launch_k(kv8_append_kernel<false>, grid, AP_THREADS, 0, st, a));
+    }
     N550_LAUNCH_CHECK();
     return N550_OK;
 }
