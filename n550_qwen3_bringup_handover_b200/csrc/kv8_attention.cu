@@ -45,9 +45,9 @@ constexpr int STAGE = 4 * BLK;                  // K of two blocks | V of two bl
 
 // What the producer says about a ring stage: one or two blocks of one pair.
 struct __align__(16) Rec {
-    int s, kvh, blk[2], ctx;                    // blk[0] < 0: nothing to read, blk[1] < 0: one block
+    int blk[2], ctx, flags;                     // blk[0] < 0: nothing to read, blk[1] < 0: one block
     float ks[2], vs[2];
-    int flags, slot, pad;                       // partial slot, or -1: the whole pair
+    int s, kvh, slot, pad;                      // partial slot, or -1: the whole pair
 };
 enum { R_FIRST = 1, R_LAST = 2, R_END = 4, R_Q = 8 };   // of a piece, of the run; the piece's first tile
 
@@ -58,10 +58,12 @@ struct Lay {
     int upp;                                    // LAY_EVEN: units per pair
 };
 
-// LT: most query tokens (2 heads each) of an instance. S has 4 columns a token,
-// O (and P) 6; the MMA's column side is a multiple of 16.
+// LT: most query tokens (2 heads each) of an instance. S has 4 columns a token, O
+// (and P) 6, at most 12 of 16 for each softmax group (so that a row of P has the
+// same swizzle in every group).
+template <int LT> constexpr int groups() { return LT == 1 ? 1 : LT / 2; }       // of four softmax warps
 template <int LT> constexpr int s_cols() { return LT == 1 ? 16 : 4 * LT; }
-template <int LT> constexpr int p_cols() { return (6 * LT + 15) / 16 * 16; }
+template <int LT> constexpr int p_cols() { return 16 * groups<LT>(); }
 template <int LT> constexpr int tmem_cols() {
     return 2 * (s_cols<LT>() + p_cols<LT>()) <= 64 ? 64 : 2 * (s_cols<LT>() + p_cols<LT>()) <= 128 ? 128 : 256;
 }
@@ -73,7 +75,6 @@ template <int LT> constexpr int op_bytes() { return 2 * 128 * (s_cols<LT>() + p_
 template <int LT> constexpr int stages() { return LT == 8 ? 4 : 2; }
 template <int LT> constexpr int per_sm() { return LT == 1 ? 3 : LT == 4 ? 2 : 1; }
 template <int LT> constexpr int smem_bytes(int L) { return stages<LT>() * (STAGE + L * 512) + op_bytes<LT>() + 1024; }
-template <int LT> constexpr int groups() { return LT == 1 ? 1 : LT / 2; }       // of four softmax warps
 template <int LT> constexpr int threads() { return (3 + 4 * groups<LT>()) * 32; }
 
 // The pair that a run leaves to the merge: its pieces are in runs c .. c + n - 1.
@@ -276,7 +277,7 @@ kv8_attn_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
     __shared__ Rec rec[ST];
     __shared__ __align__(8) uint64_t full[ST], empty[ST], q_ready[4], q_free[2], s_full[2], p_full[2], pv_done[2], o_free[2], done;
     __shared__ float q_scale[4][NC];            // power of two of each query row, by piece modulo 4
-    __shared__ float xmax[2][4][NC], xsum[2][4][NC];
+    __shared__ __align__(16) float xmax[2][4][NC], xsum[2][4][NC];
     __shared__ int xdead[G][2][4];
     __shared__ uint32_t tmem_slot;
 
@@ -632,7 +633,7 @@ kv8_attn_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
                 for (int c = 0; c < NG; c++) qf[c] = c < ng ? q_scale[piece & 3][c0 + c] : 0.f;
             }
             if (dead || w.blk[0] >= 0) {
-                const uint32_t ts = tS + lane_off + (t & 1) * NS + 2 * c0, to = tO + lane_off + (piece & 1) * NP + 3 * c0;
+                const uint32_t ts = tS + lane_off + (t & 1) * NS + 2 * c0, to = tO + lane_off + (piece & 1) * NP + 16 * grp;
                 const int blk = half ? w.blk[1] : w.blk[0], pos = blk * KV8_BLOCK + (row & 63);
                 const float kf = (half ? w.ks[1] : w.ks[0]) * kKv8ScaleLog2;
                 float s[NG];
@@ -653,48 +654,50 @@ kv8_attn_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
                         }
                     }
                 }
-                const float (*xm)[NC] = xmax[bars & 1];
+                const float (*xm)[NC] = xmax[bars & 1];            // [warp][column]
                 if (meet(dead)) break;
                 // the tile's maximum, and V's scale: O moves when either changes
                 const float vmax = w.blk[1] < 0 ? w.vs[0] : fmaxf(w.vs[0], w.vs[1]);
                 const bool moved = !(vmax <= vref && vmax * 16.f >= vref);
-                const float vmove = moved && tiles ? vref / vmax : 1.f;
-                float corr[NG];
+                float x[NG];
                 bool grow = moved;
 #pragma unroll
                 for (int c = 0; c < NG; c++) {
-                    corr[c] = 1.f;
-                    if (c < ng) {
-                        const float x = fmaxf(fmaxf(xm[0][c0 + c], xm[1][c0 + c]), fmaxf(xm[2][c0 + c], xm[3][c0 + c]));
-                        if (x > m[c]) {
-                            corr[c] = ex2(m[c] - x);
-                            m[c] = x;
-                            l[c] *= corr[c];
-                            grow = true;
-                        }
-                    }
+                    x[c] = fmaxf(fmaxf(xm[0][c0 + c], xm[1][c0 + c]), fmaxf(xm[2][c0 + c], xm[3][c0 + c]));
+                    grow |= c < ng && x[c] > m[c];
                 }
-                if (moved) vref = vmax;
                 bool alive = true;
-                if (grow && tiles) {                               // warp-uniform
-                    // O holds the tiles before: P.V of the last one must have ended
-                    alive = warp_wait(&pv_done[(t - 1) & 1], ((t - 1) >> 1) & 1);
-                    if (alive) {
-                        uint32_t o[(3 * NG + 3) / 4 * 4];
-                        tc_fence_after();
-                        load_cols<3 * NG>(to, o);
+                if (grow) {                                        // warp-uniform
+                    const float vmove = moved && tiles ? vref / vmax : 1.f;
+                    if (moved) vref = vmax;
+                    float corr[NG];
 #pragma unroll
-                        for (int c = 0; c < NG; c++)
+                    for (int c = 0; c < NG; c++) {
+                        const float to_m = c < ng ? fmaxf(m[c], x[c]) : m[c];
+                        corr[c] = to_m > m[c] ? ex2(m[c] - to_m) : 1.f;
+                        m[c] = to_m;
+                        l[c] *= corr[c];
+                    }
+                    if (tiles) {
+                        // O holds the tiles before: P.V of the last one must have ended
+                        alive = warp_wait(&pv_done[(t - 1) & 1], ((t - 1) >> 1) & 1);
+                        if (alive) {
+                            uint32_t o[(3 * NG + 3) / 4 * 4];
+                            tc_fence_after();
+                            load_cols<3 * NG>(to, o);
 #pragma unroll
-                            for (int k = 0; k < 3; k++)
-                                o[3 * c + k] = __float_as_uint(__uint_as_float(o[3 * c + k]) * (corr[c] * vmove));
-                        store_cols<3 * NG>(to, o);
+                            for (int c = 0; c < NG; c++)
+#pragma unroll
+                                for (int k = 0; k < 3; k++)
+                                    o[3 * c + k] = __float_as_uint(__uint_as_float(o[3 * c + k]) * (corr[c] * vmove));
+                            store_cols<3 * NG>(to, o);
+                        }
                     }
                 }
                 // this buffer of P was read by P.V of two tiles ago
                 if (alive && t >= 2) alive = warp_wait(&pv_done[t & 1], ((t - 2) >> 1) & 1);
                 if (alive) {
-                    uint8_t *dst = sP + (t & 1) * NP * 128;
+                    uint8_t *dst = sP + ((t & 1) * NP + 16 * grp) * 128;
                     const float ratio = blk < 0 ? 0.f : 256.f * ((half ? w.vs[1] : w.vs[0]) / vref);
 #pragma unroll
                     for (int c = 0; c < NG; c += 2) {
@@ -708,8 +711,8 @@ kv8_attn_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
 #pragma unroll
                         for (int k = 0; k < 3; k++) {
                             const uint32_t e = f32x2_to_e4m3x2(a, b);
-                            dst[sw(3 * (c0 + c) + k, row)] = (uint8_t)e;
-                            dst[sw(3 * (c0 + c) + 3 + k, row)] = (uint8_t)(e >> 8);
+                            dst[sw(3 * c + k, row)] = (uint8_t)e;
+                            dst[sw(3 * c + 3 + k, row)] = (uint8_t)(e >> 8);
                             const float2 f = e4m3x2_to_f32x2(e);
                             a = (a - f.x) * 16.f;
                             b = (b - f.y) * 16.f;
@@ -736,7 +739,7 @@ kv8_attn_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
             }
 
             // ---------------- the piece ends ----------------
-            const uint32_t to = tO + lane_off + (piece & 1) * NP + 3 * c0;
+            const uint32_t to = tO + lane_off + (piece & 1) * NP + 16 * grp;
             uint32_t o[(3 * NG + 3) / 4 * 4];
 #pragma unroll
             for (int c = 0; c < (3 * NG + 3) / 4 * 4; c++) o[c] = 0u;
