@@ -22,7 +22,7 @@
 namespace n550 {
 namespace {
 
-constexpr int SL_THREADS = 256;
+constexpr int SL_THREADS = 512;                 // one CTA per SM by registers: 32 doubles of query a lane
 constexpr int SL_WARPS = SL_THREADS / 32;
 constexpr int SL_STEP = 16;                     // blocks a warp scores at a time
 
@@ -39,6 +39,12 @@ __device__ __forceinline__ unsigned long long order_key(double x) {
     return b >> 63 ? ~b : b | 1ull << 63;
 }
 
+__device__ __forceinline__ void min_cluster_u32(uint32_t addr, unsigned int v) {
+    asm volatile("red.relaxed.cluster.shared::cluster.min.u32 [%0], %1;" ::"r"(addr), "r"(v) : "memory");
+}
+__device__ __forceinline__ void max_cluster_u32(uint32_t addr, unsigned int v) {
+    asm volatile("red.relaxed.cluster.shared::cluster.max.u32 [%0], %1;" ::"r"(addr), "r"(v) : "memory");
+}
 __device__ __forceinline__ void st_cluster_u64(uint32_t addr, unsigned long long v) {
     asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(addr), "l"(v) : "memory");
 }
@@ -47,7 +53,8 @@ __device__ __forceinline__ void st_cluster_u64(uint32_t addr, unsigned long long
 __global__ void __launch_bounds__(SL_THREADS) kv8_select_kernel(const Kv8SelectArgs p) {
     extern __shared__ unsigned long long key[];                // [nb] in the cluster's first CTA
     __shared__ unsigned int hist[256];
-    __shared__ unsigned long long wmin[SL_WARPS], wmax[SL_WARPS], found;   // found: digit and counts
+    __shared__ unsigned int range[2];                          // upper halves of the least and largest key that is not forced
+    __shared__ unsigned long long found;                       // digit and counts
     __shared__ int wgt[SL_WARPS], weq[SL_WARPS];
     dep_wait();
     dep_launch();
@@ -62,7 +69,9 @@ __global__ void __launch_bounds__(SL_THREADS) kv8_select_kernel(const Kv8SelectA
         return;
     }
     const size_t plane = p.c.plane(slot, kvh);
-    cluster_arrive_relaxed();                                  // (the first CTA must be there before it is written to)
+    if (threadIdx.x == 0) { range[0] = ~0u; range[1] = 0u; }
+    cluster_arrive();                                          // the first CTA is there before it is written to
+    const int f0 = p.n_sink, f1 = nb - p.n_recent;             // forced: b < f0 or b >= f1 (n_sink + n_recent <= n_select < nb)
 
     // ---------------- scores: lane l the dimensions 16 (l % 8) .. of block l / 8 of 4 ----------------
     {
@@ -89,6 +98,7 @@ __global__ void __launch_bounds__(SL_THREADS) kv8_select_kernel(const Kv8SelectA
         }
         const uint32_t dst = mapa_shared(smem_u32(key), 0);
         cluster_wait();
+        unsigned int least = ~0u, most = 0u;
         const uint8_t *kb = p.c.kb + plane * p.c.nb * 2 * KV8_HD;
         const float *ks = p.c.ks + plane * p.c.nb;
         for (int b0 = (rank * SL_WARPS + warp) * SL_STEP; b0 < nb; b0 += cs * SL_WARPS * SL_STEP) {
@@ -129,37 +139,33 @@ __global__ void __launch_bounds__(SL_THREADS) kv8_select_kernel(const Kv8SelectA
                 if ((lane & 7) == 0 && b < nb) {
                     double v = fmax(a[0], a[1]) * 0x1p496 * (double)sc[j];
                     if (!(v == v)) v = -INFINITY;
-                    st_cluster_u64(dst + 8u * b, order_key(v));
+                    const unsigned long long x = order_key(v);
+                    st_cluster_u64(dst + 8u * b, x);
+                    if (b >= f0 && b < f1) {
+                        least = min(least, (unsigned int)(x >> 32));
+                        most = max(most, (unsigned int)(x >> 32));
+                    }
                 }
             }
+        }
+        if ((lane & 7) == 0 && least <= most) {
+            const uint32_t r = mapa_shared(smem_u32(range), 0);
+            min_cluster_u32(r, least);
+            max_cluster_u32(r + 4, most);
         }
     }
     cluster_sync();
     if (rank) return;
 
     // ---------------- the n_rest largest of the blocks that are not forced ----------------
-    const int f0 = p.n_sink, f1 = nb - p.n_recent;             // forced: b < f0 or b >= f1 (n_sink + n_recent <= n_select < nb)
-    unsigned long long lo = ~0ull, hi = 0;
-    for (int b = f0 + threadIdx.x; b < f1; b += SL_THREADS) {
-        lo = min(lo, key[b]);
-        hi = max(hi, key[b]);
-    }
-#pragma unroll
-    for (int x = 16; x > 0; x >>= 1) {
-        lo = min(lo, __shfl_xor_sync(0xFFFFFFFFu, lo, x));
-        hi = max(hi, __shfl_xor_sync(0xFFFFFFFFu, hi, x));
-    }
-    if (lane == 0) { wmin[warp] = lo; wmax[warp] = hi; }
-    __syncthreads();
-#pragma unroll
-    for (int w = 0; w < SL_WARPS; w++) { lo = min(lo, wmin[w]); hi = max(hi, wmax[w]); }
+    const unsigned int lo = range[0], hi = range[1];           // (some block is not forced: nb > n_select)
     int k = p.n_select - p.n_sink - p.n_recent;                // still to take among those equal to `at` above `bits`
-    int bits = lo == hi ? 0 : 64 - __clzll(lo ^ hi);           // key bits not decided yet
-    unsigned long long at = bits == 64 ? 0 : hi >> bits;       // the decided bits of the k-th largest key
+    int bits = 64 - __clz(lo ^ hi);                            // key bits not decided yet (32 when the halves are equal)
+    unsigned long long at = bits == 64 ? 0 : (unsigned long long)hi << 32 >> bits;   // the decided bits of the k-th largest key
     bool done = k == 0;
     while (bits > 0 && !done) {
         const int take = min(bits, 8), rest = bits - take;
-        hist[threadIdx.x] = 0;
+        if (threadIdx.x < 256) hist[threadIdx.x] = 0;
         __syncthreads();
         for (int b = f0 + threadIdx.x; b < f1; b += SL_THREADS) {
             const unsigned long long x = key[b];
@@ -179,18 +185,15 @@ __global__ void __launch_bounds__(SL_THREADS) kv8_select_kernel(const Kv8SelectA
             }
             before -= sum;                                     // keys with larger digits
             if ((int)before < k && (int)(before + sum) >= k) {
-                int i = 0;
-                unsigned int c = 0;
+                int i = 0;                                     // the first digit that reaches k
+                unsigned int above = before, c = n[0];
 #pragma unroll
-                for (int j = 7; j >= 0; j--) {                 // the first digit that reaches k
-                    unsigned int run = 0;
-#pragma unroll
-                    for (int m = 0; m <= j; m++) run += n[m];
-                    if ((int)(before + run) >= k) { i = j; c = n[j]; }
-                }
-                unsigned int above = before;
-#pragma unroll
-                for (int m = 0; m < 8; m++) above += m < i ? n[m] : 0;
+                for (int m = 1; m < 8; m++)
+                    if ((int)(above + c) < k) {
+                        above += c;
+                        c = n[m];
+                        i = m;
+                    }
                 found = (unsigned long long)(255 - 8 * lane - i) | (unsigned long long)above << 8 | (unsigned long long)c << 32;
             }
         }
@@ -246,7 +249,9 @@ int launch_kv8_select(cudaStream_t st, const Kv8SelectArgs &a) {
         attr[dev] = true;
     }
     const int pairs = a.n_seqs * KV8_NKV;
-    const int cs = pairs <= 32 ? 8 : pairs <= 64 ? 4 : pairs <= 256 ? 2 : 1;
+    // as many CTAs as fit the 148 SMs at once, up to the portable 8 per cluster (128 pairs:
+    // 13 us in clusters of 1, 21 in clusters of 4; 8 pairs: 37 us in clusters of 1, 13 of 8)
+    const int cs = pairs <= 18 ? 8 : pairs <= 37 ? 4 : pairs <= 74 ? 2 : 1;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(cs, KV8_NKV, a.n_seqs);
     cfg.blockDim = dim3(SL_THREADS);
