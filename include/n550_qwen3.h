@@ -276,8 +276,8 @@ size_t n550_attention_decode_workspace(int n_seqs, int max_len);
  *                     (NULL: not kept; n550_kv8_select_blocks needs them)
  * A value is its code times its block's scale, which BF16 holds exactly. k, v
  * and k_bounds are 16-byte aligned. Nothing needs to be initialised:
- * n550_kv8_append defines what later calls read. max_len need not be a multiple
- * of the block.
+ * n550_kv8_append defines what later calls read. max_len (up to 2^30) need not be
+ * a multiple of the block.
  *
  * seq_ids and pos are device int32 arrays, as for the BF16 cache. A slot id
  * outside the cache or a negative position makes a sequence empty: append
@@ -316,7 +316,8 @@ int n550_kv8_append(void *stream, const n550_kv8_cache *c, int layer, const void
  * position pos[s], q [n_seqs][ldq >= 2048] BF16, out [n_seqs][ldo >= 2048] BF16.
  * workspace may be NULL (one CTA per sequence and KV head) or
  * n550_attention_kv8_workspace(n_seqs) bytes, 16-byte aligned, not shared by calls
- * that can overlap; its contents before and after a call mean nothing. */
+ * that can overlap; its contents before and after a call mean nothing (a
+ * smaller or unaligned one counts as NULL). */
 int n550_attention_decode_kv8(void *stream, const uint16_t *q, int ldq, const n550_kv8_cache *c,
                               int layer, const int32_t *seq_ids, const int32_t *pos, int n_seqs,
                               uint16_t *out, int ldo, void *workspace, size_t workspace_bytes);
@@ -324,8 +325,10 @@ size_t n550_attention_kv8_workspace(int n_seqs);
 
 /* n550_attention_prefill over the 8-bit cache: n_seqs x L queries at positions
  * pos0 .. pos0+L-1 whose K/V were appended, causal; q and out [n_seqs*L] rows.
- * workspace may be NULL (slower) or
- * n550_attention_prefill_kv8_workspace(n_seqs, L, pos0) bytes, as above. */
+ * As in the BF16 prefill, a NaN in the V of one of these L positions also reaches
+ * that dimension of the queries before it. workspace may be NULL (slower) or
+ * n550_attention_prefill_kv8_workspace(n_seqs, L, pos0) bytes, as above; from 9
+ * queries on it holds the context as BF16, 4096 bytes per sequence and position. */
 int n550_attention_prefill_kv8(void *stream, const uint16_t *q, int ldq, const n550_kv8_cache *c,
                                int layer, const int32_t *seq_ids, int n_seqs, int L, int pos0,
                                uint16_t *out, int ldo, void *workspace, size_t workspace_bytes);
@@ -349,7 +352,7 @@ int n550_kv8_select_blocks(void *stream, const uint16_t *q, int ldq, const n550_
 
 /* n550_attention_decode_kv8 over listed blocks only: sequence s and KV head h
  * attend to those positions <= pos[s] that lie in the blocks blocks[s][h][0 ..
- * n_select). Entries that are negative or past the context are skipped; a block
+ * n_select) (n_select <= 2^24). Entries that are negative or past the context are skipped; a block
  * listed twice counts twice; with no position left the rows are zero. */
 int n550_attention_sparse_kv8(void *stream, const uint16_t *q, int ldq, const n550_kv8_cache *c,
                               int layer, const int32_t *seq_ids, const int32_t *pos,

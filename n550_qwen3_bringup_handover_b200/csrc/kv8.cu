@@ -6,7 +6,7 @@ namespace n550 {
 
 int kv8_view(const n550_kv8_cache *c, int layer, Kv8View *v) {
     if (!c || !c->k || !c->v || !c->k_scale || !c->v_scale || c->n_slots <= 0 || c->n_layers <= 0 ||
-        c->max_len <= 0 || layer < 0 || layer >= c->n_layers ||
+        c->max_len <= 0 || c->max_len > 1 << 30 || layer < 0 || layer >= c->n_layers ||
         (((uintptr_t)c->k | (uintptr_t)c->v | (uintptr_t)c->k_bounds) & 15) ||
         (((uintptr_t)c->k_scale | (uintptr_t)c->v_scale) & 3) ||
         (long long)c->n_slots * c->n_layers * KV8_NKV > (1LL << 31) - 1)

@@ -193,8 +193,8 @@ __device__ __forceinline__ long long locate(const Kv8AttnArgs &p, const Lay lay,
     constexpr int ROUND = 8;
     const int lane = threadIdx.x & 31;
     int ctx[ROUND], sum[ROUND];
-    auto round = [&](int s0) -> int {            // returns the round's units
-        int all = 0;
+    auto round = [&](int s0) -> long long {      // returns the round's units
+        long long all = 0;
 #pragma unroll
         for (int i = 0; i < ROUND; i++) ctx[i] = s0 + 32 * i + lane < p.n_seqs ? seq_ctx(p, s0 + 32 * i + lane) : -KV8_BLOCK;
 #pragma unroll
@@ -212,21 +212,22 @@ __device__ __forceinline__ long long locate(const Kv8AttnArgs &p, const Lay lay,
     long long base = 0;                          // units before the round that holds u
     if (p.n_seqs > 32 * ROUND)
         for (;; s0 += 32 * ROUND) {
-            const int n = round(s0);
+            const long long n = round(s0);
             if (u < base + n) break;
             base += n;
         }
-    int x = (int)(u - base), mine = ctx[0];
-    bool found = x < sum[0];
+    long long rest = u - base;
+    int mine = ctx[0];
+    bool found = rest < sum[0];
 #pragma unroll
     for (int i = 1; i < ROUND; i++)
         if (!found) {
-            x -= sum[i - 1];
+            rest -= sum[i - 1];
             s0 += 32;
             mine = ctx[i];
-            found = x < sum[i];
+            found = rest < sum[i];
         }
-    const int n = mine < 0 ? 0 : ctx_blocks(mine) * KV8_NKV;
+    const int x = (int)rest, n = mine < 0 ? 0 : ctx_blocks(mine) * KV8_NKV;
     int end = n;
 #pragma unroll 1
     for (int o = 1; o < 32; o <<= 1) {
@@ -408,13 +409,14 @@ kv8_attn_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
                 seen = __shfl_sync(0xFFFFFFFFu, earlier || tile, 31);
             }
             // Lanes 2 i and 2 i + 1 share a stage where both hold a block of one piece
-            // and V's scales are near enough for weights in one scale (2^6: the
-            // smaller block's weights keep 2^-20 of their own largest).
+            // and V's scales are near enough for weights in one scale (a factor 8; with
+            // the 4 that O's scale may lag, small weights are multiples of 2^-20 of
+            // the largest instead of 2^-25).
             const int blk = __shfl_down_sync(0xFFFFFFFFu, me.blk[0], 1), fl = __shfl_down_sync(0xFFFFFFFFu, me.flags, 1);
             const float ks = __shfl_down_sync(0xFFFFFFFFu, me.ks[0], 1), vs = __shfl_down_sync(0xFFFFFFFFu, me.vs[0], 1);
             bool two = false;
             if (!(lane & 1) && i + 1 < n_units && me.blk[0] >= 0 && blk >= 0 && !(fl & R_FIRST) &&
-                fmaxf(vs, me.vs[0]) <= 64.f * fminf(vs, me.vs[0])) {
+                fmaxf(vs, me.vs[0]) <= 8.f * fminf(vs, me.vs[0])) {
                 two = true;
                 me.blk[1] = blk;
                 me.ks[1] = ks;
@@ -658,7 +660,7 @@ kv8_attn_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
                 if (meet(dead)) break;
                 // the tile's maximum, and V's scale: O moves when either changes
                 const float vmax = w.blk[1] < 0 ? w.vs[0] : fmaxf(w.vs[0], w.vs[1]);
-                const bool moved = !(vmax <= vref && vmax * 16.f >= vref);
+                const bool moved = !(vmax <= vref && vmax * 4.f >= vref);
                 float x[NG];
                 bool grow = moved;
 #pragma unroll

@@ -93,13 +93,14 @@ class Cache:
     def context(self, slot, pos):
         return 0 if not 0 <= slot < self.n_slots or pos < 0 else min(pos, self.max_len - 1) + 1
 
-    def attend(self, q, seq_ids, pos, L=1, blocks=None):
-        """(out, mass) [n * L, 2048] binary64: mass_d = sum_t (softmax_t + 2^-15) |v_td|,
+    def attend(self, q, seq_ids, pos, L=1, blocks=None, floor=2.0 ** -15):
+        """(out, mass) [n * L, 2048] binary64: mass_d = sum_t (softmax_t + floor) |v_td|,
         the scale that a rounding of the weights acts on: a weight rounded
         relative to itself moves out by that part of the first term, and one
         rounded to a multiple of 2^-25 of the largest weight (small ones are; half
         a step is 2^-26, and the weights' sum is at least the largest) by at most
-        2^-26 |v_td|, which 2^-11 of the second term covers."""
+        2^-26 |v_td|, which 2^-11 of the second term covers. (Where V's block scales
+        differ the multiple is up to 2^-20, and floor has to be 2^-10.)"""
         n = len(seq_ids)
         q = q[:, :HEADS * HD].double().cpu().view(n, L, HEADS, HD)
         out = torch.zeros((n, L, HEADS, HD), dtype=torch.float64)
@@ -118,7 +119,7 @@ class Cache:
                     k, v = self.dequant("k", slot, h, t), self.dequant("v", slot, h, t)
                     w = torch.softmax(q[i, j, 2 * h:2 * h + 2] @ k.T * 0.08838834764831845, -1)
                     out[i, j, 2 * h:2 * h + 2] = w @ v
-                    mass[i, j, 2 * h:2 * h + 2] = (w + 2.0 ** -15) @ v.abs()
+                    mass[i, j, 2 * h:2 * h + 2] = (w + floor) @ v.abs()
         return out.view(n * L, -1), mass.view(n * L, -1)
 
     def select(self, q, seq_ids, pos, n_select, n_sink, n_recent):

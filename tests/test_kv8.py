@@ -32,7 +32,7 @@ def calls(L, cache, layer=0, ptr=P, ld=2048, n=1, rows=4):
 
 @pytest.mark.parametrize("bad", [
     dict(k=None), dict(v=None), dict(k_scale=None), dict(v_scale=None), dict(k=4104), dict(v=4097),
-    dict(k_bounds=4100), dict(k_scale=4098), dict(n_slots=0), dict(n_layers=0), dict(max_len=0), dict(max_len=-5),
+    dict(k_bounds=4100), dict(k_scale=4098), dict(n_slots=0), dict(n_layers=0), dict(max_len=0), dict(max_len=-5), dict(max_len=(1 << 30) + 1),
     dict(n_slots=1 << 20, n_layers=1 << 10),
 ])
 def test_bad_caches_are_refused(bad):
@@ -58,6 +58,8 @@ def test_bad_calls_are_refused():
     assert L.n550_attention_prefill_kv8(None, P, 2048, c, 0, P, 1, 4, 2147483647, P, 2048, None, 0) == n5.ERR_ARG
     # sparse: a negative list length
     assert L.n550_attention_sparse_kv8(None, P, 2048, c, 0, P, P, P, -1, 1, P, 2048, None, 0) == n5.ERR_ARG
+    assert L.n550_attention_sparse_kv8(None, P, 2048, c, 0, P, P, P, (1 << 24) + 1, 1, P, 2048, None, 0) == n5.ERR_ARG
+    assert L.n550_attention_sparse_kv8(None, P, 2048, c, 0, P, P, None, 2, 1, P, 2048, None, 0) == n5.ERR_ARG
     # select: counts, a cache without bounds, too long a cache
     for n_select, sink, recent in [(0, 0, 0), (4, 3, 2), (4, -1, 2), (4, 1, -1), (4, 2147483647, 2147483647)]:
         assert L.n550_kv8_select_blocks(None, P, 2048, c, 0, P, P, 1, n_select, sink, recent, P) == n5.ERR_ARG

@@ -228,9 +228,95 @@ def test_decode_ragged_long_contexts():
         assert_near(out[s], (w @ v).view(-1).cpu(), (w @ v.abs()).view(-1).cpu())
 
 
+@pytest.mark.parametrize("n", [33, 300, 700])
+def test_decode_many_sequences(n):
+    """More sequences than a warp, than one round of the run search, and than two;
+    empty ones among them, also in rows and at both ends."""
+    c, ref = filled(4, 210, 75)
+    g = gen(n)
+    pos = torch.randint(-1, 210, (n,), generator=g).tolist()
+    pos[:9] = [-1] * 9
+    pos[-4:] = [-1] * 4
+    pos[20:31] = [-1] * 11
+    ids = torch.randint(0, 4, (n,), generator=g).tolist()
+    q = rows(n, 2048, torch.bfloat16, 76).cuda()
+    a = n5.attention_decode_kv8(q, c, i32(ids), i32(pos), 1)
+    b = n5.attention_decode_kv8(q, c, i32(ids), i32(pos), 1, split=False)
+    some = sorted(set(torch.randint(0, n, (25,), generator=g).tolist()) | {0, 9, 25, n - 1, n - 5})
+    for out in (a, b):
+        assert_near(out[some], *ref.attend(q[some].cpu(), [ids[i] for i in some], [pos[i] for i in some]))
+        assert (out[[i for i in range(n) if pos[i] < 0]] == 0).all()
+    # split or not, a row differs by the order of its sums alone (two roundings to BF16)
+    assert ((a.float() - b.float()).abs() <= 2.0 ** -7 * b.float().abs() + 2.0 ** -9).all()
+
+
+def test_decode_with_block_scales_far_apart():
+    """V (and K) of each block in a magnitude of its own: tiles of one block, and an
+    accumulator that changes its scale up and down."""
+    max_len = 64 * 14 + 9
+    g = gen(77)
+    size = torch.exp2(torch.randint(-20, 21, (15,), generator=g).float()).repeat_interleave(64)[:max_len, None]
+    c = fresh(1, max_len)
+    k, v = rows(max_len, 1024, torch.float32, 78), rows(max_len, 1024, torch.float32, 79) * size
+    n5.kv8_append(c, k.cuda(), v.cuda(), i32([0]), i32([0]), max_len, 1)
+    ref = Cache.of(c, 1)
+    q = rows(3, 2048, torch.bfloat16, 80, 2.0)
+    pos = [max_len - 1, 500, 320]
+    for split in (True, False):
+        out = n5.attention_decode_kv8(q.cuda(), c, i32([0] * 3), i32(pos), 1, split=split)
+        assert_near(out, *ref.attend(q, [0] * 3, pos, floor=2.0 ** -10))
+    out = n5.attention_prefill_kv8(q[:3].cuda(), c, i32([0]), 3, 700, 1)
+    assert_near(out, *ref.attend(q, [0], [700], 3, floor=2.0 ** -10))
+
+
+def test_decode_nan_stays_in_its_place():
+    c, ref = filled(1, 200, 82)
+    v = c.v.view(torch.uint8)
+    v[0, 1, 3, 77, 5] = 0x7F                                # V, KV head 3, position 77, dimension 5
+    c.k.view(torch.uint8)[0, 1, 6, 150, 9] = 0xFF           # K, KV head 6, position 150
+    q = rows(4, 2048, torch.bfloat16, 83)
+    q[3, 128] = float("nan")                                # head 1 of the last query
+    q[2, 0] = float("inf")                                  # head 0 of the third
+    pos = [199, 76, 149, 199]
+    out = n5.attention_decode_kv8(q.cuda(), c, i32([0] * 4), i32(pos), 1)
+    bad = torch.zeros((4, 16, 128), dtype=torch.bool)
+    bad[0, 6:8, 5] = bad[2, 6:8, 5] = bad[3, 6:8, 5] = True
+    bad[0, 12:14] = bad[3, 12:14] = True
+    bad[3, 1] = True
+    bad[2, 0] = True
+    assert torch.equal(out.view(4, 16, 128).isnan().cpu(), bad)
+    want, mass = ref.attend(q.nan_to_num(nan=0.0, posinf=0.0), [0] * 4, pos)
+    good = ~bad.view(4, -1)
+    err = (out.double().cpu() - want).abs()
+    assert (err <= 2.0 ** -8 * want.abs() + HALF * mass)[good].all()
+
+
 # ---------------------------------------------------------------------------
 # prefill
 # ---------------------------------------------------------------------------
+@pytest.mark.parametrize("n,L", [(1, 2), (2, 3), (3, 4), (2, 5), (1, 8), (40, 6)])
+def test_few_queries_over_long_contexts(n, L):
+    """Contexts cut into many runs: against a binary64 product on the GPU."""
+    pos0 = 6000 if n < 10 else 700
+    c = fresh(2, pos0 + L, n_layers=1)
+    for s in range(2):
+        k, v = rows(pos0 + L, 1024, torch.float32, 250 + s).cuda(), rows(pos0 + L, 1024, torch.float32, 260 + s).cuda()
+        n5.kv8_append(c, k, v, i32([s]), i32([0]), pos0 + L, 0)
+    ids = [(s + 1) % 2 for s in range(n)]
+    q = rows(n * L, 2048, torch.bfloat16, 270).cuda()
+    out = n5.attention_prefill_kv8(q, c, i32(ids), L, pos0, 0)
+    t = torch.arange(pos0 + L, device="cuda")
+    for i, s in enumerate(ids[:4]):
+        k = c.k[s, 0].double() * c.k_scale[s, 0][:, t // BLOCK, None].double()
+        v = c.v[s, 0].double() * c.v_scale[s, 0][:, t // BLOCK, None].double()
+        x = q[i * L:(i + 1) * L].double().view(L, 8, 2, 128).permute(1, 2, 0, 3).reshape(8, 2 * L, 128)
+        w = (x @ k.transpose(1, 2) * 0.08838834764831845).view(8, 2, L, -1)
+        w = torch.softmax(w.masked_fill(t > pos0 + torch.arange(L, device="cuda")[:, None], float("-inf")), -1)
+        want, mass = ((w.view(8, 2 * L, -1) @ y).view(8, 2, L, 128).permute(2, 0, 1, 3).reshape(L, -1).cpu()
+                      for y in (v, v.abs()))
+        assert_near(out[i * L:(i + 1) * L], want, mass)
+
+
 @pytest.mark.parametrize("workspace", [True, False])
 @pytest.mark.parametrize("n,L,pos0", [
     (1, 1, 0), (3, 1, 131), (2, 2, 62), (3, 3, 126), (2, 4, 63), (2, 5, 0), (1, 8, 190), (2, 9, 100), (1, 16, 7),
@@ -355,6 +441,30 @@ def test_sparse_matches_definition(split):
     empty = n5.attention_sparse_kv8(q.cuda(), c, i32(ids), i32(pos), blocks[:, :, :0].contiguous().cuda(), 1,
                                     split=split)
     assert (empty == 0).all()
+
+
+@pytest.mark.parametrize("split", [True, False])
+def test_sparse_long_lists_with_holes(split):
+    """Lists of several batches of 32 entries, with whole batches of nothing."""
+    c, ref = filled(2, 2000, 340)
+    ids, pos = [1, 0, 1], [1999, 1200, 100]
+    q = rows(3, 2048, torch.bfloat16, 341)
+    n_select = 150
+    g = gen(9)
+    blocks = torch.full((3, 8, n_select), -1, dtype=torch.int32)
+    for s in range(3):
+        for h in range(8):
+            at = torch.randperm(n_select, generator=g)[:[0, 1, 3, 20, 32, 32, 5, 12][h]]
+            if h == 4:
+                at = torch.arange(118, 150)                      # the last batches alone
+            if h == 5:
+                at = torch.arange(0, 32)                         # the first alone
+            if h == 6:
+                at = torch.tensor([31, 32, 63, 64, 149])
+            blocks[s, h, at] = torch.randperm(32, generator=g)[:at.numel()].to(torch.int32)
+    out = n5.attention_sparse_kv8(q.cuda(), c, i32(ids), i32(pos), blocks.cuda(), 1, split=split)
+    assert_near(out, *ref.attend(q, ids, pos, blocks=blocks.tolist()))
+    assert n5.device_status() == n5.OK
 
 
 def test_sparse_over_all_blocks_is_decode():
