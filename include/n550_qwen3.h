@@ -453,6 +453,19 @@ int n550_qwen3_fused_attention_prep(int on);
  * summation order. */
 int n550_qwen3_fused_decode(int on);
 
+/* Holds the model's KV cache as the 8-bit cache (n550_kv8_cache: e4m3 codes, half
+ * the bytes a decode step reads) instead of BF16 (on = 1), or goes back (0, the
+ * default). Either way the cache starts empty: call it before the first prefill.
+ * Synchronises and allocates; the other cache's memory is freed. The q/k/v step
+ * then runs as GEMM, row kernel (QK-norm, RoPE) and n550_kv8_append, the attention
+ * as n550_attention_decode_kv8 / n550_attention_prefill_kv8. Fast mode only
+ * (N550_ERR_UNSUPPORTED otherwise, and for a forward with the tensor dump on).
+ * n550_qwen3_kv8_cache gives the cache of such a model (28 layers, max_seqs slots)
+ * for calls of the entry points above, N550_ERR_ARG without one. No counterpart
+ * in the reference. */
+int n550_qwen3_use_kv8(n550_model_t *m, int on);
+int n550_qwen3_kv8_cache(const n550_model_t *m, n550_kv8_cache *c);
+
 /* Per-op tensor dump (qwen3_set_dump / EMIT, qwen3.h:169-184, qwen3.c:464-575):
  * while fn is set, n550_qwen3_forward_batch_host runs the forward op by op with
  * every intermediate tensor materialised and calls fn(ctx, layer, name, data,

@@ -124,6 +124,8 @@ def lib() -> C.CDLL:
         "n550_qwen3_split_rows": (i, [i]),
         "n550_qwen3_set_dump": (i, [vp, vp, vp]),
         "n550_qwen3_fused_decode": (i, [i]),
+        "n550_qwen3_use_kv8": (i, [vp, i]),
+        "n550_qwen3_kv8_cache": (i, [vp, C.POINTER(KV8CacheStruct)]),
         "n550_qwen3_fused_attention_prep": (i, [i]),
         "n550_qwen3_forward_rows": (i, [vp, vp, vp, vp, i, i, vp, vp]),
         "n550_qwen3_forward_rows_host": (i, [vp, vp, i, i, vp, vp]),

@@ -62,7 +62,9 @@ struct Kv8AppendArgs {
     Kv8View c;
     const void *k, *v;         // rows [n_seqs * L][ld], KV head h at columns 128 h ..
     int ld, L;
-    const int32_t *seq_ids, *pos;
+    const int32_t *seq_ids;
+    const int32_t *pos;        // first position per sequence, or NULL: pos0 for all
+    int pos0;
 };
 
 struct Kv8AttnArgs {

@@ -115,7 +115,7 @@ __global__ void __launch_bounds__(FEW_WARPS * 32) kv8_append_few_kernel(const Kv
     dep_launch();
     if (item >= n_items) return;
     const int kvh = item & 7, s = (item >> 3) / n_blk, nth = (item >> 3) % n_blk;
-    const int slot = p.seq_ids[s], p0 = p.pos[s];
+    const int slot = p.seq_ids[s], p0 = p.pos ? p.pos[s] : p.pos0;
     if (slot < 0 || slot >= p.c.n_slots || p0 < 0 || p0 > p.c.max_len - p.L) return;
     const int b = p0 / KV8_BLOCK + nth, t_blk = b * KV8_BLOCK;
     const int lo = max(p0, t_blk), hi = min(p0 + p.L, t_blk + KV8_BLOCK), n = hi - lo;
@@ -201,7 +201,7 @@ __global__ void __launch_bounds__(AP_THREADS, F32 ? 4 : 6) kv8_append_kernel(con
     dep_launch();
     const int s = blockIdx.z, kvh = blockIdx.y & 7;
     const bool is_v = blockIdx.y >= 8;
-    const int slot = p.seq_ids[s], p0 = p.pos[s];
+    const int slot = p.seq_ids[s], p0 = p.pos ? p.pos[s] : p.pos0;
     if (slot < 0 || slot >= p.c.n_slots || p0 < 0 || p0 > p.c.max_len - p.L) return;
     const int b = p0 / KV8_BLOCK + blockIdx.x, t_blk = b * KV8_BLOCK;
     const int lo = max(p0, t_blk), hi = min(p0 + p.L, t_blk + KV8_BLOCK);

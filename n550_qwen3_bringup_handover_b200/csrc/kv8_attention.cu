@@ -700,7 +700,7 @@ kv8_attn_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
                 if (alive && t >= 2) alive = warp_wait(&pv_done[t & 1], ((t - 2) >> 1) & 1);
                 if (alive) {
                     uint8_t *dst = sP + ((t & 1) * NP + 16 * grp) * 128;
-                    const float ratio = blk < 0 ? 0.f : 256.f * ((half ? w.vs[1] : w.vs[0]) / vref);
+                    const float ratio = blk < 0 || vref == 0.f ? 0.f : 256.f * ((half ? w.vs[1] : w.vs[0]) / vref);
 #pragma unroll
                     for (int c = 0; c < NG; c += 2) {
                         if (c >= ng) break;

@@ -31,6 +31,7 @@
 #include "decode_fused.h"
 #include "gemm_skinny.h"
 #include "gemm_tc.h"
+#include "kv8.h"
 #include "launch.h"
 #include "ops.h"
 #include "synth.cuh"
@@ -177,6 +178,10 @@ __global__ void synth_bf16_kernel(uint16_t *out, size_t n, uint64_t key, float s
         out[i] = f32_to_bf16_rne(synth_normal(synth_u64(key, i), scale));
 }
 
+__global__ void fill_f32_kernel(float *out, size_t n, float v) {
+    for (size_t i = blockIdx.x * (size_t)blockDim.x + threadIdx.x; i < n; i += (size_t)gridDim.x * blockDim.x) out[i] = v;
+}
+
 __global__ void fill_u16_kernel(uint16_t *out, size_t n, uint16_t v) {
     for (size_t i = blockIdx.x * (size_t)blockDim.x + threadIdx.x; i < n;
          i += (size_t)gridDim.x * blockDim.x)
@@ -240,7 +245,7 @@ qknorm_rope_kv_kernel(const float *__restrict__ qkv, int ldqkv, int ks, size_t s
                       const uint16_t *__restrict__ qn, const uint16_t *__restrict__ kn,
                       const float2 *__restrict__ rope, const int32_t *__restrict__ tok_pos,
                       const int32_t *__restrict__ tok_seq, int layer, uint16_t *kc, uint16_t *vc,
-                      int max_len, uint16_t *q_bf16, float *q_f32, int ldq) {
+                      int max_len, uint16_t *q_bf16, float *q_f32, int ldq, uint16_t *kv_rows) {
     dep_wait();
     dep_launch();
     // One warp per head (32 per token): qkv row t, or (ks > 0) the sum of ks
@@ -277,8 +282,10 @@ qknorm_rope_kv_kernel(const float *__restrict__ qkv, int ldqkv, int ks, size_t s
         }
     } else {
         const int kvh = (hd - 16) & 7;
-        uint16_t *dst = (hd < 24 ? kc : vc) +
-                        (((size_t)(seq * NLAYER + layer) * NKVH + kvh) * max_len + pos) * HDIM;
+        // kv_rows: K and V heads as rows [t][2048] (the 8-bit cache's append reads them)
+        uint16_t *dst = kv_rows ? kv_rows + (size_t)t * 2 * KVD + (hd - 16) * HDIM
+                                : (hd < 24 ? kc : vc) +
+                                      (((size_t)(seq * NLAYER + layer) * NKVH + kvh) * max_len + pos) * HDIM;
 #pragma unroll
         for (int j = 0; j < 4; j++) dst[lane + 32 * j] = f32_to_bf16_rne(v[j]);
     }
@@ -503,6 +510,11 @@ struct n550_model {
     uint16_t *fused_qkv = nullptr;          // only if q/k/v are not contiguous
     const uint16_t *wqkv[NLAYER] = {};
     uint16_t *kc = nullptr, *vc = nullptr;
+    // the 8-bit cache instead of kc / vc (n550_qwen3_use_kv8)
+    n550_kv8_cache kv8{};
+    uint16_t *kv_rows = nullptr;            // K and V rows of one layer's tokens [max_tokens][2048]
+    void *kv8_ws = nullptr, *kv8_out = nullptr;   // split partials; the context written out as BF16
+    size_t kv8_out_bytes = 0;
     float *x = nullptr, *qkv = nullptr, *qf = nullptr, *logits = nullptr;
     uint16_t *xb = nullptr, *qb = nullptr, *attn = nullptr, *h = nullptr, *xl = nullptr;
     float *tmp_a = nullptr, *tmp_b = nullptr;
@@ -593,7 +605,8 @@ void model_release(n550_model *m) {
     void *ptrs[] = {m->blob, m->fused_qkv, m->kc, m->vc, m->x, m->qkv, m->qf, m->logits, m->xb,
                     m->qb, m->attn, m->h, m->xl, m->tmp_a, m->tmp_b, m->tok_pos, m->tok_seq,
                     m->next, m->host_tok, m->zero_seq, m->part_m, m->part_l, m->part_o, m->rope, m->ws,
-                    m->fd_layers, m->fd_counters, m->fd_barrier, m->attn_counters};
+                    m->fd_layers, m->fd_counters, m->fd_barrier, m->attn_counters, m->kv8.k, m->kv8.v,
+                    m->kv8.k_scale, m->kv8.v_scale, m->kv8.k_bounds, m->kv_rows, m->kv8_ws, m->kv8_out};
     for (void *p : ptrs) if (p) cudaFree(p);
     delete m;
 }
@@ -727,8 +740,8 @@ int launch_qknorm_rope_kv(n550_model *m, cudaStream_t st, int T, int l, bool dec
                           const float *src = nullptr, int ks = 0) {
     N550_CUDA_TRY(launch_k(qknorm_rope_kv_kernel, T, 1024, 0, st, src ? src : m->qkv, QKVD, ks,
                            (size_t)T * QKVD, W(m, l, 4), W(m, l, 5), m->rope, m->tok_pos, m->tok_seq, l,
-                           m->kc, m->vc, m->cfg.max_len, decode ? nullptr : m->qb,
-                           decode ? m->qf : nullptr, QD));
+                           m->kc, m->vc, m->cfg.max_len, decode && !m->kv8.k ? nullptr : m->qb,
+                           decode && !m->kv8.k ? m->qf : nullptr, QD, m->kv_rows));
     N550_LAUNCH_CHECK();
     return N550_OK;
 }
@@ -776,11 +789,55 @@ int launch_final_norm(cudaStream_t st, uint16_t *xl, const float *x, const uint1
 // (n550_qwen3_fused_attention_prep).
 bool g_fused_prep = true;
 
+// The same over the 8-bit cache: the layer's K/V rows (m->kv_rows) are appended and
+// the queries (m->qb) attend to the codes. A prefill of many queries works
+// through its sequences in groups whose contexts fit m->kv8_out as BF16.
+int run_attention_kv8(n550_model *m, cudaStream_t st, bool decode, const int32_t *seq_ids,
+                      const int32_t *pos, int Sc, int Lc, int p0, int l) {
+    int rc = N550_OK;
+    Kv8AppendArgs ap{};
+    if ((rc = kv8_view(&m->kv8, l, &ap.c))) return rc;
+    ap.k = m->kv_rows;
+    ap.v = m->kv_rows + KVD;
+    ap.ld = 2 * KVD;
+    ap.L = Lc;
+    ap.seq_ids = seq_ids;
+    ap.pos = decode ? pos : nullptr;
+    ap.pos0 = p0;
+    STEP(N550_PROF_QKNORM_ROPE, 1, launch_kv8_append(st, ap, false, Sc));
+    Kv8AttnArgs a{};
+    a.c = ap.c;
+    a.q = m->qb; a.out = m->attn;
+    a.ldq = a.ldo = QD;
+    a.seq_ids = seq_ids;
+    a.pos = ap.pos;
+    a.pos0 = p0;
+    a.L = a.rows = Lc;
+    a.n_seqs = Sc;
+    a.n_select = -1;
+    if (Lc <= KV8_FEW) {
+        a.part = (float *)m->kv8_ws;
+        STEP(N550_PROF_ATTN, 2, launch_kv8_attn(st, a));
+        return N550_OK;
+    }
+    const int group = (int)std::min<size_t>(Sc, m->kv8_out_bytes / kv8_prefill_workspace(1, Lc, p0));
+    for (int s = 0; s < Sc; s += group) {
+        Kv8AttnArgs g = a;
+        g.q = m->qb + (size_t)s * Lc * QD;
+        g.out = m->attn + (size_t)s * Lc * QD;
+        g.seq_ids = seq_ids + s;
+        g.n_seqs = std::min(group, Sc - s);
+        STEP(N550_PROF_ATTN, 2, launch_kv8_prefill(st, g, m->kv8_out));
+    }
+    return N550_OK;
+}
+
 int run_attention(n550_model *m, cudaStream_t st, int T, bool decode, const int32_t *seq_ids,
                   const int32_t *pos, int Sc, int Lc, int p0, int l, bool q_in_bf16 = false,
                   const float *raw_qkv = nullptr, int ks = 0) {
     const n550_model_config &c = m->cfg;
     int rc = N550_OK;
+    if (m->kv8.k) return run_attention_kv8(m, st, decode, seq_ids, pos, Sc, Lc, p0, l);
     if (decode) {
         AttnDecodeArgs a{};
         a.q_f32 = q_in_bf16 ? nullptr : m->qf;
@@ -821,7 +878,7 @@ int run_layers_split(n550_model *m, cudaStream_t st, int T, bool decode, const i
     STEP(N550_PROF_RMSNORM, 1, launch_norm_rows(st, m->xb, m->x, W(m, 0, 0), T));
     for (int l = 0; l < NLAYER; l++) {
         STEP(N550_PROF_GEMM_QKV, 1, partials(m, st, m->xb, H, m->wqkv[l], T, QKVD, H, &ks));
-        if (decode && g_fused_prep) {
+        if (decode && g_fused_prep && !m->kv8.k) {
             if ((rc = run_attention(m, st, T, decode, seq_ids, pos, Sc, Lc, p0, l, false, m->ws, ks))) return rc;
         } else {
             STEP(N550_PROF_QKNORM_ROPE, 1, launch_qknorm_rope_kv(m, st, T, l, decode, m->ws, ks));
@@ -865,8 +922,17 @@ int run_layers_skinny(n550_model *m, cudaStream_t st, int T, bool decode, const 
         q.tok_pos = m->tok_pos; q.tok_seq = m->tok_seq;
         q.q_norm = W(m, l, 4); q.k_norm = W(m, l, 5);
         q.rope = m->rope;
-        STEP(N550_PROF_GEMM_QKV, 1,
-             launch_gemm_skinny(st, SK_EPI_QKV, m->xb, H, m->wqkv[l], nullptr, H, T, QKVD, H, q));
+        if (m->kv8.k) {                           // K/V rows instead of cache positions
+            SkEpilogue f{};
+            f.out = m->qkv;
+            f.ldo = QKVD;
+            STEP(N550_PROF_GEMM_QKV, 1,
+                 launch_gemm_skinny(st, SK_EPI_F32, m->xb, H, m->wqkv[l], nullptr, H, T, QKVD, H, f));
+            STEP(N550_PROF_QKNORM_ROPE, 1, launch_qknorm_rope_kv(m, st, T, l, decode));
+        } else {
+            STEP(N550_PROF_GEMM_QKV, 1,
+                 launch_gemm_skinny(st, SK_EPI_QKV, m->xb, H, m->wqkv[l], nullptr, H, T, QKVD, H, q));
+        }
         if ((rc = run_attention(m, st, T, decode, seq_ids, pos, Sc, Lc, p0, l))) return rc;
         STEP(N550_PROF_GEMM_O, 1,
              launch_gemm_skinny(st, SK_EPI_RESID, m->attn, QD, W(m, l, 6), nullptr, QD, T, H, QD, resid));
@@ -895,7 +961,7 @@ int run_layers(n550_model *m, cudaStream_t st, int T, bool decode, const int32_t
     *xl_ready = false;
     const bool exact = c.gemm_mode == N550_MODE_EXACT;
     // A decode step of a few sequences: all 28 layers in one persistent kernel
-    if (!exact && decode && g_fused_decode && T <= FD_MAX_TOKENS && c.max_len <= FD_MAX_LEN &&
+    if (!exact && !m->kv8.k && decode && g_fused_decode && T <= FD_MAX_TOKENS && c.max_len <= FD_MAX_LEN &&
         T <= c.max_seqs && fused_decode_grid() > 0) {
         ProfScope ps(m, st, N550_PROF_GEMM_QKV, 1);
         if ((rc = run_layers_fused(m, st, T, seq_ids, pos))) return rc;
@@ -912,7 +978,8 @@ int run_layers(n550_model *m, cudaStream_t st, int T, bool decode, const int32_t
         return run_layers_skinny(m, st, T, decode, seq_ids, pos, Sc, Lc, p0, xl_ready);
     if (!exact && T > 8 && T < g_split_rows)
         return run_layers_split(m, st, T, decode, seq_ids, pos, Sc, Lc, p0, xl_ready);
-    const bool fused_qkv = !exact && T >= g_split_rows;
+    const bool fused_qkv = !exact && !m->kv8.k && T >= g_split_rows;
+    const bool own_prep = decode && g_fused_prep && !m->kv8.k;      // decode attention finishes the raw q/k/v rows
     // the GEMV route of up to 4 rows normalises its input rows inside the q/k/v
     // and gate/up GEMVs (no norm launches)
     const bool gv_norm = !exact && T <= 4;
@@ -924,7 +991,7 @@ int run_layers(n550_model *m, cudaStream_t st, int T, bool decode, const int32_t
             STEP(N550_PROF_GEMM_QKV, 1,
                  launch_gemv(st, TC_EPI_F32, nullptr, 0, m->wqkv[l], H, m->qkv, QKVD, T, QKVD, H, false, m->x,
                              W(m, l, 0)));
-            if (!(decode && g_fused_prep))
+            if (!own_prep)
                 STEP(N550_PROF_QKNORM_ROPE, 1, launch_qknorm_rope_kv(m, st, T, l, decode));
         } else if (fused_qkv) {
             // One tcgen05 GEMM with QK-norm, RoPE and the K/V cache write in its epilogue.
@@ -939,12 +1006,12 @@ int run_layers(n550_model *m, cudaStream_t st, int T, bool decode, const int32_t
         } else {
             STEP(N550_PROF_GEMM_QKV, 1,
                  mgemm(m, st, TC_EPI_F32, m->xb, H, m->wqkv[l], nullptr, m->qkv, QKVD, T, QKVD, H));
-            if (!(decode && g_fused_prep))
+            if (!own_prep)
                 STEP(N550_PROF_QKNORM_ROPE, 1, launch_qknorm_rope_kv(m, st, T, l, decode));
         }
         // the fused QKV epilogue leaves BF16 queries (decode attention reads either);
         // otherwise decode attention may finish the raw q/k/v rows itself
-        const float *raw = !fused_qkv && decode && g_fused_prep ? m->qkv : nullptr;
+        const float *raw = !fused_qkv && own_prep ? m->qkv : nullptr;
         if ((rc = run_attention(m, st, T, decode, seq_ids, pos, Sc, Lc, p0, l, fused_qkv, raw, 0)))
             return rc;
         // o and down: the residual rows x were last written two or more kernels
@@ -1170,6 +1237,80 @@ int n550_qwen3_init_random(n550_model_t **out, uint64_t seed, double sigma,
     rc = model_setup(m);
     if (rc) { model_release(m); return rc; }
     *out = m;
+    return N550_OK;
+}
+
+// The captured decode step and prefill hold the cache's pointers.
+static void drop_graphs(n550_model_t *m) {
+    if (m->graph) { cudaGraphExecDestroy(m->graph); m->graph = nullptr; }
+    if (m->pgraph) { cudaGraphExecDestroy(m->pgraph); m->pgraph = nullptr; }
+    memset(m->pg_last, 0, sizeof m->pg_last);
+}
+
+int n550_qwen3_use_kv8(n550_model_t *m, int on) {
+    if (!m) return N550_ERR_ARG;
+    const n550_model_config &c = m->cfg;
+    if (c.gemm_mode != N550_MODE_FAST) return N550_ERR_UNSUPPORTED;
+    if ((on != 0) == (m->kv8.k != nullptr)) return N550_OK;
+    N550_CUDA_TRY(cudaDeviceSynchronize());
+    drop_graphs(m);
+    const size_t planes = (size_t)c.max_seqs * NLAYER * NKVH, codes = planes * (size_t)c.max_len * HDIM;
+    const size_t scales = planes * (((size_t)c.max_len + N550_KV8_BLOCK - 1) / N550_KV8_BLOCK);
+    auto give_back = [](auto &p) { if (p) cudaFree(p); p = nullptr; };
+    auto kv8_free = [&]() {
+        give_back(m->kv8.k); give_back(m->kv8.v); give_back(m->kv8.k_scale); give_back(m->kv8.v_scale);
+        give_back(m->kv8.k_bounds); give_back(m->kv_rows); give_back(m->kv8_ws); give_back(m->kv8_out);
+    };
+    auto bf16_get = [&]() -> int {
+        if (cudaMalloc((void **)&m->kc, codes * 2) != cudaSuccess || cudaMalloc((void **)&m->vc, codes * 2) != cudaSuccess) {
+            (void)cudaGetLastError();
+            give_back(m->kc); give_back(m->vc);
+            return N550_ERR_OOM;
+        }
+        N550_CUDA_TRY(cudaMemset(m->kc, 0, codes * 2));
+        N550_CUDA_TRY(cudaMemset(m->vc, 0, codes * 2));
+        N550_CUDA_TRY(cudaDeviceSynchronize());
+        return N550_OK;
+    };
+    if (!on) {
+        kv8_free();
+        return bf16_get();
+    }
+    // the BF16 cache makes room first; it comes back if the 8-bit one does not fit
+    give_back(m->kc); give_back(m->vc);
+    // contexts as BF16 for prefill attention: one whole sequence, or up to 256 MB of them
+    const size_t one = kv8_prefill_workspace(1, c.max_len, 0);
+    m->kv8_out_bytes = std::max(one, std::min(one * c.max_seqs, (size_t)256 << 20));
+    const struct { void **p; size_t n; } want[] = {
+        {(void **)&m->kv8.k, codes}, {(void **)&m->kv8.v, codes},
+        {(void **)&m->kv8.k_scale, scales * 4}, {(void **)&m->kv8.v_scale, scales * 4},
+        {(void **)&m->kv8.k_bounds, scales * 2 * HDIM},
+        {(void **)&m->kv_rows, (size_t)c.max_tokens * 2 * KVD * 2},
+        {&m->kv8_ws, kv8_attn_workspace(c.max_seqs, KV8_FEW)}, {&m->kv8_out, m->kv8_out_bytes}};
+    for (const auto &w : want)
+        if (cudaMalloc(w.p, w.n) != cudaSuccess) {
+            (void)cudaGetLastError();
+            kv8_free();
+            const int rc = bf16_get();
+            return rc ? rc : N550_ERR_OOM;
+        }
+    m->kv8.n_slots = c.max_seqs;
+    m->kv8.n_layers = NLAYER;
+    m->kv8.max_len = c.max_len;
+    // positions never written read as zeros, like the BF16 cache's
+    N550_CUDA_TRY(cudaMemset(m->kv8.k, 0, codes));
+    N550_CUDA_TRY(cudaMemset(m->kv8.v, 0, codes));
+    N550_CUDA_TRY(cudaMemset(m->kv8.k_bounds, 0, scales * 2 * HDIM));
+    fill_f32_kernel<<<grid1(scales), 256>>>(m->kv8.k_scale, scales, 0x1p-126f);
+    fill_f32_kernel<<<grid1(scales), 256>>>(m->kv8.v_scale, scales, 0x1p-126f);
+    N550_LAUNCH_CHECK();
+    N550_CUDA_TRY(cudaDeviceSynchronize());
+    return N550_OK;
+}
+
+int n550_qwen3_kv8_cache(const n550_model_t *m, n550_kv8_cache *c) {
+    if (!m || !c || !m->kv8.k) return N550_ERR_ARG;
+    *c = m->kv8;
     return N550_OK;
 }
 
@@ -1438,6 +1579,7 @@ int n550_qwen3_forward_batch_host(n550_model_t *m, const int32_t *tokens, int n_
     if (n_token > m->cfg.max_tokens) return N550_ERR_ARG;
     cudaStream_t st = 0;
     N550_CUDA_TRY(cudaMemcpyAsync(m->host_tok, tokens, (size_t)n_token * 4, cudaMemcpyHostToDevice, st));
+    if (m->dump && m->kv8.k) return N550_ERR_UNSUPPORTED;      // the dump route reads the BF16 cache
     if (m->dump) {
         if (pos0 < 0 || pos0 + n_token > m->cfg.max_len) return N550_ERR_ARG;
         int rc = dump_forward(m, st, m->host_tok, n_token, pos0);
@@ -1560,7 +1702,7 @@ int n550_qkv_rope_kv(void *stream, const uint16_t *x, int ldx, const uint16_t *w
     if (!rc) {
         if (launch_k(qknorm_rope_kv_kernel, M, 1024, 0, st, (const float *)ws, QKVD, ks,
                      (size_t)M * QKVD, q_norm, k_norm, rope, tok_pos, tok_seq, layer, k_cache, v_cache,
-                     max_len, qb, qf, ldq) != cudaSuccess)
+                     max_len, qb, qf, ldq, (uint16_t *)nullptr) != cudaSuccess)
             rc = N550_ERR_CUDA;
         (void)cudaGetLastError();
     }

@@ -18,7 +18,8 @@ class Model:
 
     def __init__(self, *, blob: np.ndarray | None = None, seed: int = 0, sigma: float = 0.02,
                  max_seqs: int = 1, max_len: int = 2048, max_tokens: int = 512,
-                 gemm_mode: int = MODE_FAST, kblock: int = 16):
+                 gemm_mode: int = MODE_FAST, kblock: int = 16, kv8: bool = False):
+        """kv8: hold the KV cache in 8 bits (n550_qwen3_use_kv8; fast mode)."""
         self.cfg = ModelConfig(max_seqs, max_len, max_tokens, gemm_mode, kblock)
         # held for close(): at interpreter exit the module's globals may be gone
         self._lib = lib()
@@ -31,6 +32,8 @@ class Model:
             rc = lib().n550_qwen3_init_random(C.byref(h), seed, sigma, C.byref(self.cfg))
         check(rc, "n550_qwen3_init")
         self._h = h
+        if kv8:
+            self.use_kv8()
 
     @property
     def handle(self):
@@ -43,6 +46,10 @@ class Model:
 
     def __del__(self):
         self.close()
+
+    def use_kv8(self, on: bool = True):
+        """Hold the KV cache in 8 bits from here on, or in BF16 again; it starts empty."""
+        check(lib().n550_qwen3_use_kv8(self._h, 1 if on else 0), "n550_qwen3_use_kv8")
 
     # ---- reference-shaped host path (sequence slot 0) ----
     def forward_batch(self, tokens, pos0: int, want_logits: bool = True):
@@ -139,6 +146,28 @@ class Model:
             C.c_void_p(pos.data_ptr()), tokens.shape[0], steps, C.c_void_p(out_ids.data_ptr()),
             1 if use_graph else 0), "n550_qwen3_decode_steps")
 
+    def kv8_cache(self):
+        """The model's own 8-bit cache as a KV8Cache (its memory, valid while the
+        model lives and keeps it)."""
+        import torch
+        from . import KV8_BLOCK, KV8CacheStruct
+        from .kv8 import KV8Cache
+        c = KV8CacheStruct()
+        check(lib().n550_qwen3_kv8_cache(self._h, C.byref(c)), "n550_qwen3_kv8_cache")
+        plane = (c.n_slots, c.n_layers, 8)
+        nb = -(-c.max_len // KV8_BLOCK)
+
+        def view(ptr, shape, kind, dtype):
+            n = int(np.prod(shape))
+            return torch.as_tensor(_DeviceArray(ptr, n, kind), device="cuda").view(dtype).view(shape)
+
+        e4 = torch.float8_e4m3fn
+        return KV8Cache(k=view(c.k, plane + (c.max_len, 128), "|u1", e4),
+                        v=view(c.v, plane + (c.max_len, 128), "|u1", e4),
+                        k_scale=view(c.k_scale, plane + (nb,), "<f4", torch.float32),
+                        v_scale=view(c.v_scale, plane + (nb,), "<f4", torch.float32),
+                        k_bounds=view(c.k_bounds, plane + (nb, 2, 128), "|u1", e4))
+
     def weight_bits(self, which: int) -> np.ndarray:
         """Copy of one QW3M tensor (BF16 bits) from the device."""
         import torch
@@ -151,8 +180,8 @@ class Model:
 
 
 class _DeviceArray:
-    """Zero-copy CUDA array interface over a device pointer of int16."""
+    """Zero-copy CUDA array interface over a device pointer (int16 unless `kind` says otherwise)."""
 
-    def __init__(self, ptr: int, n: int):
-        self.__cuda_array_interface__ = {"shape": (n,), "typestr": "<i2", "data": (ptr, False),
+    def __init__(self, ptr: int, n: int, kind: str = "<i2"):
+        self.__cuda_array_interface__ = {"shape": (n,), "typestr": kind, "data": (ptr, False),
                                          "version": 3, "strides": None}
