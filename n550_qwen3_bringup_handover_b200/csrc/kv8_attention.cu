@@ -21,14 +21,17 @@
 //   q = 2^a (h + l / 16): two parts hold a BF16 value whole, down to 2^-21 of the
 //       row's largest;
 //   w = 2^-8 (w1 + w2 / 16 + w3 / 256): three parts hold a softmax weight to 12
-//       bits (2^-13 half a step), or 2^-26 of the largest for the small ones.
-// Sums, scores and the softmax state are FP32.
+//       bits (2^-13 half a step), or 2^-26 of the tile's largest for the small ones.
+// Weights are relative to the largest score of their own tile, so each tile's O is
+// finished by its MMAs and added up, scaled, in registers: an O that stays in
+// TMEM over the tiles has to be scaled there whenever a maximum grows (in 4 of 10
+// tiles at 1152 positions). Sums, scores and the softmax state are FP32.
 //
 //   warp 0     producer: walks the run, 32 blocks a batch (one per lane: list entry,
 //              slot, scales), and fills a ring of 32 KB stages
 //   warp 1     issues the MMAs, S of the next tile before P.V of this one
-//   warps 2-5  softmax, a thread per position, and the output, a thread per
-//              dimension; they agree on a tile's maximum through shared memory.
+//   warps 2-5  softmax, a thread per position, and O, a thread per dimension (of
+//              the tile before, once its MMAs are done); they agree on a tile's maximum through shared memory.
 //              With more query tokens more such groups share the columns.
 //   last warp  splits the queries of each new pair
 #include <cuda.h>
@@ -112,15 +115,6 @@ __device__ __forceinline__ void tmem_ld_x8(uint32_t taddr, uint32_t *r) {
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
                  : "r"(taddr));
 }
-__device__ __forceinline__ void tmem_st_x8(uint32_t taddr, const uint32_t *r) {
-    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};"
-                 ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
-                 : "memory");
-}
-__device__ __forceinline__ void tmem_st_x4(uint32_t taddr, const uint32_t *r) {
-    asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1,%2,%3,%4};"
-                 ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]) : "memory");
-}
 // N columns (2 to 24, loads rounded up to a multiple of 4) of this thread's TMEM lane.
 template <int N>
 __device__ __forceinline__ void load_cols(uint32_t t, uint32_t (&r)[(N + 3) / 4 * 4]) {
@@ -130,15 +124,6 @@ __device__ __forceinline__ void load_cols(uint32_t t, uint32_t (&r)[(N + 3) / 4 
     if constexpr (N % 8 > 0 && N % 8 <= 4) tmem_ld_x4(t + at, r + at);
     tmem_ld_wait();
 }
-template <int N>
-__device__ __forceinline__ void store_cols(uint32_t t, const uint32_t (&r)[(N + 3) / 4 * 4]) {
-    int at = 0;
-    if constexpr (N >= 16) { tmem_st_32x32b_x16(t, *reinterpret_cast<const uint32_t(*)[16]>(&r[0])); at = 16; }
-    if constexpr (N % 16 > 4) { tmem_st_x8(t + at, r + at); at += 8; }
-    if constexpr (N % 8 > 0 && N % 8 <= 4) tmem_st_x4(t + at, r + at);
-    tmem_st_wait();
-}
-
 // Maximum over the warp; a NaN counts as nothing.
 __device__ __forceinline__ float warp_max(float x) {
     float y;
@@ -276,7 +261,7 @@ kv8_attn_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
     uint8_t *sP = sQ + 2 * NS * 128;                                               // [2][NP][128]
     uint8_t *sraw = sP + 2 * NP * 128;                                             // [ST][L][2 heads x 128 BF16]
     __shared__ Rec rec[ST];
-    __shared__ __align__(8) uint64_t full[ST], empty[ST], q_ready[4], q_free[2], s_full[2], p_full[2], pv_done[2], o_free[2], done;
+    __shared__ __align__(8) uint64_t full[ST], empty[ST], q_ready[4], q_free[2], s_full[2], p_full[2], pv_done[2], done;
     __shared__ float q_scale[4][NC];            // power of two of each query row, by piece modulo 4
     __shared__ __align__(16) float xmax[2][4][NC], xsum[2][4][NC];
     __shared__ int xdead[G][2][4];
@@ -292,7 +277,6 @@ kv8_attn_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
             mbar_init(&s_full[i], 1);
             mbar_init(&p_full[i], 4 * G);
             mbar_init(&pv_done[i], 1);
-            mbar_init(&o_free[i], 4 * G);
         }
         mbar_init(&done, 1);
         fence_mbar_init();
@@ -409,9 +393,8 @@ kv8_attn_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
                 seen = __shfl_sync(0xFFFFFFFFu, earlier || tile, 31);
             }
             // Lanes 2 i and 2 i + 1 share a stage where both hold a block of one piece
-            // and V's scales are near enough for weights in one scale (a factor 8; with
-            // the 4 that O's scale may lag, small weights are multiples of 2^-20 of
-            // the largest instead of 2^-25).
+            // and V's scales are near enough for weights in one scale (a factor 8: the
+            // small weights of one are then multiples of 2^-22 of its largest instead of 2^-25).
             const int blk = __shfl_down_sync(0xFFFFFFFFu, me.blk[0], 1), fl = __shfl_down_sync(0xFFFFFFFFu, me.flags, 1);
             const float ks = __shfl_down_sync(0xFFFFFFFFu, me.ks[0], 1), vs = __shfl_down_sync(0xFFFFFFFFu, me.vs[0], 1);
             bool two = false;
@@ -492,26 +475,23 @@ kv8_attn_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
         constexpr uint32_t id_s = idesc_e4m3(NS, 0), id_o = idesc_e4m3(NP, 1);
         const uint32_t aR = smem_u32(ring), aQ = smem_u32(sQ), aP = smem_u32(sP);
         int t = 0, piece = -1;                   // tiles whose S was issued; this piece with tiles
-        int w_st = 0, w_half = 0, w_first = 0, w_piece = 0;       // the tile whose P.V is due
+        int w_st = 0, w_half = 0;                // the tile whose P.V is due
         bool due = false, ok = true;
+        // (The softmax has read the O of tile u - 2, this one's columns, before its weights of tile u.)
         auto issue_pv = [&]() -> bool {
             const int u = t - 1, b = u & 1;
             due = false;
             if (!warp_wait(&p_full[b], (u >> 1) & 1)) return false;
-            // the first P.V of a piece overwrites O: its buffer must have been read out
-            if (w_first && !warp_wait(&o_free[w_piece & 1], ((w_piece >> 1) & 1) ^ 1)) return false;
             tc_fence_after();
-            const uint32_t v = aR + w_st * STAGE + 2 * BLK, pp = aP + b * NP * 128, d = tO + (w_piece & 1) * NP;
+            const uint32_t v = aR + w_st * STAGE + 2 * BLK, pp = aP + b * NP * 128, d = tO + b * NP;
             const int steps = w_half ? 2 : 4;
             for (int k = 0; k < steps; k++)
                 if (elect_one_sync())
-                    umma_e4m3(d, umma_desc_sw128_mn(v + k * 4096, 0), umma_desc_sw128(pp + k * 32), id_o,
-                              (w_first && k == 0) ? 0u : 1u);
+                    umma_e4m3(d, umma_desc_sw128_mn(v + k * 4096, 0), umma_desc_sw128(pp + k * 32), id_o, k > 0 ? 1u : 0u);
             if (elect_one_sync()) { umma_commit(&empty[w_st]); umma_commit(&pv_done[b]); }
             __syncwarp();
             return true;
         };
-        bool first = false;                      // no tile of this piece yet
         for (int r = 0;; r++) {
             const int st = r % ST;
             // nothing to issue S for yet: the due P.V frees its stage
@@ -523,7 +503,6 @@ kv8_attn_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
                 if (piece >= 0 && elect_one_sync()) umma_commit(&q_free[piece & 1]);
                 __syncwarp();
                 piece++;
-                first = true;
                 if (!(ok = warp_wait(&q_ready[piece & 3], (piece >> 2) & 1))) break;
             }
             if (w.blk[0] < 0) {
@@ -543,9 +522,6 @@ kv8_attn_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
                 due = true;
                 w_st = st;
                 w_half = w.blk[1] < 0;
-                w_first = first;
-                w_piece = piece;
-                first = false;
             }
             if (w.flags & R_END) break;
         }
@@ -604,10 +580,11 @@ kv8_attn_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
         const int grp = (warp - 2) >> 2, c0 = grp * NG, ng = min(NG, 2 * p.L - c0);     // ng <= 0: nothing to do but keep step
         const int qw = warp & 3, row = qw * 32 + lane, half = row >> 6;
         const uint32_t lane_off = (uint32_t)(qw * 32) << 16;
-        int t = 0, piece = -1, tiles = 0, bars = 0, ends = 0;      // tiles done; pieces with tiles; this piece's tiles
-        float m[NG], l[NG], qf[NG] = {}, vref = 0.f;
+        int t = 0, piece = -1, bars = 0, ends = 0;                 // tiles, pieces with tiles, meetings, ended pieces
+        float qf[NG] = {};
         bool dead = false;
-        // A group's four warps pass here together, also when one's wait ran out: then all leave.
+        // A group's four warps pass here together, and leave together: after the last
+        // record, or when a wait of one of them ran out.
         auto meet = [&](bool mine) -> bool {
             int *d = xdead[grp][bars & 1];
             if (lane == 0) d[qw] = mine;
@@ -615,42 +592,105 @@ kv8_attn_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
             bars++;
             return d[0] | d[1] | d[2] | d[3];
         };
+        // The piece so far: maximum, this lane's part of the sum, this lane's dimension of O.
+        float m[NG], l[NG], o[NG];
+        auto reset = [&]() {
+#pragma unroll
+            for (int c = 0; c < NG; c++) { m[c] = -INFINITY; l[c] = 0.f; o[c] = 0.f; }
+        };
+        reset();
+        // The last tile whose weights are out: its maximum and sum, V's scale, whether it is owed to the piece.
+        float tm[NG], tl[NG], tv = 0.f;
+        bool owed = false;
+        auto collect = [&]() {
+            const int u = t - 1;
+            owed = false;
+            if (dead || (dead = !warp_wait(&pv_done[u & 1], (u >> 1) & 1))) return;
+            uint32_t x[(3 * NG + 3) / 4 * 4];
+            tc_fence_after();
+            load_cols<3 * NG>(tO + lane_off + (u & 1) * NP + 16 * grp, x);
+            tc_fence_before();
+#pragma unroll
+            for (int c = 0; c < NG; c++) {
+                const float part = fmaf(fmaf(__uint_as_float(x[3 * c + 2]), 0.0625f, __uint_as_float(x[3 * c + 1])), 0.0625f,
+                                        __uint_as_float(x[3 * c]));
+                const float mn = fmaxf(m[c], tm[c]), ref = mn == -INFINITY ? 0.f : mn;
+                const float a = ex2(m[c] - ref), b = ex2(tm[c] - ref);
+                o[c] = o[c] * a + part * (b * tv);
+                l[c] = l[c] * a + tl[c] * b;
+                m[c] = mn;
+            }
+        };
+        // Output of the piece that ended: divided by the sum of its weights, or as a
+        // partial. False: some warp's wait ran out, all leave.
+        bool ending = false;
+        int old_s = 0, old_kvh = 0, old_slot = 0;
+        auto finish = [&]() -> bool {
+            ending = false;
+            ends++;
+#pragma unroll
+            for (int c = 0; c < NG; c++) {
+#pragma unroll
+                for (int k = 16; k > 0; k >>= 1) l[c] += __shfl_xor_sync(0xFFFFFFFFu, l[c], k);
+                if (lane == 0) xsum[ends & 1][qw][c0 + c] = l[c];
+            }
+            if (meet(dead)) return false;
+            const float (*xs)[NC] = xsum[ends & 1];
+#pragma unroll
+            for (int c = 0; c < NG; c++) {
+                if (c >= ng) break;
+                const int col = c0 + c;
+                const float L = (xs[0][col] + xs[1][col]) + (xs[2][col] + xs[3][col]);
+                if (old_slot < 0) {
+                    const size_t orow = (size_t)old_s * p.rows + p.row0 + (col >> 1);
+                    // no position at all: zero
+                    p.out[orow * p.ldo + (2 * old_kvh + (col & 1)) * KV8_HD + row] =
+                        f32_to_bf16_rne(L == 0.f ? 0.f : o[c] * (1.f / L));
+                } else {
+                    float *part = p.part + part_base(gridDim.x) + (size_t)old_slot * (2 * p.L) * (KV8_HD + 2);
+                    part[col * KV8_HD + row] = o[c];
+                    if (row == 0) {
+                        part[2 * p.L * KV8_HD + 2 * col] = m[c];
+                        part[2 * p.L * KV8_HD + 2 * col + 1] = L;
+                    }
+                }
+            }
+            reset();
+            return true;
+        };
         for (int r = 0;; r++) {
             const int st = r % ST;
-            dead = dead || !warp_wait(&full[st], (r / ST) & 1);
+            if (dead || (dead = !warp_wait(&full[st], (r / ST) & 1))) {
+                meet(true);
+                break;
+            }
             const Rec w = rec[st];
             __syncwarp();
             if (lane == 0) mbar_arrive(&empty[st]);
-            if (w.flags & R_FIRST) {
-                tiles = 0;
-                vref = 0.f;
-                ends++;
-#pragma unroll
-                for (int c = 0; c < NG; c++) { m[c] = -INFINITY; l[c] = 0.f; }
-            }
-            if (!dead && (w.flags & R_Q)) {
+            if (w.flags & R_Q) {
                 piece++;
                 dead = !warp_wait(&q_ready[piece & 3], (piece >> 2) & 1);
 #pragma unroll
                 for (int c = 0; c < NG; c++) qf[c] = c < ng ? q_scale[piece & 3][c0 + c] : 0.f;
             }
-            if (dead || w.blk[0] >= 0) {
-                const uint32_t ts = tS + lane_off + (t & 1) * NS + 2 * c0, to = tO + lane_off + (piece & 1) * NP + 16 * grp;
+            const bool tile = w.blk[0] >= 0;
+            float x[NG], sum[NG], vmax = 0.f;                      // this tile's maximum and sum
+            if (tile && !dead) {
                 const int blk = half ? w.blk[1] : w.blk[0], pos = blk * KV8_BLOCK + (row & 63);
                 const float kf = (half ? w.ks[1] : w.ks[0]) * kKv8ScaleLog2;
                 float s[NG];
-                if (!dead) dead = !warp_wait(&s_full[t & 1], (t >> 1) & 1);
+                dead = !warp_wait(&s_full[t & 1], (t >> 1) & 1);
                 if (!dead) {
                     uint32_t v[(2 * NG + 3) / 4 * 4];
                     tc_fence_after();
-                    load_cols<2 * NG>(ts, v);
+                    load_cols<2 * NG>(tS + lane_off + (t & 1) * NS + 2 * c0, v);
                     const int lim = blk < 0 ? -1 : w.ctx - p.L + c0 / 2;   // last position of this group's token j: lim + j
 #pragma unroll
                     for (int c = 0; c < NG; c++) {
                         s[c] = -INFINITY;
                         if (c < ng) {
-                            const float x = fmaf(__uint_as_float(v[2 * c + 1]), 0.0625f, __uint_as_float(v[2 * c]));
-                            if (blk >= 0 && pos <= lim + c / 2) s[c] = x * qf[c] * kf;
+                            const float q = fmaf(__uint_as_float(v[2 * c + 1]), 0.0625f, __uint_as_float(v[2 * c]));
+                            if (blk >= 0 && pos <= lim + c / 2) s[c] = q * qf[c] * kf;
                             const float mx = warp_max(s[c]);
                             if (lane == 0) xmax[bars & 1][qw][c0 + c] = mx;
                         }
@@ -658,134 +698,66 @@ kv8_attn_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
                 }
                 const float (*xm)[NC] = xmax[bars & 1];            // [warp][column]
                 if (meet(dead)) break;
-                // the tile's maximum, and V's scale: O moves when either changes
-                const float vmax = w.blk[1] < 0 ? w.vs[0] : fmaxf(w.vs[0], w.vs[1]);
-                const bool moved = !(vmax <= vref && vmax * 4.f >= vref);
-                float x[NG];
-                bool grow = moved;
+                vmax = w.blk[1] < 0 ? w.vs[0] : fmaxf(w.vs[0], w.vs[1]);
+                uint8_t *dst = sP + ((t & 1) * NP + 16 * grp) * 128;     // (P.V of tile t - 2 was collected)
+                const float ratio = blk < 0 || vmax == 0.f ? 0.f : 256.f * ((half ? w.vs[1] : w.vs[0]) / vmax);
 #pragma unroll
                 for (int c = 0; c < NG; c++) {
                     x[c] = fmaxf(fmaxf(xm[0][c0 + c], xm[1][c0 + c]), fmaxf(xm[2][c0 + c], xm[3][c0 + c]));
-                    grow |= c < ng && x[c] > m[c];
+                    if (c >= ng) x[c] = -INFINITY;
+                    sum[c] = 0.f;
                 }
-                bool alive = true;
-                if (grow) {                                        // warp-uniform
-                    const float vmove = moved && tiles ? vref / vmax : 1.f;
-                    if (moved) vref = vmax;
-                    float corr[NG];
 #pragma unroll
-                    for (int c = 0; c < NG; c++) {
-                        const float to_m = c < ng ? fmaxf(m[c], x[c]) : m[c];
-                        corr[c] = to_m > m[c] ? ex2(m[c] - to_m) : 1.f;
-                        m[c] = to_m;
-                        l[c] *= corr[c];
-                    }
-                    if (tiles) {
-                        // O holds the tiles before: P.V of the last one must have ended
-                        alive = warp_wait(&pv_done[(t - 1) & 1], ((t - 1) >> 1) & 1);
-                        if (alive) {
-                            uint32_t o[(3 * NG + 3) / 4 * 4];
-                            tc_fence_after();
-                            load_cols<3 * NG>(to, o);
+                for (int c = 0; c < NG; c += 2) {
+                    if (c >= ng) break;
+                    float a = sum[c] = ex2(s[c] - (x[c] == -INFINITY ? 0.f : x[c]));
+                    float b = sum[c + 1] = ex2(s[c + 1] - (x[c + 1] == -INFINITY ? 0.f : x[c + 1]));
+                    a *= ratio;
+                    b *= ratio;
 #pragma unroll
-                            for (int c = 0; c < NG; c++)
-#pragma unroll
-                                for (int k = 0; k < 3; k++)
-                                    o[3 * c + k] = __float_as_uint(__uint_as_float(o[3 * c + k]) * (corr[c] * vmove));
-                            store_cols<3 * NG>(to, o);
-                        }
+                    for (int k = 0; k < 3; k++) {
+                        const uint32_t e = f32x2_to_e4m3x2(a, b);
+                        dst[sw(3 * c + k, row)] = (uint8_t)e;
+                        dst[sw(3 * c + 3 + k, row)] = (uint8_t)(e >> 8);
+                        const float2 f = e4m3x2_to_f32x2(e);
+                        a = (a - f.x) * 16.f;
+                        b = (b - f.y) * 16.f;
                     }
                 }
-                // this buffer of P was read by P.V of two tiles ago
-                if (alive && t >= 2) alive = warp_wait(&pv_done[t & 1], ((t - 2) >> 1) & 1);
-                if (alive) {
-                    uint8_t *dst = sP + ((t & 1) * NP + 16 * grp) * 128;
-                    const float ratio = blk < 0 || vref == 0.f ? 0.f : 256.f * ((half ? w.vs[1] : w.vs[0]) / vref);
+                // codes of V behind the context may be anything, NaN too: a weight of 0 needs a 0
+                if (grp == 0 && blk >= 0 && pos >= w.ctx) {
+                    uint4 *z = (uint4 *)(ring + st * STAGE + 2 * BLK + row * 128);
 #pragma unroll
-                    for (int c = 0; c < NG; c += 2) {
-                        if (c >= ng) break;
-                        float a = ex2(s[c] - (m[c] == -INFINITY ? 0.f : m[c]));
-                        float b = ex2(s[c + 1] - (m[c + 1] == -INFINITY ? 0.f : m[c + 1]));
-                        l[c] += a;
-                        l[c + 1] += b;
-                        a *= ratio;
-                        b *= ratio;
-#pragma unroll
-                        for (int k = 0; k < 3; k++) {
-                            const uint32_t e = f32x2_to_e4m3x2(a, b);
-                            dst[sw(3 * c + k, row)] = (uint8_t)e;
-                            dst[sw(3 * c + 3 + k, row)] = (uint8_t)(e >> 8);
-                            const float2 f = e4m3x2_to_f32x2(e);
-                            a = (a - f.x) * 16.f;
-                            b = (b - f.y) * 16.f;
-                        }
-                    }
-                    // codes of V behind the context may be anything, NaN too: a weight of 0 needs a 0
-                    if (grp == 0 && blk >= 0 && pos >= w.ctx) {
-                        uint4 *z = (uint4 *)(ring + st * STAGE + 2 * BLK + row * 128);
-#pragma unroll
-                        for (int k = 0; k < 8; k++) z[k] = make_uint4(0u, 0u, 0u, 0u);
-                    }
-                    fence_proxy_async_smem();
-                    tc_fence_before();
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(&p_full[t & 1]);
+                    for (int k = 0; k < 8; k++) z[k] = make_uint4(0u, 0u, 0u, 0u);
                 }
-                dead = !alive;                                     // leaves at the next meeting
+                fence_proxy_async_smem();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&p_full[t & 1]);
+            }
+            // Meanwhile the tile before this one: its O, and the output if its piece is over. A
+            // piece ends with a record that says so; the next record collects its last tile.
+            if (owed) collect();
+            if (ending) {
+                if (!finish()) break;
+            }
+            if (tile) {
                 t++;
-                tiles++;
-            }
-            if (!(w.flags & R_LAST)) {
-                if (dead ? meet(dead) : (w.flags & R_END) != 0) break;
-                continue;
-            }
-
-            // ---------------- the piece ends ----------------
-            const uint32_t to = tO + lane_off + (piece & 1) * NP + 16 * grp;
-            uint32_t o[(3 * NG + 3) / 4 * 4];
+                owed = true;
+                tv = vmax * 0.00390625f;
 #pragma unroll
-            for (int c = 0; c < (3 * NG + 3) / 4 * 4; c++) o[c] = 0u;
-#pragma unroll
-            for (int c = 0; c < NG; c++) {
-                float x = l[c];
-#pragma unroll
-                for (int k = 16; k > 0; k >>= 1) x += __shfl_xor_sync(0xFFFFFFFFu, x, k);
-                if (lane == 0) xsum[ends & 1][qw][c0 + c] = x;
+                for (int c = 0; c < NG; c++) { tm[c] = x[c]; tl[c] = sum[c]; }
             }
-            if (tiles && !dead) {
-                dead = !warp_wait(&pv_done[(t - 1) & 1], ((t - 1) >> 1) & 1);
-                if (!dead) {
-                    tc_fence_after();
-                    load_cols<3 * NG>(to, o);
-                    tc_fence_before();
-                }
+            if (w.flags & R_LAST) {
+                ending = true;
+                old_s = w.s; old_kvh = w.kvh; old_slot = w.slot;
             }
-            __syncwarp();
-            if (tiles && lane == 0) mbar_arrive(&o_free[piece & 1]);
-            if (meet(dead)) break;
-            const float (*xs)[NC] = xsum[ends & 1];
-#pragma unroll
-            for (int c = 0; c < NG; c++) {
-                if (c >= ng) break;
-                const int col = c0 + c;
-                const float L = (xs[0][col] + xs[1][col]) + (xs[2][col] + xs[3][col]);
-                const float O = fmaf(fmaf(__uint_as_float(o[3 * c + 2]), 0.0625f, __uint_as_float(o[3 * c + 1])), 0.0625f,
-                                     __uint_as_float(o[3 * c])) * (vref * 0.00390625f);
-                if (w.slot < 0) {
-                    const size_t orow = (size_t)w.s * p.rows + p.row0 + (col >> 1);
-                    // no position at all: zero
-                    p.out[orow * p.ldo + (2 * w.kvh + (col & 1)) * KV8_HD + row] =
-                        f32_to_bf16_rne(L == 0.f ? 0.f : O * (1.f / L));
-                } else {
-                    float *part = p.part + part_base(gridDim.x) + (size_t)w.slot * (2 * p.L) * (KV8_HD + 2);
-                    part[col * KV8_HD + row] = O;
-                    if (row == 0) {
-                        part[2 * p.L * KV8_HD + 2 * col] = m[c];
-                        part[2 * p.L * KV8_HD + 2 * col + 1] = L;
-                    }
-                }
+            if (w.flags & R_END) {
+                if (owed) collect();
+                if (ending) finish();
+                else meet(dead);
+                break;
             }
-            if (w.flags & R_END) break;
         }
     }
     tc_fence_before();

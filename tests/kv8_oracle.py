@@ -100,7 +100,7 @@ class Cache:
         rounded to a multiple of 2^-25 of the largest weight (small ones are; half
         a step is 2^-26, and the weights' sum is at least the largest) by at most
         2^-26 |v_td|, which 2^-11 of the second term covers. (Where V's block scales
-        differ the multiple is up to 2^-20, and floor has to be 2^-10.)"""
+        differ the multiple is up to 2^-22, and floor has to be 2^-12.)"""
         n = len(seq_ids)
         q = q[:, :HEADS * HD].double().cpu().view(n, L, HEADS, HD)
         out = torch.zeros((n, L, HEADS, HD), dtype=torch.float64)
