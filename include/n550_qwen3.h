@@ -327,8 +327,10 @@ size_t n550_attention_kv8_workspace(int n_seqs);
  * pos0 .. pos0+L-1 whose K/V were appended, causal; q and out [n_seqs*L] rows.
  * As in the BF16 prefill, a NaN in the V of one of these L positions also reaches
  * that dimension of the queries before it. workspace may be NULL (slower) or
- * n550_attention_prefill_kv8_workspace(n_seqs, L, pos0) bytes, as above; from 9
- * queries on it holds the context as BF16, 4096 bytes per sequence and position. */
+ * n550_attention_prefill_kv8_workspace(n_seqs, L, pos0) bytes, as above. Up to 8
+ * queries (and more, where few sequences have long contexts) stream the codes in
+ * passes of 8; otherwise the workspace holds the context as BF16, 4096 bytes
+ * per sequence and position. */
 int n550_attention_prefill_kv8(void *stream, const uint16_t *q, int ldq, const n550_kv8_cache *c,
                                int layer, const int32_t *seq_ids, int n_seqs, int L, int pos0,
                                uint16_t *out, int ldo, void *workspace, size_t workspace_bytes);

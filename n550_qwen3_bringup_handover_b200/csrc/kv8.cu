@@ -93,7 +93,8 @@ int n550_attention_sparse_kv8(void *stream, const uint16_t *q, int ldq, const n5
 
 size_t n550_attention_prefill_kv8_workspace(int n_seqs, int L, int pos0) {
     if (n_seqs <= 0 || L <= 0 || pos0 < 0) return 0;
-    return L <= KV8_FEW ? kv8_attn_workspace(n_seqs, L) : kv8_prefill_workspace(n_seqs, L, pos0);
+    return kv8_in_passes(n_seqs, L, pos0) ? kv8_attn_workspace(n_seqs, L < KV8_FEW ? L : KV8_FEW)
+                                          : kv8_prefill_workspace(n_seqs, L, pos0);
 }
 
 int n550_attention_prefill_kv8(void *stream, const uint16_t *q, int ldq, const n550_kv8_cache *c,
@@ -111,16 +112,9 @@ int n550_attention_prefill_kv8(void *stream, const uint16_t *q, int ldq, const n
     a.rows = L;
     const size_t need = n550_attention_prefill_kv8_workspace(n_seqs, L, pos0);
     float *ws = split_ws(workspace, workspace_bytes, need);
-    if (L > KV8_FEW && ws) return launch_kv8_prefill((cudaStream_t)stream, a, ws);
-    // few queries, or no workspace: the streaming kernel, KV8_FEW queries a pass
-    if (L <= KV8_FEW) a.part = ws;
-    for (int j = 0; j < L; j += KV8_FEW) {
-        a.row0 = j;
-        a.pos0 = pos0 + j;
-        a.L = L - j < KV8_FEW ? L - j : KV8_FEW;
-        if (int rc = launch_kv8_attn((cudaStream_t)stream, a)) return rc;
-    }
-    return N550_OK;
+    if (ws && !kv8_in_passes(n_seqs, L, pos0)) return launch_kv8_prefill((cudaStream_t)stream, a, ws);
+    a.part = ws;                                   // (no workspace: passes without splits)
+    return launch_kv8_passes((cudaStream_t)stream, a);
 }
 
 int n550_kv8_select_blocks(void *stream, const uint16_t *q, int ldq, const n550_kv8_cache *c, int layer,

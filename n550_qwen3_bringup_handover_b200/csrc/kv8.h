@@ -82,6 +82,10 @@ struct Kv8AttnArgs {
 
 int launch_kv8_append(cudaStream_t st, const Kv8AppendArgs &a, bool f32, int n_seqs);
 constexpr int KV8_FEW = 8;     // most queries per sequence of launch_kv8_attn
+// Whether L queries per sequence at positions pos0 .. take the streaming kernel, in
+// passes of KV8_FEW, rather than launch_kv8_prefill; and those passes.
+bool kv8_in_passes(int n_seqs, int L, int pos0);
+int launch_kv8_passes(cudaStream_t st, const Kv8AttnArgs &a);
 // Many queries: codes written out as BF16 to `ws` (kv8_prefill_workspace bytes), then
 // the BF16 prefill kernel.
 int launch_kv8_prefill(cudaStream_t st, const Kv8AttnArgs &a, void *ws);

@@ -879,10 +879,16 @@ int launch(cudaStream_t st, const CUtensorMap &tk, const CUtensorMap &tv, const 
 
 }  // namespace
 
+// For calls of up to L queries: the instances differ in their number of runs, so the
+// largest need of all of them.
 size_t kv8_attn_workspace(int n_seqs, int L) {
     if (n_seqs <= 0 || L <= 0) return 0;
-    const size_t n = max_ctas(L);
-    return n * sizeof(Cross) + n * 2 * (2 * L) * (KV8_HD + 2) * sizeof(float);
+    size_t most = 0;
+    for (int l = 1; l <= L; l++) {
+        const size_t n = max_ctas(l), need = n * sizeof(Cross) + n * 2 * (2 * l) * (KV8_HD + 2) * sizeof(float);
+        most = need > most ? need : most;
+    }
+    return most;
 }
 
 int launch_kv8_attn(cudaStream_t st, const Kv8AttnArgs &a) {

@@ -64,6 +64,31 @@ kv8_write_out_kernel(const Kv8View c, const int32_t *seq_ids, int len, uint16_t 
 
 }  // namespace
 
+// Time of both ways in us, from B200 measurements: a pass of up to 8 queries streams
+// the codes at 2.2 TB/s after 15 us; writing out moves 768 bytes per position and
+// head at 5 TB/s, and then a CTA takes 2 us for each 128 positions of 128 queries of
+// a KV head, the longest context of a wave of 148 of them deciding. Measured
+// (passes / whole, sequences x queries over positions): 8 x 5 over 2005 27 / 53, 8 x 16
+// over 2016 60 / 54, 64 x 8 over 508 51 / 82, 2 x 8 over 30008 67 / 550 (16 CTAs).
+bool kv8_in_passes(int n_seqs, int L, int pos0) {
+    if (L <= KV8_FEW) return true;
+    const double positions = (double)n_seqs * ((double)pos0 + L) * KV8_NKV;
+    const double passes = (L + KV8_FEW - 1) / KV8_FEW * (15.0 + positions * 256 / 2.2e6);
+    const double items = (double)n_seqs * KV8_NKV * ((L + 127) / 128), waves = (double)(((long long)items + 147) / 148);
+    return passes < 4.0 + positions * 768 / 5e6 + waves * (((double)pos0 + L) / 128) * 2.0;
+}
+
+int launch_kv8_passes(cudaStream_t st, const Kv8AttnArgs &a) {
+    Kv8AttnArgs p = a;
+    for (int j = 0; j < a.L; j += KV8_FEW) {
+        p.row0 = j;
+        p.pos0 = a.pos0 + j;
+        p.L = a.L - j < KV8_FEW ? a.L - j : KV8_FEW;
+        if (int rc = launch_kv8_attn(st, p)) return rc;
+    }
+    return N550_OK;
+}
+
 size_t kv8_prefill_workspace(int n_seqs, int L, int pos0) {
     return 2 * sizeof(uint16_t) * (size_t)n_seqs * KV8_NKV * ((size_t)pos0 + L) * KV8_HD;
 }

@@ -815,9 +815,9 @@ int run_attention_kv8(n550_model *m, cudaStream_t st, bool decode, const int32_t
     a.L = a.rows = Lc;
     a.n_seqs = Sc;
     a.n_select = -1;
-    if (Lc <= KV8_FEW) {
+    if (kv8_in_passes(Sc, Lc, p0)) {
         a.part = (float *)m->kv8_ws;
-        STEP(N550_PROF_ATTN, 2, launch_kv8_attn(st, a));
+        STEP(N550_PROF_ATTN, 2 * ((Lc + KV8_FEW - 1) / KV8_FEW), launch_kv8_passes(st, a));
         return N550_OK;
     }
     const int group = (int)std::min<size_t>(Sc, m->kv8_out_bytes / kv8_prefill_workspace(1, Lc, p0));

@@ -80,6 +80,18 @@ def test_empty_calls_do_nothing():
     assert L.n550_attention_prefill_kv8_workspace(0, 4, 0) == 0
 
 
+def test_workspace_covers_every_pass():
+    """A call of L queries may end with a pass of any smaller number, whose instance
+    has more runs: the workspace never shrinks with L."""
+    L = n5.lib()
+    sizes = [L.n550_attention_prefill_kv8_workspace(1, q, 100000) for q in range(1, 9)]
+    assert sizes == sorted(sizes) and sizes[0] == L.n550_attention_kv8_workspace(1)
+    # 296 runs of 4 queries: two partials of 8 columns x (128 + max + sum) and a record each
+    assert sizes[7] >= 296 * (2 * 8 * 130 * 4 + 16)
+    # many queries over a context that the passes would read too often: the context as BF16
+    assert L.n550_attention_prefill_kv8_workspace(3, 512, 88) == 3 * 600 * 4096
+
+
 def test_cache_class_refuses_tensors():
     with pytest.raises(ValueError):
         n5.KV8Cache(0, 64)

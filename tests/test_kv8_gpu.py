@@ -294,7 +294,7 @@ def test_decode_nan_stays_in_its_place():
 # ---------------------------------------------------------------------------
 # prefill
 # ---------------------------------------------------------------------------
-@pytest.mark.parametrize("n,L", [(1, 2), (2, 3), (3, 4), (2, 5), (1, 8), (40, 6)])
+@pytest.mark.parametrize("n,L", [(1, 2), (2, 3), (3, 4), (2, 5), (1, 8), (40, 6), (1, 12), (1, 13), (2, 21), (1, 160)])
 def test_few_queries_over_long_contexts(n, L):
     """Contexts cut into many runs: against a binary64 product on the GPU."""
     pos0 = 6000 if n < 10 else 700
