@@ -58,6 +58,13 @@ __device__ __forceinline__ int kv8_ctx(const Kv8View &c, int slot, int pos) {
     return slot < 0 || slot >= c.n_slots || pos < 0 ? 0 : min(pos, c.max_len - 1) + 1;
 }
 
+// FP16 pair -> two e4m3 codes, as above.
+__device__ __forceinline__ uint32_t f16x2_to_e4m3x2(uint32_t h) {
+    uint16_t r;
+    asm("cvt.rn.satfinite.e4m3x2.f16x2 %0, %1;" : "=h"(r) : "r"(h));
+    return r;
+}
+
 struct Kv8AppendArgs {
     Kv8View c;
     const void *k, *v;         // rows [n_seqs * L][ld], KV head h at columns 128 h ..

@@ -76,12 +76,6 @@ __device__ __forceinline__ uint32_t hmax2(uint32_t a, uint32_t b) {
     asm("max.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
     return r;
 }
-// FP16 pair that holds e4m3 values -> its two codes (exact).
-__device__ __forceinline__ uint32_t f16x2_to_e4m3x2(uint32_t h) {
-    uint16_t r;
-    asm("cvt.rn.satfinite.e4m3x2.f16x2 %0, %1;" : "=h"(r) : "r"(h));
-    return r;
-}
 constexpr uint32_t kHInf = 0x7C007C00u, kHNegInf = 0xFC00FC00u;
 
 // ---------------------------------------------------------------------------

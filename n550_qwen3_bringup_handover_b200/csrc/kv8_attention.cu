@@ -20,8 +20,9 @@
 // weights in e4m3 parts, four bits a part:
 //   q = 2^a (h + l / 16): two parts hold a BF16 value whole, down to 2^-21 of the
 //       row's largest;
-//   w = 2^-8 (w1 + w2 / 16 + w3 / 256): three parts hold a softmax weight to 12
-//       bits (2^-13 half a step), or 2^-26 of the tile's largest for the small ones.
+//   w = 2^-8 (w1 + w2 / 16 + w3 / 256): a softmax weight is rounded to FP16's 11 bits
+//       (2^-12 of it at most), which three parts hold whole, or as a multiple of
+//       2^-25 of the tile's largest where it is small.
 // Weights are relative to the largest score of their own tile, so each tile's O is
 // finished by its MMAs and added up, scaled, in registers: an O that stays in
 // TMEM over the tiles has to be scaled there whenever a maximum grows (in 4 of 10
@@ -62,8 +63,9 @@ struct Lay {
 };
 
 // LT: most query tokens (2 heads each) of an instance. S has 4 columns a token, O
-// (and P) 6, at most 12 of 16 for each softmax group (so that a row of P has the
-// same swizzle in every group).
+// (and P) 6, at most 12 of 16 for each softmax group. A group's P is [128 positions]
+// [16 columns] bytes, an MN-major operand without swizzle, so that a position's
+// weights are one 16-byte store: column 6 j + 2 k + h is part k of token j, head h.
 template <int LT> constexpr int groups() { return LT == 1 ? 1 : LT / 2; }       // of four softmax warps
 template <int LT> constexpr int s_cols() { return LT == 1 ? 16 : 4 * LT; }
 template <int LT> constexpr int p_cols() { return 16 * groups<LT>(); }
@@ -101,9 +103,17 @@ __device__ __forceinline__ void umma_e4m3(uint32_t d_tmem, uint64_t a_desc, uint
         ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
         : "memory");
 }
-// Instruction descriptor: D FP32, A and B e4m3 (format 0), M = 128; a_mn: A is MN-major.
-__host__ __device__ constexpr uint32_t idesc_e4m3(int N, int a_mn) {
-    return (1u << 4) | ((uint32_t)a_mn << 15) | ((uint32_t)(N >> 3) << 17) | ((128u >> 4) << 24);
+// Instruction descriptor: D FP32, A and B e4m3 (format 0), M = 128; mn: both MN-major.
+__host__ __device__ constexpr uint32_t idesc_e4m3(int N, int mn) {
+    return (1u << 4) | ((uint32_t)mn << 15) | ((uint32_t)mn << 16) | ((uint32_t)(N >> 3) << 17) | ((128u >> 4) << 24);
+}
+
+// Shared-memory descriptor of an MN-major 8-bit operand without swizzle: 16 MN
+// elements x 8 K rows are 128 bytes in one piece, the next 8 K rows `k_step` and the
+// next 16 MN elements `mn_step` bytes on.
+__device__ __forceinline__ uint64_t umma_desc_mn(uint32_t smem_addr, uint32_t k_step, uint32_t mn_step) {
+    return (uint64_t)(smem_addr >> 4 & 0x3FFFu) | (uint64_t)(k_step >> 4) << 16 | (uint64_t)(mn_step >> 4) << 32 |
+           (uint64_t)1 << 46;
 }
 
 __device__ __forceinline__ void tmem_ld_x4(uint32_t taddr, uint32_t *r) {
@@ -142,6 +152,37 @@ __device__ __forceinline__ bool mbar_test(uint64_t *bar, uint32_t parity) {
 }
 __device__ __forceinline__ bool warp_wait(uint64_t *bar, uint32_t parity) {
     return __all_sync(0xFFFFFFFFu, mbar_wait(bar, parity));
+}
+__device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
+    uint32_t r;
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+__device__ __forceinline__ uint32_t hmul2(uint32_t a, uint32_t b) {
+    uint32_t r;
+    asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+}
+__device__ __forceinline__ uint32_t hfma2(uint32_t a, uint32_t b, uint32_t c) {
+    uint32_t r;
+    asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(c));
+    return r;
+}
+// 2 or 4 consecutive floats in shared memory, aligned to their size.
+template <int N>
+__device__ __forceinline__ void get_row(const float *p, float (&x)[N]) {
+    if constexpr (N == 2) {
+        const float2 v = *(const float2 *)p;
+        x[0] = v.x; x[1] = v.y;
+    } else {
+        const float4 v = *(const float4 *)p;
+        x[0] = v.x; x[1] = v.y; x[2] = v.z; x[3] = v.w;
+    }
+}
+template <int N>
+__device__ __forceinline__ void put_row(float *p, const float (&x)[N]) {
+    if constexpr (N == 2) *(float2 *)p = make_float2(x[0], x[1]);
+    else *(float4 *)p = make_float4(x[0], x[1], x[2], x[3]);
 }
 // Byte offset of byte k of row n in an operand of 128-byte rows, 128-byte swizzle.
 __device__ __forceinline__ uint32_t sw(int n, int k) { return n * 128 + ((((k >> 4) ^ n) & 7) << 4) + (k & 15); }
@@ -488,7 +529,8 @@ kv8_attn_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
             const int steps = w_half ? 2 : 4;
             for (int k = 0; k < steps; k++)
                 if (elect_one_sync())
-                    umma_e4m3(d, umma_desc_sw128_mn(v + k * 4096, 0), umma_desc_sw128(pp + k * 32), id_o, k > 0 ? 1u : 0u);
+                    umma_e4m3(d, umma_desc_sw128_mn(v + k * 4096, 0), umma_desc_mn(pp + k * 512, 128, 2048), id_o,
+                              k > 0 ? 1u : 0u);
             if (elect_one_sync()) { umma_commit(&empty[w_st]); umma_commit(&pv_done[b]); }
             __syncwarp();
             return true;
@@ -613,8 +655,9 @@ kv8_attn_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
             tc_fence_before();
 #pragma unroll
             for (int c = 0; c < NG; c++) {
-                const float part = fmaf(fmaf(__uint_as_float(x[3 * c + 2]), 0.0625f, __uint_as_float(x[3 * c + 1])), 0.0625f,
-                                        __uint_as_float(x[3 * c]));
+                const int n = 6 * (c >> 1) + (c & 1);
+                const float part = fmaf(fmaf(__uint_as_float(x[n + 4]), 0.0625f, __uint_as_float(x[n + 2])), 0.0625f,
+                                        __uint_as_float(x[n]));
                 const float mn = fmaxf(m[c], tm[c]), ref = mn == -INFINITY ? 0.f : mn;
                 const float a = ex2(m[c] - ref), b = ex2(tm[c] - ref);
                 o[c] = o[c] * a + part * (b * tv);
@@ -692,39 +735,37 @@ kv8_attn_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
                         if (c < ng) {
                             const float q = fmaf(__uint_as_float(v[2 * c + 1]), 0.0625f, __uint_as_float(v[2 * c]));
                             if (blk >= 0 && pos <= lim + c / 2) s[c] = q * qf[c] * kf;
-                            const float mx = warp_max(s[c]);
-                            if (lane == 0) xmax[bars & 1][qw][c0 + c] = mx;
                         }
+                        x[c] = warp_max(s[c]);
                     }
+                    if (lane == 0) put_row<NG>(&xmax[bars & 1][qw][c0], x);
                 }
                 const float (*xm)[NC] = xmax[bars & 1];            // [warp][column]
                 if (meet(dead)) break;
                 vmax = w.blk[1] < 0 ? w.vs[0] : fmaxf(w.vs[0], w.vs[1]);
-                uint8_t *dst = sP + ((t & 1) * NP + 16 * grp) * 128;     // (P.V of tile t - 2 was collected)
+                uint8_t *dst = sP + (t & 1) * NP * 128 + grp * 2048;     // (P.V of tile t - 2 was collected)
                 const float ratio = blk < 0 || vmax == 0.f ? 0.f : 256.f * ((half ? w.vs[1] : w.vs[0]) / vmax);
+                float xw[4][NG];
+#pragma unroll
+                for (int k = 0; k < 4; k++) get_row<NG>(&xm[k][c0], xw[k]);
+                uint32_t part[8] = {};                             // columns in pairs of two heads, 16 bits each
 #pragma unroll
                 for (int c = 0; c < NG; c++) {
-                    x[c] = fmaxf(fmaxf(xm[0][c0 + c], xm[1][c0 + c]), fmaxf(xm[2][c0 + c], xm[3][c0 + c]));
-                    if (c >= ng) x[c] = -INFINITY;
-                    sum[c] = 0.f;
+                    x[c] = fmaxf(fmaxf(xw[0][c], xw[1][c]), fmaxf(xw[2][c], xw[3][c]));
+                    sum[c] = ex2(s[c] - (x[c] == -INFINITY ? 0.f : x[c]));
                 }
 #pragma unroll
                 for (int c = 0; c < NG; c += 2) {
-                    if (c >= ng) break;
-                    float a = sum[c] = ex2(s[c] - (x[c] == -INFINITY ? 0.f : x[c]));
-                    float b = sum[c + 1] = ex2(s[c + 1] - (x[c + 1] == -INFINITY ? 0.f : x[c + 1]));
-                    a *= ratio;
-                    b *= ratio;
+                    uint32_t a = pack_f16x2(sum[c] * ratio, sum[c + 1] * ratio);
 #pragma unroll
                     for (int k = 0; k < 3; k++) {
-                        const uint32_t e = f32x2_to_e4m3x2(a, b);
-                        dst[sw(3 * c + k, row)] = (uint8_t)e;
-                        dst[sw(3 * c + 3 + k, row)] = (uint8_t)(e >> 8);
-                        const float2 f = e4m3x2_to_f32x2(e);
-                        a = (a - f.x) * 16.f;
-                        b = (b - f.y) * 16.f;
+                        part[3 * (c / 2) + k] = f16x2_to_e4m3x2(a);
+                        // what is left, times 16 (both steps exact)
+                        if (k < 2) a = hfma2(e4m3x2_to_f16x2(part[3 * (c / 2) + k]), 0xCC00CC00u, hmul2(a, 0x4C004C00u));
                     }
                 }
+                *(uint4 *)(dst + row * 16) = make_uint4(part[0] | part[1] << 16, part[2] | part[3] << 16,
+                                                        part[4] | part[5] << 16, part[6] | part[7] << 16);
                 // codes of V behind the context may be anything, NaN too: a weight of 0 needs a 0
                 if (grp == 0 && blk >= 0 && pos >= w.ctx) {
                     uint4 *z = (uint4 *)(ring + st * STAGE + 2 * BLK + row * 128);

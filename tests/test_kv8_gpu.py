@@ -3,8 +3,8 @@ kv8_oracle.py: append bit for bit, selections index for index, attention within
 the roundings it makes.
 
 Attention tolerance, per element: the output is rounded to BF16 (2^-8 |out|);
-the softmax weights enter the tensor cores in 12 bits (2^-13 each; 2^-11 would be
-FP16's) or, on the whole-tile prefill route, in BF16 (2^-8 each), and small ones as
+the softmax weights enter the tensor cores in FP16's 11 bits (2^-12 each; the
+allowance is 2^-11) or, on the whole-tile prefill route, in BF16 (2^-8 each), and small ones as
 multiples of 2^-25 of the largest, which moves the result by at most that part of
 mass (Cache.attend); sums and scores in FP32 and the hardware exponential add less
 than 2^-13 of mass at these sizes (score errors below 2^-15: 128 products of
