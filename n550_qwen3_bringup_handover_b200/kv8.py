@@ -73,13 +73,12 @@ class KV8Cache:
 
 def _ids(seq_ids, pos=None):
     """Number of sequences; both must be contiguous int32 vectors of that length."""
-    import torch
-    for name, t in (("seq_ids", seq_ids), ("pos", pos)):
-        if t is not None and (t.dtype != torch.int32 or t.dim() != 1 or not t.is_contiguous()):
-            raise ValueError(f"{name} must be a contiguous int32 vector")
-    n = seq_ids.shape[0]
-    if pos is not None and pos.shape[0] != n:
-        raise ValueError(f"pos must hold {n} positions")
+    from torch import int32
+    n, = shape = seq_ids.shape if seq_ids.dim() == 1 else (-1,)
+    if n < 0 or seq_ids.dtype != int32 or not seq_ids.is_contiguous():
+        raise ValueError("seq_ids must be a contiguous int32 vector")
+    if pos is not None and (pos.shape != shape or pos.dtype != int32 or not pos.is_contiguous()):
+        raise ValueError(f"pos must be a contiguous int32 vector of {n}")
     return n
 
 
@@ -116,9 +115,9 @@ def _q_out(q, rows, out):
     return ldq, out, _rows("out", out, rows, _NH * _HD, (torch.bfloat16,))
 
 
-def _workspace(nbytes, device):
-    import torch
-    return torch.empty(nbytes, dtype=torch.uint8, device=device)
+def _workspace(nbytes, q):
+    # in q's type: new_empty takes device and dtype over without parsing them
+    return q.new_empty((nbytes + 1) // 2)
 
 
 def attention_decode_kv8(q, cache, seq_ids, pos, layer, out=None, split=True):
@@ -130,7 +129,7 @@ def attention_decode_kv8(q, cache, seq_ids, pos, layer, out=None, split=True):
     st = _stream(cache, q, seq_ids, pos, out)
     L = lib()
     nbytes = L.n550_attention_kv8_workspace(n) if split else 0
-    ws = _workspace(nbytes, q.device) if nbytes else None
+    ws = _workspace(nbytes, q) if nbytes else None
     check(L.n550_attention_decode_kv8(st, q.data_ptr(), ldq, cache._ref, layer, seq_ids.data_ptr(),
                                       pos.data_ptr(), n, out.data_ptr(), ldo, ws.data_ptr() if nbytes else None, nbytes),
           "n550_attention_decode_kv8")
@@ -149,7 +148,7 @@ def attention_sparse_kv8(q, cache, seq_ids, pos, blocks, layer, out=None, split=
     st = _stream(cache, q, seq_ids, pos, blocks, out)
     L = lib()
     nbytes = L.n550_attention_kv8_workspace(n) if split else 0
-    ws = _workspace(nbytes, q.device) if nbytes else None
+    ws = _workspace(nbytes, q) if nbytes else None
     check(L.n550_attention_sparse_kv8(st, q.data_ptr(), ldq, cache._ref, layer, seq_ids.data_ptr(),
                                       pos.data_ptr(), blocks.data_ptr(), blocks.shape[2], n,
                                       out.data_ptr(), ldo, ws.data_ptr() if nbytes else None, nbytes), "n550_attention_sparse_kv8")
@@ -166,7 +165,7 @@ def attention_prefill_kv8(q, cache, seq_ids, L, pos0, layer, out=None, workspace
     st = _stream(cache, q, seq_ids, out)
     lb = lib()
     nbytes = lb.n550_attention_prefill_kv8_workspace(n, L, pos0) if workspace else 0
-    ws = _workspace(nbytes, q.device) if nbytes else None
+    ws = _workspace(nbytes, q) if nbytes else None
     check(lb.n550_attention_prefill_kv8(st, q.data_ptr(), ldq, cache._ref, layer, seq_ids.data_ptr(), n,
                                         L, pos0, out.data_ptr(), ldo, ws.data_ptr() if nbytes else None, nbytes),
           "n550_attention_prefill_kv8")
