@@ -16,8 +16,8 @@
 // as the 128-row side of O^T = V^T P^T. No code passes through a register; the
 // mma.sync form of this kernel, which turned codes into FP16 there, issued about
 // 390 instructions per warp and 16 positions and stopped at 4.7 TB/s (256
-// sequences x 1152 positions, 114 us). The 8-column side has room for queries and
-// weights in e4m3 parts, four bits a part:
+// sequences x 1152 positions, 114 us; now 103, 5.2 TB/s). The 16-column side has room for
+// queries and weights in e4m3 parts, four bits a part:
 //   q = 2^a (h + l / 16): two parts hold a BF16 value whole, down to 2^-21 of the
 //       row's largest;
 //   w = 2^-8 (w1 + w2 / 16 + w3 / 256): a softmax weight is rounded to FP16's 11 bits
@@ -331,14 +331,16 @@ kv8_attn_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
     tc_fence_after();
     const uint32_t tmem = tmem_slot, tS = tmem, tO = tmem + 2 * NS;
     dep_launch();
+    // Block lists, positions, scales, codes and queries all come from earlier kernels, and
+    // out and the workspace may be in use by them; what every CTA reads first may be on
+    // its way to L2 before they end. (All warps wait here: the limits of the waits below
+    // do not count the time of earlier kernels.)
+    if (warp == 0 && lay.kind == LAY_RAGGED && lane * 32 < p.n_seqs) {
+        asm volatile("prefetch.global.L2 [%0];" ::"l"(p.pos + lane * 32));
+        asm volatile("prefetch.global.L2 [%0];" ::"l"(p.seq_ids + lane * 32));
+    }
+    dep_wait();
     if (warp == 0) {
-        // Block lists, positions, scales, codes and queries all come from earlier kernels;
-        // what every CTA reads first may be on its way to L2 before they end.
-        if (lay.kind == LAY_RAGGED && lane * 32 < p.n_seqs) {
-            asm volatile("prefetch.global.L2 [%0];" ::"l"(p.pos + lane * 32));
-            asm volatile("prefetch.global.L2 [%0];" ::"l"(p.seq_ids + lane * 32));
-        }
-        dep_wait();
         Cur cur{};
         int n_units;
         long long u0 = 0, total = 0;
@@ -617,7 +619,6 @@ kv8_attn_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
             if (flags & R_END) break;
         }
     } else {
-        dep_wait();                              // out and the workspace may be in use by earlier kernels
         // ---------------- softmax and output: a group's columns c0 .. c0 + NG - 1 ----------------
         constexpr int NG = NC / G;
         const int grp = (warp - 2) >> 2, c0 = grp * NG, ng = min(NG, 2 * p.L - c0);     // ng <= 0: nothing to do but keep step

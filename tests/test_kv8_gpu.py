@@ -118,7 +118,9 @@ def test_append_rewound_and_reused_slots():
         assert_state(c, ref, 1)
 
 
-def test_append_special_values():
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("L", [20, 6])
+def test_append_special_values(L, dtype):
     inf, nan = float("inf"), float("nan")
     k = rows(20, 1024, torch.float32, 8)
     k[0, 0], k[1, 1], k[2, 2], k[3, 3] = inf, -inf, nan, 3.3e38
@@ -128,8 +130,9 @@ def test_append_special_values():
     k[:, 512:640] = inf                                     # nothing but infinities
     k[5, 640:768] = 448.0 * 2 ** 9                          # the border of a scale, and just over it
     k[5, 768:896] = torch.nextafter(torch.tensor(448.0 * 2 ** 9), torch.tensor(inf))
+    k = k[:L].to(dtype)
     v = -k.flip(1)
-    for L, p in [(20, 0), (20, 30)]:
+    for p in (0, 30):
         c, ref = fresh(1, 64), Cache.of(fresh(1, 64), 0)
         if p:
             z = rows(30, 1024, torch.float32, 9)
@@ -509,6 +512,38 @@ def test_prompt_then_tokens_with_selection():
         pos += 1
         at += 1
     assert_state(c, ref, 1)
+
+
+def test_workspaces_of_the_c_interface():
+    """Garbage in the workspace changes nothing; one too small or unaligned counts as none."""
+    import ctypes as C
+    L = n5.lib()
+    c, ref = filled(2, 3000, 430)
+    q, ids, pos = rows(2, 2048, torch.bfloat16, 431).cuda(), i32([1, 0]), i32([2999, 2000])
+    st = torch.cuda.current_stream().cuda_stream
+    need = L.n550_attention_kv8_workspace(2)
+    ws = torch.empty(need + 32, dtype=torch.uint8, device="cuda")
+
+    def call(ptr, n):
+        out = torch.empty((2, 2048), dtype=torch.bfloat16, device="cuda")
+        assert L.n550_attention_decode_kv8(st, q.data_ptr(), 2048, C.byref(c._c), 1, ids.data_ptr(), pos.data_ptr(), 2,
+                                           out.data_ptr(), 2048, ptr, n) == n5.OK
+        return out
+
+    got = []
+    for fill in (0, 0x7F, 0xFF):
+        ws.fill_(fill)
+        got.append(call(ws.data_ptr(), need))
+    assert_near(got[0], *ref.attend(q.cpu(), [1, 0], [2999, 2000]))
+    assert torch.equal(got[0], got[1]) and torch.equal(got[0], got[2])
+    whole = call(None, 0)
+    for ptr, n in ((ws.data_ptr(), need - 1), (ws.data_ptr() + 8, need)):
+        assert torch.equal(call(ptr, n), whole)
+    q40 = rows(2 * 40, 2048, torch.bfloat16, 432).cuda()
+    out = torch.empty((80, 2048), dtype=torch.bfloat16, device="cuda")
+    assert L.n550_attention_prefill_kv8(st, q40.data_ptr(), 2048, C.byref(c._c), 1, ids.data_ptr(), 2, 40, 100,
+                                        out.data_ptr(), 2048, ws.data_ptr(), 64) == n5.OK
+    assert torch.equal(out, n5.attention_prefill_kv8(q40, c, ids, 40, 100, 1, workspace=False))
 
 
 def test_captured_step_replays_on_new_inputs():
