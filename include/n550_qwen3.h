@@ -459,8 +459,8 @@ int n550_qwen3_fused_decode(int on);
  * the bytes a decode step reads) instead of BF16 (on = 1), or goes back (0, the
  * default). Either way the cache starts empty: call it before the first prefill.
  * Synchronises and allocates; the other cache's memory is freed. The q/k/v step
- * then runs as GEMM, row kernel (QK-norm, RoPE) and n550_kv8_append, the attention
- * as n550_attention_decode_kv8 / n550_attention_prefill_kv8. Fast mode only
+ * then leaves BF16 K/V rows (after QK-norm and RoPE, in the GEMM's epilogue where the
+ * batch has one) for n550_kv8_append, and the attention runs as n550_attention_decode_kv8 / n550_attention_prefill_kv8. Fast mode only
  * (N550_ERR_UNSUPPORTED otherwise, and for a forward with the tensor dump on).
  * n550_qwen3_kv8_cache gives the cache of such a model (28 layers, max_seqs slots)
  * for calls of the entry points above, N550_ERR_ARG without one. No counterpart

@@ -356,9 +356,11 @@ gemm_skinny_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constan
                     }
                 } else {
                     const int kvh = (hd - 16) & 7;
-                    uint16_t *dst = (hd < 24 ? ep.kc : ep.vc) +
-                                    (((size_t)(seq * N_LAYERS + ep.layer) * N_KV_HEADS + kvh) * ep.max_len +
-                                     pos) * HEAD;
+                    uint16_t *dst = ep.kv_rows
+                                        ? ep.kv_rows + (size_t)t * 2 * N_KV_HEADS * HEAD + (hd - 16) * HEAD
+                                        : (hd < 24 ? ep.kc : ep.vc) +
+                                              (((size_t)(seq * N_LAYERS + ep.layer) * N_KV_HEADS + kvh) *
+                                                   ep.max_len + pos) * HEAD;
 #pragma unroll
                     for (int j = 0; j < 4; j++) dst[lane + 32 * j] = f32_to_bf16_rne(v[j]);
                 }
@@ -532,7 +534,7 @@ int launch_gemm_skinny(cudaStream_t st, int epi, const uint16_t *x, int ldx, con
     const bool silu = epi == SK_EPI_SILU;
     if (silu && (!w2 || (((uintptr_t)w2) & 15) || !ep.h)) return N550_ERR_ARG;
     if ((epi == SK_EPI_F32 || epi == SK_EPI_RESID) && !ep.out) return N550_ERR_ARG;
-    if (epi == SK_EPI_QKV && (N != 32 * HEAD || !ep.kc || !ep.vc || !ep.tok_pos || !ep.tok_seq ||
+    if (epi == SK_EPI_QKV && (N != 32 * HEAD || (!ep.kv_rows && (!ep.kc || !ep.vc)) || !ep.tok_pos || !ep.tok_seq ||
                               !ep.rope || !ep.q_norm || !ep.k_norm || (!ep.q_f32 && !ep.q_bf16)))
         return N550_ERR_ARG;
     const int tn = T <= 32 ? 32 : 64;

@@ -24,6 +24,7 @@ struct SkEpilogue {
     uint16_t *q_bf16;           // [T][ldq] BF16 queries
     int ldq;
     uint16_t *kc, *vc;          // KV cache [seq][layer][kv_head][pos][128]
+    uint16_t *kv_rows;          // instead of the caches: K and V heads as rows [T][2048] (or NULL)
     int layer, max_len;
     const int32_t *tok_pos, *tok_seq;   // per token
     const uint16_t *q_norm, *k_norm;    // BF16 [128]

@@ -255,7 +255,8 @@ __device__ __forceinline__ void epilogue_qkv(const TcQkv &p, uint32_t *stg, int 
         const int kvh = (head - 16) & 7;
         uint16_t *cache = head < 24 ? p.kc : p.vc;
         const size_t slot = ((size_t)p.tok_seq[mc] * 28 + p.layer) * 8 + kvh;
-        dst_row = cache + (slot * p.max_len + pos) * 128;
+        dst_row = p.kv_rows ? p.kv_rows + (size_t)mc * 2048 + (head - 16) * 128
+                            : cache + (slot * p.max_len + pos) * 128;
     }
     if (!row_ok) dst_row = nullptr;
     float scale = 1.f;
@@ -352,7 +353,8 @@ __device__ __forceinline__ void epilogue_qkv_half(const TcQkv &p, uint32_t *stg,
         const int kvh = (head - 16) & 7;
         uint16_t *cache = head < 24 ? p.kc : p.vc;
         const size_t slot = ((size_t)p.tok_seq[mc] * 28 + p.layer) * 8 + kvh;
-        dst_row = cache + (slot * p.max_len + pos) * 128;
+        dst_row = p.kv_rows ? p.kv_rows + (size_t)mc * 2048 + (head - 16) * 128
+                            : cache + (slot * p.max_len + pos) * 128;
     }
     if (!row_ok) dst_row = nullptr;
     float scale = 1.f;
@@ -995,7 +997,7 @@ int launch_gemm_tc_qkv(cudaStream_t st, const uint16_t *a, int lda, const uint16
                        const TcQkv &q, int M, int K, int max_ctas) {
     if (M <= 0) return N550_OK;
     if (!tc_shape_ok(a, lda, w, K, K)) return N550_ERR_UNSUPPORTED;
-    if (!q.q_bf16 || !q.kc || !q.vc || !q.tok_pos || !q.tok_seq || !q.rope ||
+    if (!q.q_bf16 || (!q.kv_rows && (!q.kc || !q.vc)) || !q.tok_pos || !q.tok_seq || !q.rope ||
         (q.ldq % 8))
         return N550_ERR_ARG;
     int rc = get_encoder();

@@ -22,6 +22,7 @@ struct TcQkv {
     uint16_t *q_bf16;          // [M, ldq] BF16 queries
     int ldq;
     uint16_t *kc, *vc;         // KV cache [seq][layer][kv_head][pos][128]
+    uint16_t *kv_rows;         // instead of the caches: K and V heads as rows [M][2048] (or NULL)
     int layer, max_len;
     const int32_t *tok_pos, *tok_seq;   // per row
     const uint16_t *q_norm, *k_norm;    // BF16 [128]

@@ -915,24 +915,16 @@ int run_layers_skinny(n550_model *m, cudaStream_t st, int T, bool decode, const 
     swiglu.ldh = INTER;
     for (int l = 0; l < NLAYER; l++) {
         SkEpilogue q{};
-        q.q_f32 = decode ? m->qf : nullptr;       // decode attention reads FP32 queries
-        q.q_bf16 = decode ? nullptr : m->qb;      // the tcgen05 prefill attention BF16
+        // decode attention reads FP32 queries, the tcgen05 kernels (prefill, 8-bit cache) BF16
+        q.q_f32 = decode && !m->kv8.k ? m->qf : nullptr;
+        q.q_bf16 = decode && !m->kv8.k ? nullptr : m->qb;
         q.ldq = QD;
-        q.kc = m->kc; q.vc = m->vc; q.layer = l; q.max_len = c.max_len;
+        q.kc = m->kc; q.vc = m->vc; q.kv_rows = m->kv_rows; q.layer = l; q.max_len = c.max_len;
         q.tok_pos = m->tok_pos; q.tok_seq = m->tok_seq;
         q.q_norm = W(m, l, 4); q.k_norm = W(m, l, 5);
         q.rope = m->rope;
-        if (m->kv8.k) {                           // K/V rows instead of cache positions
-            SkEpilogue f{};
-            f.out = m->qkv;
-            f.ldo = QKVD;
-            STEP(N550_PROF_GEMM_QKV, 1,
-                 launch_gemm_skinny(st, SK_EPI_F32, m->xb, H, m->wqkv[l], nullptr, H, T, QKVD, H, f));
-            STEP(N550_PROF_QKNORM_ROPE, 1, launch_qknorm_rope_kv(m, st, T, l, decode));
-        } else {
-            STEP(N550_PROF_GEMM_QKV, 1,
-                 launch_gemm_skinny(st, SK_EPI_QKV, m->xb, H, m->wqkv[l], nullptr, H, T, QKVD, H, q));
-        }
+        STEP(N550_PROF_GEMM_QKV, 1,
+             launch_gemm_skinny(st, SK_EPI_QKV, m->xb, H, m->wqkv[l], nullptr, H, T, QKVD, H, q));
         if ((rc = run_attention(m, st, T, decode, seq_ids, pos, Sc, Lc, p0, l))) return rc;
         STEP(N550_PROF_GEMM_O, 1,
              launch_gemm_skinny(st, SK_EPI_RESID, m->attn, QD, W(m, l, 6), nullptr, QD, T, H, QD, resid));
@@ -978,7 +970,7 @@ int run_layers(n550_model *m, cudaStream_t st, int T, bool decode, const int32_t
         return run_layers_skinny(m, st, T, decode, seq_ids, pos, Sc, Lc, p0, xl_ready);
     if (!exact && T > 8 && T < g_split_rows)
         return run_layers_split(m, st, T, decode, seq_ids, pos, Sc, Lc, p0, xl_ready);
-    const bool fused_qkv = !exact && !m->kv8.k && T >= g_split_rows;
+    const bool fused_qkv = !exact && T >= g_split_rows;
     const bool own_prep = decode && g_fused_prep && !m->kv8.k;      // decode attention finishes the raw q/k/v rows
     // the GEMV route of up to 4 rows normalises its input rows inside the q/k/v
     // and gate/up GEMVs (no norm launches)
@@ -998,7 +990,7 @@ int run_layers(n550_model *m, cudaStream_t st, int T, bool decode, const int32_t
             TcQkv q{};
             q.q_bf16 = m->qb;
             q.ldq = QD;
-            q.kc = m->kc; q.vc = m->vc; q.layer = l; q.max_len = c.max_len;
+            q.kc = m->kc; q.vc = m->vc; q.kv_rows = m->kv_rows; q.layer = l; q.max_len = c.max_len;
             q.tok_pos = m->tok_pos; q.tok_seq = m->tok_seq;
             q.q_norm = W(m, l, 4); q.k_norm = W(m, l, 5);
             q.rope = m->rope; q.eps = EPS;
