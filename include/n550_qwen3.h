@@ -460,7 +460,8 @@ int n550_qwen3_fused_decode(int on);
  * default). Either way the cache starts empty: call it before the first prefill.
  * Synchronises and allocates; the other cache's memory is freed. The q/k/v step
  * then leaves BF16 K/V rows (after QK-norm and RoPE, in the GEMM's epilogue where the
- * batch has one) for n550_kv8_append, and the attention runs as n550_attention_decode_kv8 / n550_attention_prefill_kv8. Fast mode only
+ * batch has one) for n550_kv8_append, and the attention runs as
+ * n550_attention_decode_kv8 / n550_attention_prefill_kv8. Fast mode only
  * (N550_ERR_UNSUPPORTED otherwise, and for a forward with the tensor dump on).
  * n550_qwen3_kv8_cache gives the cache of such a model (28 layers, max_seqs slots)
  * for calls of the entry points above, N550_ERR_ARG without one. No counterpart
