@@ -443,8 +443,9 @@ int n550_qwen3_split_rows(int rows);
 
 /* Decode steps that take the split-K or GEMV q/k/v route: the decode attention
  * kernel applies QK-norm and RoPE to the raw q/k/v rows and writes the new K/V
- * itself (1, default) or a separate row kernel does (0). Bit-identical
- * results either way. */
+ * itself (1, default) or a separate row kernel does (0). Over the 8-bit cache the
+ * row kernel also appends (1) or leaves that to n550_kv8_append's kernel (0).
+ * Bit-identical results either way. */
 int n550_qwen3_fused_attention_prep(int on);
 
 /* Decode steps of 1-4 sequences as one persistent kernel (1) or as the

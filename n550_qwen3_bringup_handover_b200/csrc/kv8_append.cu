@@ -10,21 +10,11 @@
 // every step above exact but for the one rounding; held codes lose bits only
 // where they fall below 2^-6. Rounding is monotone, so the extreme codes of a
 // block and channel, rescaled like the codes, stay its extreme codes.
-#include "kv8.h"
+#include "kv8_quant.cuh"
 #include "launch.h"
 
 namespace n550 {
 namespace {
-
-// Exponent e of the smallest power of two 2^e with amax <= 448 * 2^e, at least
-// -126 (so that the scale and its reciprocal are normal numbers).
-__device__ __forceinline__ int scale_exp(uint32_t amax_bits) {
-    const int e = (int)(amax_bits >> 23) - 127 - 8 + ((amax_bits & 0x7FFFFFu) > 0x600000u);
-    return max(e, -126);
-}
-__device__ __forceinline__ float pow2(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
-// 1 / s of a power of two with exponent in [-126, 120]
-__device__ __forceinline__ float inv_pow2(float s) { return __uint_as_float((254u << 23) - __float_as_uint(s)); }
 
 // FP32 bits of the largest magnitude of N words (FP32, or pairs of BF16), infinities
 // and NaN being larger than all numbers; FINITE: of the numbers alone.
@@ -55,26 +45,6 @@ __device__ __forceinline__ uint32_t codes4(const uint32_t *w, float inv) {
         }
     }
     return f32x2_to_e4m3x2(x[0], x[1]) | f32x2_to_e4m3x2(x[2], x[3]) << 16;
-}
-// Four held codes at a scale 1 / shrink times larger.
-__device__ __forceinline__ uint32_t shrink4(uint32_t c, float shrink) {
-    const float2 a = e4m3x2_to_f32x2(c & 0xFFFFu), b = e4m3x2_to_f32x2(c >> 16);
-    return f32x2_to_e4m3x2(a.x * shrink, a.y * shrink) | f32x2_to_e4m3x2(b.x * shrink, b.y * shrink) << 16;
-}
-// Codes with each NaN (0x7F, 0xFF) replaced by 0: what a NaN counts as in the bounds.
-__device__ __forceinline__ uint32_t nan_to_zero(uint32_t c) {
-    const uint32_t n = ((c & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u;     // 0x80 at each NaN
-    return n ? c & ~((n >> 7) * 0xFFu) : c;
-}
-__device__ __forceinline__ uint32_t hmin2(uint32_t a, uint32_t b) {
-    uint32_t r;
-    asm("min.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
-    return r;
-}
-__device__ __forceinline__ uint32_t hmax2(uint32_t a, uint32_t b) {
-    uint32_t r;
-    asm("max.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
-    return r;
 }
 constexpr uint32_t kHInf = 0x7C007C00u, kHNegInf = 0xFC00FC00u;
 

@@ -31,7 +31,7 @@
 #include "decode_fused.h"
 #include "gemm_skinny.h"
 #include "gemm_tc.h"
-#include "kv8.h"
+#include "kv8_quant.cuh"
 #include "launch.h"
 #include "ops.h"
 #include "synth.cuh"
@@ -240,12 +240,14 @@ __device__ __forceinline__ float sum_slices(const float *p, int ks, size_t slice
     return a;
 }
 
+// PUT8: one row per sequence, K and V quantised into the 8-bit cache at once.
+template <bool PUT8>
 __global__ void __launch_bounds__(1024)
 qknorm_rope_kv_kernel(const float *__restrict__ qkv, int ldqkv, int ks, size_t slice,
                       const uint16_t *__restrict__ qn, const uint16_t *__restrict__ kn,
                       const float2 *__restrict__ rope, const int32_t *__restrict__ tok_pos,
                       const int32_t *__restrict__ tok_seq, int layer, uint16_t *kc, uint16_t *vc,
-                      int max_len, uint16_t *q_bf16, float *q_f32, int ldq, uint16_t *kv_rows) {
+                      int max_len, uint16_t *q_bf16, float *q_f32, int ldq, uint16_t *kv_rows, const Kv8View kv8) {
     dep_wait();
     dep_launch();
     // One warp per head (32 per token): qkv row t, or (ks > 0) the sum of ks
@@ -282,6 +284,12 @@ qknorm_rope_kv_kernel(const float *__restrict__ qkv, int ldqkv, int ks, size_t s
         }
     } else {
         const int kvh = (hd - 16) & 7;
+        if (PUT8) {                                // the rounding of the rows that append reads
+#pragma unroll
+            for (int j = 0; j < 4; j++) v[j] = bf16_bits_to_f32(f32_to_bf16_rne(v[j]));
+            kv8_put_row(kv8, seq, kvh, hd >= 24, pos, v, lane);
+            return;
+        }
         // kv_rows: K and V heads as rows [t][2048] (the 8-bit cache's append reads them)
         uint16_t *dst = kv_rows ? kv_rows + (size_t)t * 2 * KVD + (hd - 16) * HDIM
                                 : (hd < 24 ? kc : vc) +
@@ -736,12 +744,23 @@ int mgemm(n550_model *m, cudaStream_t st, int epi, const uint16_t *a, int lda, c
                           ldc, M, N, K, 0);
 }
 
+// Decode attention takes the q/k/v rows before QK-norm and RoPE and finishes
+// them itself (the K/V write included) instead of a separate row kernel; over the
+// 8-bit cache, the row kernel appends instead of a separate kernel
+// (n550_qwen3_fused_attention_prep).
+bool g_fused_prep = true;
+
 int launch_qknorm_rope_kv(n550_model *m, cudaStream_t st, int T, int l, bool decode,
                           const float *src = nullptr, int ks = 0) {
-    N550_CUDA_TRY(launch_k(qknorm_rope_kv_kernel, T, 1024, 0, st, src ? src : m->qkv, QKVD, ks,
+    Kv8View kv8{};
+    const bool put8 = decode && m->kv8.k && g_fused_prep;
+    if (put8)
+        if (int rc = kv8_view(&m->kv8, l, &kv8)) return rc;
+    N550_CUDA_TRY(launch_k(put8 ? qknorm_rope_kv_kernel<true> : qknorm_rope_kv_kernel<false>, T, 1024, 0, st,
+                           src ? src : m->qkv, QKVD, ks,
                            (size_t)T * QKVD, W(m, l, 4), W(m, l, 5), m->rope, m->tok_pos, m->tok_seq, l,
                            m->kc, m->vc, m->cfg.max_len, decode && !m->kv8.k ? nullptr : m->qb,
-                           decode && !m->kv8.k ? m->qf : nullptr, QD, m->kv_rows));
+                           decode && !m->kv8.k ? m->qf : nullptr, QD, m->kv_rows, kv8));
     N550_LAUNCH_CHECK();
     return N550_OK;
 }
@@ -784,16 +803,11 @@ int launch_final_norm(cudaStream_t st, uint16_t *xl, const float *x, const uint1
         if ((rc = (expr))) return rc;                 \
     } while (0)
 
-// Decode attention takes the q/k/v rows before QK-norm and RoPE and finishes
-// them itself (the K/V write included) instead of a separate row kernel
-// (n550_qwen3_fused_attention_prep).
-bool g_fused_prep = true;
-
-// The same over the 8-bit cache: the layer's K/V rows (m->kv_rows) are appended and
-// the queries (m->qb) attend to the codes. A prefill of many queries works
+// The same over the 8-bit cache: the layer's K/V rows (m->kv_rows) are appended (unless
+// launch_qknorm_rope_kv did that) and the queries (m->qb) attend to the codes. A prefill of many queries works
 // through its sequences in groups whose contexts fit m->kv8_out as BF16.
 int run_attention_kv8(n550_model *m, cudaStream_t st, bool decode, const int32_t *seq_ids,
-                      const int32_t *pos, int Sc, int Lc, int p0, int l) {
+                      const int32_t *pos, int Sc, int Lc, int p0, int l, bool appended) {
     int rc = N550_OK;
     Kv8AppendArgs ap{};
     if ((rc = kv8_view(&m->kv8, l, &ap.c))) return rc;
@@ -804,7 +818,7 @@ int run_attention_kv8(n550_model *m, cudaStream_t st, bool decode, const int32_t
     ap.seq_ids = seq_ids;
     ap.pos = decode ? pos : nullptr;
     ap.pos0 = p0;
-    STEP(N550_PROF_QKNORM_ROPE, 1, launch_kv8_append(st, ap, false, Sc));
+    if (!appended) STEP(N550_PROF_QKNORM_ROPE, 1, launch_kv8_append(st, ap, false, Sc));
     Kv8AttnArgs a{};
     a.c = ap.c;
     a.q = m->qb; a.out = m->attn;
@@ -834,10 +848,11 @@ int run_attention_kv8(n550_model *m, cudaStream_t st, bool decode, const int32_t
 
 int run_attention(n550_model *m, cudaStream_t st, int T, bool decode, const int32_t *seq_ids,
                   const int32_t *pos, int Sc, int Lc, int p0, int l, bool q_in_bf16 = false,
-                  const float *raw_qkv = nullptr, int ks = 0) {
+                  const float *raw_qkv = nullptr, int ks = 0, bool row_kernel = false) {
     const n550_model_config &c = m->cfg;
     int rc = N550_OK;
-    if (m->kv8.k) return run_attention_kv8(m, st, decode, seq_ids, pos, Sc, Lc, p0, l);
+    if (m->kv8.k)
+        return run_attention_kv8(m, st, decode, seq_ids, pos, Sc, Lc, p0, l, row_kernel && decode && g_fused_prep);
     if (decode) {
         AttnDecodeArgs a{};
         a.q_f32 = q_in_bf16 ? nullptr : m->qf;
@@ -882,7 +897,7 @@ int run_layers_split(n550_model *m, cudaStream_t st, int T, bool decode, const i
             if ((rc = run_attention(m, st, T, decode, seq_ids, pos, Sc, Lc, p0, l, false, m->ws, ks))) return rc;
         } else {
             STEP(N550_PROF_QKNORM_ROPE, 1, launch_qknorm_rope_kv(m, st, T, l, decode, m->ws, ks));
-            if ((rc = run_attention(m, st, T, decode, seq_ids, pos, Sc, Lc, p0, l))) return rc;
+            if ((rc = run_attention(m, st, T, decode, seq_ids, pos, Sc, Lc, p0, l, false, nullptr, 0, true))) return rc;
         }
         STEP(N550_PROF_GEMM_O, 1, partials(m, st, m->attn, QD, W(m, l, 6), T, H, QD, &ks));
         STEP(N550_PROF_RMSNORM, 1, launch_resid_norm(st, m->x, m->ws, ks, T, W(m, l, 7), m->xb));
@@ -1004,7 +1019,7 @@ int run_layers(n550_model *m, cudaStream_t st, int T, bool decode, const int32_t
         // the fused QKV epilogue leaves BF16 queries (decode attention reads either);
         // otherwise decode attention may finish the raw q/k/v rows itself
         const float *raw = !fused_qkv && own_prep ? m->qkv : nullptr;
-        if ((rc = run_attention(m, st, T, decode, seq_ids, pos, Sc, Lc, p0, l, fused_qkv, raw, 0)))
+        if ((rc = run_attention(m, st, T, decode, seq_ids, pos, Sc, Lc, p0, l, fused_qkv, raw, 0, !fused_qkv)))
             return rc;
         // o and down: the residual rows x were last written two or more kernels
         // back (the embedding or the previous residual GEMM), never by the
@@ -1692,9 +1707,9 @@ int n550_qkv_rope_kv(void *stream, const uint16_t *x, int ldx, const uint16_t *w
     else
         rc = launch_gemm_simt(st, TC_EPI_F32, x, ldx, wqkv, H, ws, QKVD, M, QKVD, H);
     if (!rc) {
-        if (launch_k(qknorm_rope_kv_kernel, M, 1024, 0, st, (const float *)ws, QKVD, ks,
+        if (launch_k(qknorm_rope_kv_kernel<false>, M, 1024, 0, st, (const float *)ws, QKVD, ks,
                      (size_t)M * QKVD, q_norm, k_norm, rope, tok_pos, tok_seq, layer, k_cache, v_cache,
-                     max_len, qb, qf, ldq, (uint16_t *)nullptr) != cudaSuccess)
+                     max_len, qb, qf, ldq, (uint16_t *)nullptr, Kv8View{}) != cudaSuccess)
             rc = N550_ERR_CUDA;
         (void)cudaGetLastError();
     }

@@ -56,20 +56,45 @@ def layer0_kv(m, tokens):
     return n5.rope(k.contiguous(), 8, 0).view(-1, 8, 128), v.view(-1, 8, 128)
 
 
-@pytest.mark.parametrize("n", [1, 3, 40, 290])
-def test_cache_holds_the_layers_rows(model, n):
+def check_layer0(m, tokens, slot):
     """Codes times scales of layer 0 against the rows: half an e4m3 step (2^-4 of the
     value, 2^-10 of the scale below 2^-6) and the BF16 rounding before it (2^-8),
     with 2^-12 of slack for sums in another order."""
-    t = toks(n, 5)
-    model.prefill(t.view(1, n), i32([7]), 0, next_token=i32([0]))
-    c = model.kv8_cache()
+    c = m.kv8_cache()
+    n = len(tokens)
     b = torch.arange(n, device="cuda") // BLOCK
-    for rows, codes, scale in zip(layer0_kv(model, t), (c.k, c.v), (c.k_scale, c.v_scale)):
-        s = scale[7, 0][:, b, None]
-        got = (codes[7, 0, :, :n].float() * s).transpose(0, 1)
+    for rows, codes, scale in zip(layer0_kv(m, tokens), (c.k, c.v), (c.k_scale, c.v_scale)):
+        s = scale[slot, 0][:, b, None]
+        got = (codes[slot, 0, :, :n].float() * s).transpose(0, 1)
         tol = rows.abs() * (2.0 ** -4 + 2.0 ** -8 + 2.0 ** -12) + s.transpose(0, 1) * 2.0 ** -10 + 1e-6
         assert ((got - rows).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("n", [1, 3, 40, 290])
+def test_cache_holds_the_layers_rows(model, n):
+    t = toks(n, 5)
+    model.prefill(t.view(1, n), i32([7]), 0, next_token=i32([0]))
+    check_layer0(model, t, 7)
+
+
+@pytest.mark.parametrize("n_seqs,L", [(4, 260), (5, 259), (9, 3), (64, 1)])
+def test_cache_of_a_batch(cuda, n_seqs, L):
+    """Rows written by the epilogues of the tile GEMM (from 1024 rows) and of the
+    weight-streaming one, in slots out of order; the other slots stay empty."""
+    m = n5.Model(seed=0, max_seqs=66, max_len=270, max_tokens=1300, kv8=True)
+    try:
+        t = toks(n_seqs * L, 7).view(n_seqs, L)
+        ids = torch.randperm(66, generator=torch.Generator().manual_seed(L))[:n_seqs].to(torch.int32)
+        m.prefill(t, ids.cuda(), 0, next_token=torch.empty(n_seqs, dtype=torch.int32, device="cuda"))
+        for s in range(n_seqs):
+            check_layer0(m, t[s], int(ids[s]))
+        rest = torch.ones(66, dtype=torch.bool)
+        rest[ids.long()] = False
+        c = m.kv8_cache()
+        assert not c.k.view(torch.uint8)[rest.cuda()].any() and not c.v.view(torch.uint8)[rest.cuda()].any()
+        assert n5.device_status() == n5.OK
+    finally:
+        m.close()
 
 
 @pytest.mark.parametrize("n_seqs", [1, 4, 6, 20, 36])
@@ -86,6 +111,43 @@ def test_decode_agrees_with_prefill(model, n_seqs):
     torch.cuda.synchronize()
     assert n5.device_status() == n5.OK
     assert rel(got, want) <= TOL
+
+
+@pytest.mark.parametrize("n_seqs", [1, 8, 70])
+def test_appending_in_the_row_kernel_is_bit_identical(cuda, n_seqs):
+    """Decode steps over several blocks from ragged positions (one of them 0, one the
+    cache's last): ids, codes, scales and bounds of both ways of appending."""
+    steps, max_len = 70, 260
+    start = [(s * 37) % 150 for s in range(n_seqs)]
+    t = toks(n_seqs * 150, 61).view(n_seqs, 150)
+    got = []
+    m = n5.Model(seed=0, max_seqs=n_seqs, max_len=max_len, max_tokens=256, kv8=True)
+    try:
+        for fused in (1, 0):
+            n5.check(n5.lib().n550_qwen3_fused_attention_prep(fused))
+            c = m.kv8_cache()
+            for x in (c.k, c.v, c.k_bounds):
+                x.view(torch.uint8).zero_()
+            for s in range(n_seqs):
+                if start[s]:
+                    m.prefill(t[s:s + 1, :start[s]].contiguous(), i32([s]), 0, next_token=i32([0]))
+            tok, out = t[:, 149].clone(), torch.empty((steps, n_seqs), dtype=torch.int32, device="cuda")
+            m.decode_steps(tok, torch.arange(n_seqs, dtype=torch.int32, device="cuda"), i32(start), steps, out, use_graph=False)
+            last = i32([max_len - 1])                           # (a context with holes: only its row matters)
+            m.decode(t[0, :1].contiguous(), i32([n_seqs - 1]), last, next_token=i32([0]))
+            torch.cuda.synchronize()
+            end = [p + steps for p in start]
+            nb = [-(-e // BLOCK) for e in end]
+            got.append([out.clone()] + [x[s, :, :, :end[s]].view(torch.uint8).clone() for x in (c.k, c.v) for s in range(n_seqs)] +
+                       [x[s, :, :, :nb[s]].clone() for x in (c.k_scale, c.v_scale, c.k_bounds.view(torch.uint8))
+                        for s in range(n_seqs)] +
+                       [x[n_seqs - 1, 0, :, max_len - 1].view(torch.uint8).clone() for x in (c.k, c.v)])
+    finally:
+        n5.lib().n550_qwen3_fused_attention_prep(1)
+        m.close()
+    assert n5.device_status() == n5.OK
+    for x, y in zip(*got):
+        assert torch.equal(x, y)
 
 
 def test_chunked_prefill_and_rows(model):
