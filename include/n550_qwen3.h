@@ -444,8 +444,8 @@ int n550_qwen3_split_rows(int rows);
 /* Decode steps that take the split-K or GEMV q/k/v route: the decode attention
  * kernel applies QK-norm and RoPE to the raw q/k/v rows and writes the new K/V
  * itself (1, default) or a separate row kernel does (0). Over the 8-bit cache the
- * row kernel also appends (1) or leaves that to n550_kv8_append's kernel (0).
- * Bit-identical results either way. */
+ * kernel that finishes those rows also appends (1) or leaves that to
+ * n550_kv8_append's kernel (0). Bit-identical results either way. */
 int n550_qwen3_fused_attention_prep(int on);
 
 /* Decode steps of 1-4 sequences as one persistent kernel (1) or as the
@@ -460,8 +460,8 @@ int n550_qwen3_fused_decode(int on);
  * the bytes a decode step reads) instead of BF16 (on = 1), or goes back (0, the
  * default). Either way the cache starts empty: call it before the first prefill.
  * Synchronises and allocates; the other cache's memory is freed. The q/k/v step
- * then leaves BF16 K/V rows (after QK-norm and RoPE, in the GEMM's epilogue where the
- * batch has one) for n550_kv8_append, and the attention runs as
+ * then appends its K/V rows (after QK-norm and RoPE) itself in a decode step and leaves
+ * them to n550_kv8_append otherwise, and the attention runs as
  * n550_attention_decode_kv8 / n550_attention_prefill_kv8. Fast mode only
  * (N550_ERR_UNSUPPORTED otherwise, and for a forward with the tensor dump on).
  * n550_qwen3_kv8_cache gives the cache of such a model (28 layers, max_seqs slots)

@@ -30,6 +30,7 @@
 #include "common.cuh"
 #include "gemm_skinny.h"
 #include "gemm_tc.h"
+#include "kv8_quant.cuh"
 #include "launch.h"
 #include "tmap.h"
 
@@ -185,7 +186,7 @@ gemm_skinny_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constan
                 xv[j] = (c_beg + j < c_end && t < p.T && n < p.N) ? p.ep.out[(size_t)t * p.ep.ldo + n] : 0.f;
             }
         }
-        if (EPI == SK_EPI_QKV) {
+        if (EPI == SK_EPI_QKV || EPI == SK_EPI_QKV_KV8) {
             // positions and slots of the owned tokens, then their RoPE rows
             // (64 (cos, sin) pairs = 512 B each) into shared memory
             const int i = threadIdx.x - 64;
@@ -356,7 +357,13 @@ gemm_skinny_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constan
                     }
                 } else {
                     const int kvh = (hd - 16) & 7;
-                    uint16_t *dst = ep.kv_rows
+                    if (EPI == SK_EPI_QKV_KV8 && ep.kv8.k) {      // the rounding of the rows that append reads
+#pragma unroll
+                        for (int j = 0; j < 4; j++) v[j] = bf16_bits_to_f32(f32_to_bf16_rne(v[j]));
+                        kv8_put_row(ep.kv8, seq, kvh, hd >= 24, pos, v, lane);
+                        continue;
+                    }
+                    uint16_t *dst = EPI == SK_EPI_QKV_KV8
                                         ? ep.kv_rows + (size_t)t * 2 * N_KV_HEADS * HEAD + (hd - 16) * HEAD
                                         : (hd < 24 ? ep.kc : ep.vc) +
                                               (((size_t)(seq * N_LAYERS + ep.layer) * N_KV_HEADS + kvh) *
@@ -388,7 +395,7 @@ SkLayout sk_layout(int tn, int stages, int cs, int epi) {
     l.stage_region = std::max(stages * stage, tn * 128 * 4);
     l.recv_off = l.stage_region;
     l.aux_off = l.recv_off + (cs > 1 ? cs * tno * 128 * 4 : 0);
-    const int aux = epi == SK_EPI_QKV ? ((tno * 8 + 15) & ~15) + tno * 64 * 8 : 0;
+    const int aux = epi == SK_EPI_QKV || epi == SK_EPI_QKV_KV8 ? ((tno * 8 + 15) & ~15) + tno * 64 * 8 : 0;
     l.bar_off = (l.aux_off + aux + 15) & ~15;
     l.smem = 1024 + l.bar_off + SK_BAR_BYTES;
     return l;
@@ -469,20 +476,23 @@ int sk_dispatch(cudaStream_t st, int epi, const CUtensorMap &tw, const CUtensorM
     case SK_EPI_RESID: return sk_launch<TN, SK_EPI_RESID>(st, tw, tw2, tx, p, ctas, cs, smem);
     case SK_EPI_SILU: return sk_launch<TN, SK_EPI_SILU>(st, tw, tw2, tx, p, ctas, cs, smem);
     case SK_EPI_QKV: return sk_launch<TN, SK_EPI_QKV>(st, tw, tw2, tx, p, ctas, cs, smem);
+    case SK_EPI_QKV_KV8: return sk_launch<TN, SK_EPI_QKV_KV8>(st, tw, tw2, tx, p, ctas, cs, smem);
     default: return N550_ERR_ARG;
     }
 }
 
 bool sk_fits(int tn, int epi, int cs, int smem) {
-    switch (tn * 4 + epi) {
-    case 32 * 4 + SK_EPI_F32: return sk_cluster_fits<32, SK_EPI_F32>(cs, smem);
-    case 32 * 4 + SK_EPI_RESID: return sk_cluster_fits<32, SK_EPI_RESID>(cs, smem);
-    case 32 * 4 + SK_EPI_SILU: return sk_cluster_fits<32, SK_EPI_SILU>(cs, smem);
-    case 32 * 4 + SK_EPI_QKV: return sk_cluster_fits<32, SK_EPI_QKV>(cs, smem);
-    case 64 * 4 + SK_EPI_F32: return sk_cluster_fits<64, SK_EPI_F32>(cs, smem);
-    case 64 * 4 + SK_EPI_RESID: return sk_cluster_fits<64, SK_EPI_RESID>(cs, smem);
-    case 64 * 4 + SK_EPI_SILU: return sk_cluster_fits<64, SK_EPI_SILU>(cs, smem);
-    case 64 * 4 + SK_EPI_QKV: return sk_cluster_fits<64, SK_EPI_QKV>(cs, smem);
+    switch (tn * 8 + epi) {
+    case 32 * 8 + SK_EPI_F32: return sk_cluster_fits<32, SK_EPI_F32>(cs, smem);
+    case 32 * 8 + SK_EPI_RESID: return sk_cluster_fits<32, SK_EPI_RESID>(cs, smem);
+    case 32 * 8 + SK_EPI_SILU: return sk_cluster_fits<32, SK_EPI_SILU>(cs, smem);
+    case 32 * 8 + SK_EPI_QKV: return sk_cluster_fits<32, SK_EPI_QKV>(cs, smem);
+    case 32 * 8 + SK_EPI_QKV_KV8: return sk_cluster_fits<32, SK_EPI_QKV_KV8>(cs, smem);
+    case 64 * 8 + SK_EPI_F32: return sk_cluster_fits<64, SK_EPI_F32>(cs, smem);
+    case 64 * 8 + SK_EPI_RESID: return sk_cluster_fits<64, SK_EPI_RESID>(cs, smem);
+    case 64 * 8 + SK_EPI_SILU: return sk_cluster_fits<64, SK_EPI_SILU>(cs, smem);
+    case 64 * 8 + SK_EPI_QKV: return sk_cluster_fits<64, SK_EPI_QKV>(cs, smem);
+    case 64 * 8 + SK_EPI_QKV_KV8: return sk_cluster_fits<64, SK_EPI_QKV_KV8>(cs, smem);
     default: return false;
     }
 }
@@ -529,13 +539,16 @@ int g_skinny_rows_gemm = SK_AUTO_GEMM_T;
 int launch_gemm_skinny(cudaStream_t st, int epi, const uint16_t *x, int ldx, const uint16_t *w,
                        const uint16_t *w2, int ldw, int T, int N, int K, const SkEpilogue &ep, int cs) {
     if (T <= 0 || N <= 0) return N550_OK;
-    if (T > SK_MAX_T || K <= 0 || epi < SK_EPI_F32 || epi > SK_EPI_QKV) return N550_ERR_ARG;
+    if (T > SK_MAX_T || K <= 0 || epi < SK_EPI_F32 || epi > SK_EPI_QKV_KV8) return N550_ERR_ARG;
     if (!tc_shape_ok(x, ldx, w, ldw, K)) return N550_ERR_UNSUPPORTED;
     const bool silu = epi == SK_EPI_SILU;
     if (silu && (!w2 || (((uintptr_t)w2) & 15) || !ep.h)) return N550_ERR_ARG;
     if ((epi == SK_EPI_F32 || epi == SK_EPI_RESID) && !ep.out) return N550_ERR_ARG;
-    if (epi == SK_EPI_QKV && (N != 32 * HEAD || (!ep.kv_rows && (!ep.kc || !ep.vc)) || !ep.tok_pos || !ep.tok_seq ||
-                              !ep.rope || !ep.q_norm || !ep.k_norm || (!ep.q_f32 && !ep.q_bf16)))
+    if ((epi == SK_EPI_QKV && (!ep.kc || !ep.vc)) || (epi == SK_EPI_QKV_KV8 && !ep.kv8.k && !ep.kv_rows))
+        return N550_ERR_ARG;
+    if ((epi == SK_EPI_QKV || epi == SK_EPI_QKV_KV8) &&
+        (N != 32 * HEAD || !ep.tok_pos || !ep.tok_seq || !ep.rope || !ep.q_norm || !ep.k_norm ||
+         (!ep.q_f32 && !ep.q_bf16)))
         return N550_ERR_ARG;
     const int tn = T <= 32 ? 32 : 64;
     const int n_tt = (T + tn - 1) / tn;

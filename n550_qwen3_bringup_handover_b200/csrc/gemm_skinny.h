@@ -4,6 +4,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include "kv8.h"
+
 namespace n550 {
 
 // Epilogues of the skinny GEMM (Y = X[T,K] . W[N,K]^T, T <= 128 tokens).
@@ -11,7 +13,8 @@ enum {
     SK_EPI_F32 = 0,     // out[t][n] = y                      (FP32)
     SK_EPI_RESID = 1,   // out[t][n] += y                     (residual add, qwen3.c:523/543)
     SK_EPI_SILU = 2,    // h[t][n] = silu(y_gate) * y_up      (BF16, W = gate rows, W2 = up rows)
-    SK_EPI_QKV = 3      // per-head QK-norm + RoPE, q out, K/V into the cache (qwen3.c:477-511)
+    SK_EPI_QKV = 3,     // per-head QK-norm + RoPE, q out, K/V into the cache (qwen3.c:477-511)
+    SK_EPI_QKV_KV8 = 4  // the same, K/V into the 8-bit cache or as rows for its append
 };
 
 struct SkEpilogue {
@@ -24,11 +27,14 @@ struct SkEpilogue {
     uint16_t *q_bf16;           // [T][ldq] BF16 queries
     int ldq;
     uint16_t *kc, *vc;          // KV cache [seq][layer][kv_head][pos][128]
-    uint16_t *kv_rows;          // instead of the caches: K and V heads as rows [T][2048] (or NULL)
     int layer, max_len;
     const int32_t *tok_pos, *tok_seq;   // per token
     const uint16_t *q_norm, *k_norm;    // BF16 [128]
     const float2 *rope;         // [max_len][64] (cos, sin)
+    // QKV_KV8, instead of kc and vc: the 8-bit cache when every token is a sequence's
+    // only one (kv8.k set), or K and V heads as rows [T][2048]
+    Kv8View kv8;
+    uint16_t *kv_rows;
 };
 
 // n550_gemm_skinny_config: 0 = automatic (the skinny GEMM for M <=

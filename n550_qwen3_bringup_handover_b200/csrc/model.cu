@@ -804,7 +804,7 @@ int launch_final_norm(cudaStream_t st, uint16_t *xl, const float *x, const uint1
     } while (0)
 
 // The same over the 8-bit cache: the layer's K/V rows (m->kv_rows) are appended (unless
-// launch_qknorm_rope_kv did that) and the queries (m->qb) attend to the codes. A prefill of many queries works
+// the kernel before did that) and the queries (m->qb) attend to the codes. A prefill of many queries works
 // through its sequences in groups whose contexts fit m->kv8_out as BF16.
 int run_attention_kv8(n550_model *m, cudaStream_t st, bool decode, const int32_t *seq_ids,
                       const int32_t *pos, int Sc, int Lc, int p0, int l, bool appended) {
@@ -848,11 +848,11 @@ int run_attention_kv8(n550_model *m, cudaStream_t st, bool decode, const int32_t
 
 int run_attention(n550_model *m, cudaStream_t st, int T, bool decode, const int32_t *seq_ids,
                   const int32_t *pos, int Sc, int Lc, int p0, int l, bool q_in_bf16 = false,
-                  const float *raw_qkv = nullptr, int ks = 0, bool row_kernel = false) {
+                  const float *raw_qkv = nullptr, int ks = 0, bool appended = false) {
     const n550_model_config &c = m->cfg;
     int rc = N550_OK;
     if (m->kv8.k)
-        return run_attention_kv8(m, st, decode, seq_ids, pos, Sc, Lc, p0, l, row_kernel && decode && g_fused_prep);
+        return run_attention_kv8(m, st, decode, seq_ids, pos, Sc, Lc, p0, l, appended);
     if (decode) {
         AttnDecodeArgs a{};
         a.q_f32 = q_in_bf16 ? nullptr : m->qf;
@@ -897,7 +897,8 @@ int run_layers_split(n550_model *m, cudaStream_t st, int T, bool decode, const i
             if ((rc = run_attention(m, st, T, decode, seq_ids, pos, Sc, Lc, p0, l, false, m->ws, ks))) return rc;
         } else {
             STEP(N550_PROF_QKNORM_ROPE, 1, launch_qknorm_rope_kv(m, st, T, l, decode, m->ws, ks));
-            if ((rc = run_attention(m, st, T, decode, seq_ids, pos, Sc, Lc, p0, l, false, nullptr, 0, true))) return rc;
+            if ((rc = run_attention(m, st, T, decode, seq_ids, pos, Sc, Lc, p0, l, false, nullptr, 0, decode && g_fused_prep)))
+                return rc;
         }
         STEP(N550_PROF_GEMM_O, 1, partials(m, st, m->attn, QD, W(m, l, 6), T, H, QD, &ks));
         STEP(N550_PROF_RMSNORM, 1, launch_resid_norm(st, m->x, m->ws, ks, T, W(m, l, 7), m->xb));
@@ -938,9 +939,11 @@ int run_layers_skinny(n550_model *m, cudaStream_t st, int T, bool decode, const 
         q.tok_pos = m->tok_pos; q.tok_seq = m->tok_seq;
         q.q_norm = W(m, l, 4); q.k_norm = W(m, l, 5);
         q.rope = m->rope;
+        const bool put8 = m->kv8.k && decode && g_fused_prep;
+        if (put8 && (rc = kv8_view(&m->kv8, l, &q.kv8))) return rc;
         STEP(N550_PROF_GEMM_QKV, 1,
-             launch_gemm_skinny(st, SK_EPI_QKV, m->xb, H, m->wqkv[l], nullptr, H, T, QKVD, H, q));
-        if ((rc = run_attention(m, st, T, decode, seq_ids, pos, Sc, Lc, p0, l))) return rc;
+             launch_gemm_skinny(st, m->kv8.k ? SK_EPI_QKV_KV8 : SK_EPI_QKV, m->xb, H, m->wqkv[l], nullptr, H, T, QKVD, H, q));
+        if ((rc = run_attention(m, st, T, decode, seq_ids, pos, Sc, Lc, p0, l, false, nullptr, 0, put8))) return rc;
         STEP(N550_PROF_GEMM_O, 1,
              launch_gemm_skinny(st, SK_EPI_RESID, m->attn, QD, W(m, l, 6), nullptr, QD, T, H, QD, resid));
         STEP(N550_PROF_RMSNORM, 1, launch_norm_rows(st, m->xb, m->x, W(m, l, 7), T));
@@ -1019,7 +1022,7 @@ int run_layers(n550_model *m, cudaStream_t st, int T, bool decode, const int32_t
         // the fused QKV epilogue leaves BF16 queries (decode attention reads either);
         // otherwise decode attention may finish the raw q/k/v rows itself
         const float *raw = !fused_qkv && own_prep ? m->qkv : nullptr;
-        if ((rc = run_attention(m, st, T, decode, seq_ids, pos, Sc, Lc, p0, l, fused_qkv, raw, 0, !fused_qkv)))
+        if ((rc = run_attention(m, st, T, decode, seq_ids, pos, Sc, Lc, p0, l, fused_qkv, raw, 0, !fused_qkv && decode && g_fused_prep)))
             return rc;
         // o and down: the residual rows x were last written two or more kernels
         // back (the embedding or the previous residual GEMM), never by the

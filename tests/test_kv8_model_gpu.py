@@ -113,8 +113,8 @@ def test_decode_agrees_with_prefill(model, n_seqs):
     assert rel(got, want) <= TOL
 
 
-@pytest.mark.parametrize("n_seqs", [1, 8, 70])
-def test_appending_in_the_row_kernel_is_bit_identical(cuda, n_seqs):
+@pytest.mark.parametrize("n_seqs", [1, 8, 20, 70])
+def test_appending_in_the_kernel_before_is_bit_identical(cuda, n_seqs):
     """Decode steps over several blocks from ragged positions (one of them 0, one the
     cache's last): ids, codes, scales and bounds of both ways of appending."""
     steps, max_len = 70, 260
