@@ -459,7 +459,10 @@ int n550_qwen3_fused_decode(int on);
 /* Holds the model's KV cache as the 8-bit cache (n550_kv8_cache: e4m3 codes, half
  * the bytes a decode step reads) instead of BF16 (on = 1), or goes back (0, the
  * default). Either way the cache starts empty: call it before the first prefill.
- * Synchronises and allocates; the other cache's memory is freed. The q/k/v step
+ * Synchronises and allocates; the other cache's memory is freed first, and so are
+ * the pointers of an n550_qwen3_kv8_cache. N550_ERR_OOM: the new cache does not fit,
+ * the BF16 one is (again) the model's; if that does not fit either, the forwards
+ * return N550_ERR_OOM until a call of this function succeeds. The q/k/v step
  * then appends its K/V rows (after QK-norm and RoPE) itself in a decode step and leaves
  * them to n550_kv8_append otherwise, and the attention runs as
  * n550_attention_decode_kv8 / n550_attention_prefill_kv8. Fast mode only

@@ -1250,6 +1250,10 @@ int n550_qwen3_init_random(n550_model_t **out, uint64_t seed, double sigma,
     return N550_OK;
 }
 
+// Neither cache: n550_qwen3_use_kv8 could not allocate the one it was to change to, nor
+// the one it had. The forwards refuse until a call of it succeeds.
+static bool no_cache(const n550_model_t *m) { return !m->kv8.k && !(m->kc && m->vc); }
+
 // The captured decode step and prefill hold the cache's pointers.
 static void drop_graphs(n550_model_t *m) {
     if (m->graph) { cudaGraphExecDestroy(m->graph); m->graph = nullptr; }
@@ -1261,7 +1265,7 @@ int n550_qwen3_use_kv8(n550_model_t *m, int on) {
     if (!m) return N550_ERR_ARG;
     const n550_model_config &c = m->cfg;
     if (c.gemm_mode != N550_MODE_FAST) return N550_ERR_UNSUPPORTED;
-    if ((on != 0) == (m->kv8.k != nullptr)) return N550_OK;
+    if (on ? m->kv8.k != nullptr : m->kc != nullptr) return N550_OK;
     N550_CUDA_TRY(cudaDeviceSynchronize());
     drop_graphs(m);
     const size_t planes = (size_t)c.max_seqs * NLAYER * NKVH, codes = planes * (size_t)c.max_len * HDIM;
@@ -1342,6 +1346,7 @@ static int prefill_eager(n550_model_t *m, cudaStream_t st, const int32_t *tokens
 int n550_qwen3_prefill(n550_model_t *m, void *stream, const int32_t *tokens, const int32_t *seq_ids,
                        int n_seqs, int seq_len, int pos0, float *logits, int32_t *next_token) {
     if (!m || !tokens || !seq_ids || n_seqs < 1 || seq_len < 1 || pos0 < 0) return N550_ERR_ARG;
+    if (no_cache(m)) return N550_ERR_OOM;
     const n550_model_config &c = m->cfg;
     if (pos0 + seq_len > c.max_len) return N550_ERR_ARG;
     cudaStream_t st = (cudaStream_t)stream;
@@ -1422,6 +1427,7 @@ static int prefill_eager(n550_model_t *m, cudaStream_t st, const int32_t *tokens
 int n550_qwen3_decode(n550_model_t *m, void *stream, const int32_t *tokens, const int32_t *seq_ids,
                       const int32_t *pos, int n_seqs, float *logits, int32_t *next_token) {
     if (!m || !tokens || !seq_ids || !pos || n_seqs < 1) return N550_ERR_ARG;
+    if (no_cache(m)) return N550_ERR_OOM;
     const n550_model_config &c = m->cfg;
     if (n_seqs > c.max_tokens || n_seqs > c.max_seqs) return N550_ERR_ARG;
     cudaStream_t st = (cudaStream_t)stream;
@@ -1440,6 +1446,7 @@ int n550_qwen3_decode(n550_model_t *m, void *stream, const int32_t *tokens, cons
 int n550_qwen3_decode_steps(n550_model_t *m, void *stream, int32_t *tokens, const int32_t *seq_ids,
                             int32_t *pos, int n_seqs, int steps, int32_t *out_ids, int use_graph) {
     if (!m || !tokens || !seq_ids || !pos || !out_ids || n_seqs < 1 || steps < 0) return N550_ERR_ARG;
+    if (no_cache(m)) return N550_ERR_OOM;
     if (n_seqs > m->cfg.max_tokens || n_seqs > m->cfg.max_seqs) return N550_ERR_ARG;
     cudaStream_t st = (cudaStream_t)stream;
     N550_CUDA_TRY(cudaMemsetAsync(m->step_counter, 0, 4, st));   // ordered before the capture stream joins
@@ -1539,6 +1546,7 @@ int n550_qwen3_forward_rows(n550_model_t *m, void *stream, const int32_t *tokens
     if (!m || !tokens || !seq_id || n_token < 1 || n_token > N550_ROWS_MAX || pos0 < 0 ||
         (!logits && !next_ids))
         return N550_ERR_ARG;
+    if (no_cache(m)) return N550_ERR_OOM;
     const n550_model_config &c = m->cfg;
     if (pos0 + n_token > c.max_len || n_token > c.max_tokens) return N550_ERR_ARG;
     cudaStream_t st = (cudaStream_t)stream;
@@ -1586,6 +1594,7 @@ int n550_qwen3_set_dump(n550_model_t *m, n550_dump_fn fn, void *ctx) {
 int n550_qwen3_forward_batch_host(n550_model_t *m, const int32_t *tokens, int n_token, int pos0,
                                   float *logits_host) {
     if (!m || !tokens || n_token < 1) return N550_ERR_ARG;
+    if (no_cache(m)) return N550_ERR_OOM;
     if (n_token > m->cfg.max_tokens) return N550_ERR_ARG;
     cudaStream_t st = 0;
     N550_CUDA_TRY(cudaMemcpyAsync(m->host_tok, tokens, (size_t)n_token * 4, cudaMemcpyHostToDevice, st));

@@ -220,3 +220,40 @@ def test_graph_replay_switching_back_and_refusals(cuda):
             e.use_kv8()
     finally:
         e.close()
+
+
+def test_no_room_for_the_cache_to_go_back_to(cuda):
+    """The BF16 cache (twice the 8-bit one) does not fit any more: N550_ERR_OOM from there
+    on, not a launch over memory that is gone, and a second try that has room works."""
+    m = n5.Model(seed=0, max_seqs=1, max_len=32768, max_tokens=64, kv8=True)       # BF16 3.8 GB, 8-bit 1.9 GB
+    hold = None
+    try:
+        t, ids, nx = toks(20, 71), i32([0]), i32([0])
+        want, got = logits(1), logits(1)
+        m.use_kv8(False)
+        m.prefill(t.view(1, 20), ids, 0, want, nx)
+        m.use_kv8()
+        torch.cuda.synchronize()
+        torch.cuda.empty_cache()
+        free = torch.cuda.mem_get_info()[0]
+        hold = torch.empty(free - (512 << 20), dtype=torch.uint8, device="cuda")
+        calls = [lambda: m.use_kv8(False), lambda: m.prefill(t.view(1, 20), ids, 0, got, nx),
+                 lambda: m.decode(nx, ids, i32([20]), got), lambda: m.forward_batch(np.arange(4, dtype=np.int32), 0),
+                 lambda: m.forward_rows(np.arange(4, dtype=np.int32), 0),
+                 lambda: m.decode_steps(nx, ids, i32([20]), 2, torch.empty((2, 1), dtype=torch.int32, device="cuda"))]
+        for call in calls:
+            with pytest.raises(n5.N550Error) as e:
+                call()
+            assert e.value.status == n5.ERR_OOM
+        with pytest.raises(n5.N550Error):
+            m.kv8_cache()
+        hold = None
+        torch.cuda.empty_cache()
+        m.use_kv8(False)
+        m.prefill(t.view(1, 20), ids, 0, got, nx)
+        torch.cuda.synchronize()
+        assert torch.equal(got, want)
+    finally:
+        hold = None
+        m.close()
+        torch.cuda.empty_cache()
