@@ -876,7 +876,7 @@ constexpr int kSms = 148;
 template <int LT>
 int ctas() { return kSms * per_sm<LT>(); }
 static_assert(3 * (smem_bytes<1>(1) + 2048) <= 233472 && 2 * (smem_bytes<4>(4) + 2560) <= 233472 &&
-                  smem_bytes<8>(8) + 3072 <= 233472,
+                  smem_bytes<8>(8) + 3 * 1024 <= 233472,
               "shared memory of an SM: 228 KB, 1 KB a CTA reserved, the rest of the sum static");
 static_assert(3 * tmem_cols<1>() <= 512 && 2 * tmem_cols<4>() <= 512 && tmem_cols<8>() <= 512, "TMEM of an SM");
 int max_ctas(int L) { return L == 1 ? ctas<1>() : L <= 4 ? ctas<4>() : ctas<8>(); }
