@@ -73,11 +73,12 @@ class KV8Cache:
 
 def _ids(seq_ids, pos=None):
     """Number of sequences; both must be contiguous int32 vectors of that length."""
-    from torch import int32
-    n, = shape = seq_ids.shape if seq_ids.dim() == 1 else (-1,)
-    if n < 0 or seq_ids.dtype != int32 or not seq_ids.is_contiguous():
+    import torch
+    i32 = torch.int32
+    if seq_ids.dim() != 1 or seq_ids.dtype != i32 or not seq_ids.is_contiguous():
         raise ValueError("seq_ids must be a contiguous int32 vector")
-    if pos is not None and (pos.shape != shape or pos.dtype != int32 or not pos.is_contiguous()):
+    n = seq_ids.numel()
+    if pos is not None and (pos.dim() != 1 or pos.numel() != n or pos.dtype != i32 or not pos.is_contiguous()):
         raise ValueError(f"pos must be a contiguous int32 vector of {n}")
     return n
 
@@ -111,7 +112,9 @@ def _q_out(q, rows, out):
     import torch
     ldq = _rows("q", q, rows, _NH * _HD, (torch.bfloat16,))
     if out is None:
-        return ldq, q.new_empty((rows, _NH * _HD)), _NH * _HD
+        w = _NH * _HD
+        # (the cheaper call where q is such a matrix itself)
+        return ldq, torch.empty_like(q) if ldq == w == q.shape[1] else q.new_empty((rows, w)), w
     return ldq, out, _rows("out", out, rows, _NH * _HD, (torch.bfloat16,))
 
 
@@ -141,7 +144,8 @@ def attention_sparse_kv8(q, cache, seq_ids, pos, blocks, layer, out=None, split=
     blocks int32 [n_seqs, 8, n_select], entries outside the context skipped."""
     import torch
     n = _ids(seq_ids, pos)
-    if blocks.dtype != torch.int32 or blocks.dim() != 3 or tuple(blocks.shape[:2]) != (n, _NKV) or \
+    shape = blocks.shape
+    if blocks.dtype != torch.int32 or len(shape) != 3 or shape[0] != n or shape[1] != _NKV or \
             not blocks.is_contiguous():
         raise ValueError(f"blocks must be a contiguous int32 tensor [{n}, 8, n_select]")
     ldq, out, ldo = _q_out(q, n, out)
@@ -150,7 +154,7 @@ def attention_sparse_kv8(q, cache, seq_ids, pos, blocks, layer, out=None, split=
     nbytes = L.n550_attention_kv8_workspace(n) if split else 0
     ws = _workspace(nbytes, q) if nbytes else None
     check(L.n550_attention_sparse_kv8(st, q.data_ptr(), ldq, cache._ref, layer, seq_ids.data_ptr(),
-                                      pos.data_ptr(), blocks.data_ptr(), blocks.shape[2], n,
+                                      pos.data_ptr(), blocks.data_ptr(), shape[2], n,
                                       out.data_ptr(), ldo, ws.data_ptr() if nbytes else None, nbytes), "n550_attention_sparse_kv8")
     return out
 
