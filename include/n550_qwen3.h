@@ -374,6 +374,15 @@ int n550_device_status(void);
  * the reference. */
 int n550_check_wait_expiry(void *stream, long long cycles);
 
+/* Health check of the failure path of n550_attention_decode_kv8: merges the partials
+ * of a split call alone, over whatever `workspace` (n550_attention_kv8_workspace
+ * bytes, required) holds, as after an attention kernel whose waits expired before it
+ * had written its records. Records {sequence, KV head, pieces, slot} (int32, one
+ * per run) that name no pair or pieces of a call with n_seqs sequences are skipped:
+ * out [n_seqs][ldo >= 2048] keeps those rows, and nothing else is written. */
+int n550_check_kv8_merge(void *stream, int n_seqs, void *workspace, size_t workspace_bytes, uint16_t *out,
+                         int ldo);
+
 /* ===========================================================================
  * 3. Model runtime (qwen3.h:203-257 re-designed for HBM): weights, KV cache
  *    and activations live on one GPU; many independent sequences share it.

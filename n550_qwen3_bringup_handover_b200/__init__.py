@@ -102,6 +102,7 @@ def lib() -> C.CDLL:
         "n550_kv8_append": (i, [vp, vp, i, vp, vp, i, i, vp, vp, i, i]),
         "n550_attention_decode_kv8": (i, [vp, vp, i, vp, i, vp, vp, i, vp, i, vp, sz]),
         "n550_attention_kv8_workspace": (sz, [i]),
+        "n550_check_kv8_merge": (i, [vp, i, vp, sz, vp, i]),
         "n550_attention_prefill_kv8": (i, [vp, vp, i, vp, i, vp, i, i, i, vp, i, vp, sz]),
         "n550_attention_prefill_kv8_workspace": (sz, [i, i, i]),
         "n550_kv8_select_blocks": (i, [vp, vp, i, vp, i, vp, vp, i, i, i, i, vp]),

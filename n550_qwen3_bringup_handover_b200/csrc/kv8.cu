@@ -91,6 +91,15 @@ int n550_attention_sparse_kv8(void *stream, const uint16_t *q, int ldq, const n5
     return launch_kv8_attn((cudaStream_t)stream, a);
 }
 
+int n550_check_kv8_merge(void *stream, int n_seqs, void *workspace, size_t workspace_bytes, uint16_t *out,
+                         int ldo) {
+    if (n_seqs < 1 || n_seqs > kMaxSeqs || !rows_ok(out, ldo, 2)) return N550_ERR_ARG;
+    Kv8AttnArgs a{};
+    a.out = out; a.ldo = ldo; a.L = a.rows = 1; a.n_seqs = n_seqs;
+    a.part = split_ws(workspace, workspace_bytes, kv8_attn_workspace(n_seqs, 1));
+    return a.part ? launch_kv8_merge((cudaStream_t)stream, a) : N550_ERR_ARG;
+}
+
 size_t n550_attention_prefill_kv8_workspace(int n_seqs, int L, int pos0) {
     if (n_seqs <= 0 || L <= 0 || pos0 < 0) return 0;
     return kv8_in_passes(n_seqs, L, pos0) ? kv8_attn_workspace(n_seqs, L < KV8_FEW ? L : KV8_FEW)

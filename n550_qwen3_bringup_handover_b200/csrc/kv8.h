@@ -98,6 +98,8 @@ int launch_kv8_passes(cudaStream_t st, const Kv8AttnArgs &a);
 int launch_kv8_prefill(cudaStream_t st, const Kv8AttnArgs &a, void *ws);
 size_t kv8_prefill_workspace(int n_seqs, int L, int pos0);
 int launch_kv8_attn(cudaStream_t st, const Kv8AttnArgs &a);
+// The merge of launch_kv8_attn alone, of all the runs that a call can have.
+int launch_kv8_merge(cudaStream_t st, const Kv8AttnArgs &a);
 size_t kv8_attn_workspace(int n_seqs, int L);
 
 struct Kv8SelectArgs {

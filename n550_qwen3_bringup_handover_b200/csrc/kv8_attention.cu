@@ -86,6 +86,12 @@ template <int LT> constexpr int threads() { return (3 + 4 * groups<LT>()) * 32; 
 struct Cross {
     int s, kvh, n, slot;                        // n = 0: none; slot: the first piece's (2 c or 2 c + 1)
 };
+// Whether run c's record names a pair of the call and pieces of its runs. Records are
+// read from a workspace that nothing initialises; what is merged for one that no run
+// wrote has to stay inside it and inside out.
+__device__ __forceinline__ bool cross_ok(const Cross &x, int c, int n_runs, int n_seqs) {
+    return x.n > 0 && x.n <= n_runs - c && x.s >= 0 && x.s < n_seqs && x.kvh >= 0 && x.kvh < KV8_NKV;
+}
 
 __device__ __forceinline__ float ex2(float x) {
     float y;
@@ -362,6 +368,10 @@ kv8_attn_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
                 return u0;
             }, &cur);
             n_units = (int)(u1 - u0);
+            // An empty merge record until batch() has the run's last unit: a run whose waits
+            // expire before that leaves this one.
+            if (lane == 0) ((Cross *)p.part)[blockIdx.x] = Cross{};
+            __syncwarp();
         }
         // ---------------- producer: lane i takes unit 32 k + i ----------------
         bool seen = false;                       // the piece that reaches into this batch had a tile
@@ -469,7 +479,6 @@ kv8_attn_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
             me.flags = R_END;
             sends = 1;
             plane = 0;
-            if (lane == 0) ((Cross *)p.part)[blockIdx.x] = Cross{};
         }
         int r = 0;                               // records issued
         bool ok = true;
@@ -823,7 +832,7 @@ __global__ void __launch_bounds__(CMB_WARPS * 32) kv8_combine_kernel(const Kv8At
     const int4 x4 = __ldcg((const int4 *)p.part + blockIdx.x);
     const Cross x = *(const Cross *)&x4;
     const int pieces = x.n;
-    if (!pieces) return;
+    if (!cross_ok(x, blockIdx.x, n_runs, p.n_seqs)) return;
     const int n_col = 2 * p.L, wpc = max(1, CMB_WARPS / n_col), sub = warp % wpc;
     const size_t stride = (size_t)n_col * (KV8_HD + 2);
     // piece k: slot 2 (c + k), but the first one's is given
@@ -931,6 +940,13 @@ size_t kv8_attn_workspace(int n_seqs, int L) {
         most = need > most ? need : most;
     }
     return most;
+}
+
+int launch_kv8_merge(cudaStream_t st, const Kv8AttnArgs &a) {
+    const int n = max_ctas(a.L);
+    N550_CUDA_TRY(launch_k(kv8_combine_kernel, dim3(n - 1), CMB_WARPS * 32, 0, st, a, n));
+    N550_LAUNCH_CHECK();
+    return N550_OK;
 }
 
 int launch_kv8_attn(cudaStream_t st, const Kv8AttnArgs &a) {

@@ -120,3 +120,12 @@ def test_oracle_rounding_is_e4m3():
     assert torch.equal(round_codes(x.double()), x.to(torch.float8_e4m3fn).view(torch.uint8))
     assert scale_for(torch.tensor([448.0])) == 1.0 and scale_for(torch.tensor([448.5])) == 2.0
     assert scale_for(torch.tensor([0.0])) == 2.0 ** -126
+
+
+def test_merge_check_refuses():
+    """No workspace, too small or unaligned a one, no sequences, no rows to write to."""
+    L = n5.lib()
+    need = L.n550_attention_kv8_workspace(1)
+    for n, ws, size, out, ld in [(1, None, need, P, 2048), (1, P, need - 1, P, 2048), (1, P + 8, need, P, 2048), (0, P, need, P, 2048),
+                                 (65536, P, need, P, 2048), (1, P, need, None, 2048), (1, P, need, P, 2040)]:
+        assert L.n550_check_kv8_merge(None, n, ws, size, out, ld) == n5.ERR_ARG

@@ -669,3 +669,43 @@ def test_wrapper_refusals():
     off = torch.empty(2 * 2048 + 4, dtype=torch.bfloat16, device="cuda")[4:].view(2, 2048)
     with pytest.raises(n5.N550Error):
         n5.attention_decode_kv8(off, c, sid, pos, 1)          # not 16-byte aligned
+
+
+@pytest.mark.parametrize("fill", [0x00, 0x7F, 0xFF, None])
+def test_merge_skips_records_that_no_run_wrote(fill):
+    """The merge after an attention kernel that gave up before its records were written:
+    whatever the workspace holds, only rows of records that name a pair and pieces of the
+    call are written. (1 << 30 pieces, a sequence or a head that is not there and one
+    piece too many would otherwise lead out of the workspace and out of `out`.)"""
+    L, n, runs = n5.lib(), 3, 444                             # 148 SMs x 3 CTAs
+    need = L.n550_attention_kv8_workspace(n)
+    assert need == runs * (16 + 2 * 2 * 130 * 4)
+    ws = torch.zeros(need // 4, dtype=torch.int32, device="cuda")
+    rec = ws[:4 * runs].view(runs, 4)                         # sequence, KV head, pieces, slot
+    part = ws[4 * runs:].view(torch.float32).view(2 * runs, 2 * 130)
+    big = 2147483647
+    if fill is not None:
+        ws.view(torch.uint8).fill_(fill)
+    else:
+        rec[:, :] = torch.tensor([[0, 0, 1 << 30, 0], [n, 0, 2, 0], [-1, 0, 2, 0], [0, 8, 2, 0], [0, -1, 2, 0], [0, 0, -1, 0],
+                                  [0, 0, -big - 1, 0], [big, 0, 2, 0], [0, big, 2, 0], [0, 0, runs - 8, 0], [0, 0, big, 0],
+                                  [0, 0, 0, 0]], dtype=torch.int32).repeat(37, 1).cuda()
+        for c in range(9, runs, 12):
+            rec[c, 2] = runs - c + 1                          # one piece more than there are runs
+    out = torch.full((n + 2, 2048), 7.0, dtype=torch.bfloat16, device="cuda")
+    rows_ = out[1:1 + n]
+
+    def merge():
+        n5.check(L.n550_check_kv8_merge(n5.stream_ptr(), n, ws.data_ptr(), need, rows_.data_ptr(), 2048))
+        torch.cuda.synchronize()
+
+    merge()
+    assert (out == 7).all()
+    # one record among them that a run wrote: pieces in runs 440 and 441, the first in slot 881
+    rec[440] = i32([2, 5, 2, 881])
+    part[881, :256], part[881, 256:] = 3.0, torch.tensor([1.0, 4.0, 1.0, 4.0], device="cuda")
+    part[882, :256], part[882, 256:] = 5.0, torch.tensor([1.0, 4.0, 1.0, 4.0], device="cuda")
+    merge()
+    want = torch.full((n + 2, 2048), 7.0, dtype=torch.bfloat16)
+    want[3, 5 * 256:6 * 256] = 1.0                            # (3 + 5) / (4 + 4)
+    assert torch.equal(out.cpu(), want)
