@@ -83,11 +83,24 @@ def _ids(seq_ids, pos=None):
     return n
 
 
+_INT_MAX = 2 ** 31 - 1
+
+
+def _c_ints(**values):
+    """Numbers that the library takes as C ints: ctypes would cut larger ones to their
+    lower 32 bits."""
+    for name, x in values.items():
+        if not -_INT_MAX <= x <= _INT_MAX:
+            raise ValueError(f"{name} = {x} does not fit 32 bits")
+
+
 def _rows(name, t, rows, cols, dtypes):
     shape, stride = t.shape, t.stride()
     if len(shape) != 2 or shape[0] != rows or shape[1] < cols or t.dtype not in dtypes or \
             (stride[1] != 1 and rows > 0):
         raise ValueError(f"{name} must be [{rows}, >= {cols}] with contiguous rows of {dtypes}")
+    if rows > 1 and stride[0] > _INT_MAX:
+        raise ValueError(f"{name} must have a row stride below 2^31 elements")
     # the stride of a single row is never used; torch reports any number there
     return stride[0] if rows > 1 else cols
 
@@ -96,6 +109,7 @@ def kv8_append(cache, k, v, seq_ids, pos, L, layer):
     """Quantise len(seq_ids) x L rows of k and v ([n_seqs*L, >= 1024] float32 or
     bfloat16) into positions pos[s] .. pos[s]+L-1 of slot seq_ids[s]."""
     import torch
+    _c_ints(layer=layer, L=L)
     st = _stream(cache, k, v, seq_ids, pos)
     n = _ids(seq_ids, pos)
     if L < 0:
@@ -128,6 +142,7 @@ def attention_decode_kv8(q, cache, seq_ids, pos, layer, out=None, split=True):
     cache; split=True passes a split-KV workspace, split=False runs one CTA per
     (sequence, KV head)."""
     n = _ids(seq_ids, pos)
+    _c_ints(layer=layer)
     ldq, out, ldo = _q_out(q, n, out)
     st = _stream(cache, q, seq_ids, pos, out)
     L = lib()
@@ -148,6 +163,7 @@ def attention_sparse_kv8(q, cache, seq_ids, pos, blocks, layer, out=None, split=
     if blocks.dtype != torch.int32 or len(shape) != 3 or shape[0] != n or shape[1] != _NKV or \
             not blocks.is_contiguous():
         raise ValueError(f"blocks must be a contiguous int32 tensor [{n}, 8, n_select]")
+    _c_ints(layer=layer, n_select=shape[2])
     ldq, out, ldo = _q_out(q, n, out)
     st = _stream(cache, q, seq_ids, pos, blocks, out)
     L = lib()
@@ -163,6 +179,7 @@ def attention_prefill_kv8(q, cache, seq_ids, L, pos0, layer, out=None, workspace
     """Causal attention of len(seq_ids) sequences x L queries (rows of q, BF16) at
     positions pos0.. over the 8-bit cache, which holds their K/V already."""
     n = _ids(seq_ids)
+    _c_ints(L=L, pos0=pos0, layer=layer)
     if L < 0:
         raise ValueError("L must not be negative")
     ldq, out, ldo = _q_out(q, n * L, out)
@@ -182,6 +199,7 @@ def kv8_select_blocks(q, cache, seq_ids, pos, layer, n_select, n_sink=1, n_recen
     -1 behind the last."""
     import torch
     n = _ids(seq_ids, pos)
+    _c_ints(layer=layer, n_select=n_select, n_sink=n_sink, n_recent=n_recent)
     ldq = _rows("q", q, n, _NH * _HD, (torch.bfloat16,))
     if out is None:
         out = torch.empty((n, _NKV, max(n_select, 0)), dtype=torch.int32, device=q.device)

@@ -129,3 +129,27 @@ def test_merge_check_refuses():
     for n, ws, size, out, ld in [(1, None, need, P, 2048), (1, P, need - 1, P, 2048), (1, P + 8, need, P, 2048), (0, P, need, P, 2048),
                                  (65536, P, need, P, 2048), (1, P, need, None, 2048), (1, P, need, P, 2040)]:
         assert L.n550_check_kv8_merge(None, n, ws, size, out, ld) == n5.ERR_ARG
+
+
+def test_wrappers_refuse_numbers_beyond_a_c_int():
+    """ctypes passes the lower 32 bits of an int: layer 2^32 would be layer 0, and rows
+    2^32 + 2048 elements apart would be read 2048 apart."""
+    ids, q = torch.zeros(2, dtype=torch.int32), torch.zeros((2, 2048), dtype=torch.bfloat16)
+    kv, blocks = torch.zeros((2, 1024)), torch.zeros((2, 8, 1), dtype=torch.int32)
+    for big in (2 ** 31, 2 ** 32, 2 ** 32 + 1, -2 ** 32, 2 ** 64):
+        calls = [lambda: n5.kv8_append(None, kv, kv, ids, ids, 1, big),
+                 lambda: n5.attention_decode_kv8(q, None, ids, ids, big),
+                 lambda: n5.attention_sparse_kv8(q, None, ids, ids, blocks, big),
+                 lambda: n5.attention_prefill_kv8(q, None, ids, 1, 0, big),
+                 lambda: n5.attention_prefill_kv8(q, None, ids, 1, big, 0),
+                 lambda: n5.kv8_select_blocks(q, None, ids, ids, big, 4),
+                 lambda: n5.kv8_select_blocks(q, None, ids, ids, 0, 4, big, 0),
+                 lambda: n5.kv8_select_blocks(q, None, ids, ids, 0, 4, 0, big)]
+        for call in calls:
+            with pytest.raises(ValueError, match="32 bits"):
+                call()
+    far = torch.empty_strided((2, 2048), (2 ** 32 + 2048, 1), dtype=torch.bfloat16, device="meta")
+    with pytest.raises(ValueError, match="row stride"):
+        n5.attention_decode_kv8(far, None, ids, ids, 0)
+    with pytest.raises(ValueError, match="row stride"):
+        n5.attention_decode_kv8(q, None, ids, ids, 0, out=far)
