@@ -185,7 +185,8 @@ def attention_prefill_kv8(q, cache, seq_ids, L, pos0, layer, out=None, workspace
     ldq, out, ldo = _q_out(q, n * L, out)
     st = _stream(cache, q, seq_ids, out)
     lb = lib()
-    nbytes = lb.n550_attention_prefill_kv8_workspace(n, L, pos0) if workspace else 0
+    # (positions outside the cache need none: the call below refuses them)
+    nbytes = lb.n550_attention_prefill_kv8_workspace(n, L, pos0) if workspace and pos0 + L <= cache.max_len else 0
     ws = _workspace(nbytes, q) if nbytes else None
     check(lb.n550_attention_prefill_kv8(st, q.data_ptr(), ldq, cache._ref, layer, seq_ids.data_ptr(), n,
                                         L, pos0, out.data_ptr(), ldo, ws.data_ptr() if nbytes else None, nbytes),

@@ -709,3 +709,12 @@ def test_merge_skips_records_that_no_run_wrote(fill):
     want = torch.full((n + 2, 2048), 7.0, dtype=torch.bfloat16)
     want[3, 5 * 256:6 * 256] = 1.0                            # (3 + 5) / (4 + 4)
     assert torch.equal(out.cpu(), want)
+
+
+@pytest.mark.parametrize("pos0", [1, 1 << 30, 2 ** 31 - 1])
+def test_prefill_past_the_cache_is_refused_before_its_workspace(pos0):
+    """The workspace of 300 queries at 2^30 would be 4 TB: the call is refused as such."""
+    c, _ = filled(1, 300, 720)
+    with pytest.raises(n5.N550Error) as e:
+        n5.attention_prefill_kv8(rows(300, 2048, torch.bfloat16, 721).cuda(), c, i32([0]), 300, pos0, 1)
+    assert e.value.status == n5.ERR_ARG
