@@ -36,6 +36,7 @@
 //              With more query tokens more such groups share the columns.
 //   last warp  splits the queries of each new pair
 #include <cuda.h>
+#include <float.h>
 
 #include "kv8.h"
 #include "launch.h"
@@ -731,7 +732,7 @@ kv8_attn_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
             float x[NG], sum[NG], vmax = 0.f;                      // this tile's maximum and sum
             if (tile && !dead) {
                 const int blk = half ? w.blk[1] : w.blk[0], pos = blk * KV8_BLOCK + (row & 63);
-                const float kf = (half ? w.ks[1] : w.ks[0]) * kKv8ScaleLog2;
+                const float kf = half ? w.ks[1] : w.ks[0];
                 float s[NG];
                 dead = !warp_wait(&s_full[t & 1], (t >> 1) & 1);
                 if (!dead) {
@@ -744,7 +745,11 @@ kv8_attn_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
                         s[c] = -INFINITY;
                         if (c < ng) {
                             const float q = fmaf(__uint_as_float(v[2 * c + 1]), 0.0625f, __uint_as_float(v[2 * c]));
-                            if (blk >= 0 && pos <= lim + c / 2) s[c] = q * qf[c] * kf;
+                            // The scales of q and k make one factor: q times its own could pass FP32's
+                            // largest number where the score does not. (A factor that does is taken as
+                            // that number: a sum of 0 stays 0.)
+                            const float f = qf[c] * kf;
+                            if (blk >= 0 && pos <= lim + c / 2) s[c] = q * ((f > FLT_MAX ? FLT_MAX : f) * kKv8ScaleLog2);
                         }
                         x[c] = warp_max(s[c]);
                     }

@@ -718,3 +718,31 @@ def test_prefill_past_the_cache_is_refused_before_its_workspace(pos0):
     with pytest.raises(n5.N550Error) as e:
         n5.attention_prefill_kv8(rows(300, 2048, torch.bfloat16, 721).cuda(), c, i32([0]), 300, pos0, 1)
     assert e.value.status == n5.ERR_ARG
+
+
+@pytest.mark.parametrize("qmax,kmax", [(2.0 ** 127.5, 2.0 ** -121), (2.0 ** 125, 2.0 ** -119), (2.0 ** -121, 2.0 ** 127), (2.0 ** -119, 2.0 ** 125)])
+@pytest.mark.parametrize("L", [1, 3, 7])
+def test_scores_of_queries_and_keys_at_the_ends_of_the_range(qmax, kmax, L):
+    """Queries near BF16's largest number over keys near its smallest, and the other way
+    round: their products are ordinary numbers, and so are the scores.
+
+    A score is a sum of 128 products of at most qmax kmax = 2^6.5, so below 2^13.5 before
+    the factor 2^-3.5: 128 roundings of partial sums that are below 2^13.5 move it by at
+    most 128 * 2^-24 * 2^13.5 * 2^-3.5 = 2^-7 (and a weight by that part of it). A query's
+    smallest parts are 2^-21 of its largest, half of which in 128 products with keys is
+    128 * 2^-22 * 2^6.5 * 2^-3.5 = 2^-12 more; the keys, of 4 bits, are what the cache
+    holds, also where their scale is 2^-126."""
+    n = 150
+    c = fresh(2, n)
+    g = gen(730)
+    k = (torch.rand((n, 1024), generator=g) * 2 - 1) * kmax
+    v = rows(n, 1024, torch.float32, 731)
+    n5.kv8_append(c, k.cuda(), v.cuda(), i32([1]), i32([0]), n, 1)
+    ref = Cache.of(c, 1)
+    q = ((torch.rand((L, 2048), generator=g) * 2 - 1) * qmax).to(torch.bfloat16)
+    out = n5.attention_prefill_kv8(q.cuda(), c, i32([1]), L, n - L, 1)
+    assert_near(out, *ref.attend(q, [1], [n - L], L), weight=HALF + 2.0 ** -7 + 2.0 ** -11)
+    if L == 1:
+        for split in (True, False):
+            out = n5.attention_decode_kv8(q.cuda(), c, i32([1]), i32([n - 1]), 1, split=split)
+            assert_near(out, *ref.attend(q, [1], [n - 1]), weight=HALF + 2.0 ** -7 + 2.0 ** -11)
