@@ -330,7 +330,8 @@ size_t n550_attention_kv8_workspace(int n_seqs);
  * n550_attention_prefill_kv8_workspace(n_seqs, L, pos0) bytes, as above. Up to 8
  * queries (and more, where few sequences have long contexts) stream the codes in
  * passes of 8; otherwise the workspace holds the context as BF16, 4096 bytes
- * per sequence and position. */
+ * per sequence and position. One that holds some of the sequences takes them in groups, the
+ * same bits a little slower, unless passes are faster than so many groups. */
 int n550_attention_prefill_kv8(void *stream, const uint16_t *q, int ldq, const n550_kv8_cache *c,
                                int layer, const int32_t *seq_ids, int n_seqs, int L, int pos0,
                                uint16_t *out, int ldo, void *workspace, size_t workspace_bytes);

@@ -119,10 +119,11 @@ int n550_attention_prefill_kv8(void *stream, const uint16_t *q, int ldq, const n
     a.q = q; a.ldq = ldq; a.out = out; a.ldo = ldo; a.seq_ids = seq_ids;
     a.L = L; a.pos0 = pos0; a.n_seqs = n_seqs; a.n_select = -1;
     a.rows = L;
-    const size_t need = n550_attention_prefill_kv8_workspace(n_seqs, L, pos0);
-    float *ws = split_ws(workspace, workspace_bytes, need);
-    if (ws && !kv8_in_passes(n_seqs, L, pos0)) return launch_kv8_prefill((cudaStream_t)stream, a, ws);
-    a.part = ws;                                   // (no workspace: passes without splits)
+    if (!split_ws(workspace, workspace_bytes, 0)) workspace_bytes = 0;
+    if (const int group = kv8_prefill_group(n_seqs, L, pos0, workspace_bytes))
+        return launch_kv8_prefill((cudaStream_t)stream, a, workspace, group);
+    // (a workspace too small for the splits' partials: passes without splits)
+    a.part = split_ws(workspace, workspace_bytes, kv8_attn_workspace(n_seqs, L < KV8_FEW ? L : KV8_FEW));
     return launch_kv8_passes((cudaStream_t)stream, a);
 }
 

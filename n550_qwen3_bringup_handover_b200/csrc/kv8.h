@@ -93,9 +93,11 @@ constexpr int KV8_FEW = 8;     // most queries per sequence of launch_kv8_attn
 // passes of KV8_FEW, rather than launch_kv8_prefill; and those passes.
 bool kv8_in_passes(int n_seqs, int L, int pos0);
 int launch_kv8_passes(cudaStream_t st, const Kv8AttnArgs &a);
-// Many queries: codes written out as BF16 to `ws` (kv8_prefill_workspace bytes), then
-// the BF16 prefill kernel.
-int launch_kv8_prefill(cudaStream_t st, const Kv8AttnArgs &a, void *ws);
+// Many queries: codes written out as BF16 to `ws`, then the BF16 prefill kernel, in
+// groups of `group` sequences (of which ws holds kv8_prefill_workspace bytes).
+int launch_kv8_prefill(cudaStream_t st, const Kv8AttnArgs &a, void *ws, int group);
+// Sequences per group with a workspace of that many bytes; 0: passes.
+int kv8_prefill_group(int n_seqs, int L, int pos0, size_t ws_bytes);
 size_t kv8_prefill_workspace(int n_seqs, int L, int pos0);
 int launch_kv8_attn(cudaStream_t st, const Kv8AttnArgs &a);
 // The merge of launch_kv8_attn alone, of all the runs that a call can have.

@@ -64,18 +64,43 @@ kv8_write_out_kernel(const Kv8View c, const int32_t *seq_ids, int len, uint16_t 
 
 }  // namespace
 
-// Time of both ways in us, from B200 measurements: a pass of up to 8 queries streams
-// the codes at 2.2 TB/s after 15 us; writing out moves 768 bytes per position and
-// head at 5 TB/s, and then a CTA takes 2 us for each 128 positions of 128 queries of
+namespace {
+
+// Times in us, from B200 measurements. A pass of up to 8 queries streams the codes at
+// 2.2 TB/s after 15 us; without a workspace a CTA of its own takes 1.7 us for each 128
+// positions of a pair, 148 of them at a time. Writing out moves 768 bytes per position
+// and head at 5 TB/s, and then a CTA takes 2 us for each 128 positions of 128 queries of
 // a KV head, the longest context of a wave of 148 of them deciding. Measured
 // (passes / whole, sequences x queries over positions): 8 x 5 over 2005 27 / 53, 8 x 16
-// over 2016 60 / 54, 64 x 8 over 508 51 / 82, 2 x 8 over 30008 67 / 550 (16 CTAs).
+// over 2016 60 / 54, 64 x 8 over 508 51 / 82, 2 x 8 over 30008 67 / 550 (16 CTAs);
+// (passes without a workspace / whole in groups of 1, 2, 4 sequences): 16 x 64 over 8256
+// 900 / 2402, 1264, 706; 8 x 512 over 33280 26307 / 4640, 2461, 1390.
+double passes_us(int n_seqs, int L, int pos0, bool split) {
+    const double len = (double)pos0 + L, passes = (L + KV8_FEW - 1) / KV8_FEW;
+    if (split) return passes * (15.0 + n_seqs * len * KV8_NKV * 256 / 2.2e6);
+    return passes * (4.0 + (n_seqs * KV8_NKV + 147) / 148 * (len / 128) * 1.7);
+}
+double whole_us(int n_seqs, int L, int pos0, int group) {
+    const double len = (double)pos0 + L;
+    const long long items = (long long)group * KV8_NKV * ((L + 127) / 128);
+    return (n_seqs + group - 1) / group *
+           (4.0 + group * len * KV8_NKV * 768 / 5e6 + (double)((items + 147) / 148) * (len / 128) * 2.0);
+}
+
+}  // namespace
+
 bool kv8_in_passes(int n_seqs, int L, int pos0) {
-    if (L <= KV8_FEW) return true;
-    const double positions = (double)n_seqs * ((double)pos0 + L) * KV8_NKV;
-    const double passes = (L + KV8_FEW - 1) / KV8_FEW * (15.0 + positions * 256 / 2.2e6);
-    const double items = (double)n_seqs * KV8_NKV * ((L + 127) / 128), waves = (double)(((long long)items + 147) / 148);
-    return passes < 4.0 + positions * 768 / 5e6 + waves * (((double)pos0 + L) / 128) * 2.0;
+    return L <= KV8_FEW || passes_us(n_seqs, L, pos0, true) < whole_us(n_seqs, L, pos0, n_seqs);
+}
+
+int kv8_prefill_group(int n_seqs, int L, int pos0, size_t ws_bytes) {
+    if (L <= KV8_FEW) return 0;
+    const size_t fit = ws_bytes / kv8_prefill_workspace(1, L, pos0);
+    if (fit >= (size_t)n_seqs) return kv8_in_passes(n_seqs, L, pos0) ? 0 : n_seqs;
+    if (!fit) return 0;
+    const int groups = (int)(((size_t)n_seqs + fit - 1) / fit), group = (n_seqs + groups - 1) / groups;   // of even sizes
+    const bool split = ws_bytes >= kv8_attn_workspace(n_seqs, KV8_FEW);
+    return passes_us(n_seqs, L, pos0, split) < whole_us(n_seqs, L, pos0, group) ? 0 : group;
 }
 
 int launch_kv8_passes(cudaStream_t st, const Kv8AttnArgs &a) {
@@ -93,19 +118,32 @@ size_t kv8_prefill_workspace(int n_seqs, int L, int pos0) {
     return 2 * sizeof(uint16_t) * (size_t)n_seqs * KV8_NKV * ((size_t)pos0 + L) * KV8_HD;
 }
 
-int launch_kv8_prefill(cudaStream_t st, const Kv8AttnArgs &a, void *ws) {
+namespace {
+
+// n_seqs sequences from `s0` on, whose contexts fit `ws`.
+int launch_group(cudaStream_t st, const Kv8AttnArgs &a, int s0, int n_seqs, void *ws) {
     const int len = a.pos0 + a.L;
-    uint16_t *kd = (uint16_t *)ws, *vd = kd + (size_t)a.n_seqs * KV8_NKV * len * KV8_HD;
-    const dim3 grid((len + KV8_BLOCK - 1) / KV8_BLOCK, KV8_NKV, a.n_seqs);
-    N550_CUDA_TRY(launch_k(kv8_write_out_kernel, grid, WO_THREADS, 0, st, a.c, a.seq_ids, len, kd, vd));
+    const int32_t *seq_ids = a.seq_ids + s0;
+    const size_t row = (size_t)s0 * a.L;
+    uint16_t *kd = (uint16_t *)ws, *vd = kd + (size_t)n_seqs * KV8_NKV * len * KV8_HD;
+    const dim3 grid((len + KV8_BLOCK - 1) / KV8_BLOCK, KV8_NKV, n_seqs);
+    N550_CUDA_TRY(launch_k(kv8_write_out_kernel, grid, WO_THREADS, 0, st, a.c, seq_ids, len, kd, vd));
     N550_LAUNCH_CHECK();
     AttnPrefillArgs p{};
-    p.q = a.q; p.kc = kd; p.vc = vd; p.out = a.out;
+    p.q = a.q + row * a.ldq; p.kc = kd; p.vc = vd; p.out = a.out + row * a.ldo;
     p.ldq = a.ldq; p.ldo = a.ldo; p.L = a.L; p.pos0 = a.pos0;
     p.max_len = len;
-    p.kv_planes = a.n_seqs * KV8_NKV;
+    p.kv_planes = n_seqs * KV8_NKV;
     p.packed = true;
-    return launch_attn_prefill(st, p, a.n_seqs);
+    return launch_attn_prefill(st, p, n_seqs);
+}
+
+}  // namespace
+
+int launch_kv8_prefill(cudaStream_t st, const Kv8AttnArgs &a, void *ws, int group) {
+    for (int s0 = 0; s0 < a.n_seqs; s0 += group)
+        if (int rc = launch_group(st, a, s0, a.n_seqs - s0 < group ? a.n_seqs - s0 : group, ws)) return rc;
+    return N550_OK;
 }
 
 }  // namespace n550

@@ -835,14 +835,7 @@ int run_attention_kv8(n550_model *m, cudaStream_t st, bool decode, const int32_t
         return N550_OK;
     }
     const int group = (int)std::min<size_t>(Sc, m->kv8_out_bytes / kv8_prefill_workspace(1, Lc, p0));
-    for (int s = 0; s < Sc; s += group) {
-        Kv8AttnArgs g = a;
-        g.q = m->qb + (size_t)s * Lc * QD;
-        g.out = m->attn + (size_t)s * Lc * QD;
-        g.seq_ids = seq_ids + s;
-        g.n_seqs = std::min(group, Sc - s);
-        STEP(N550_PROF_ATTN, 2, launch_kv8_prefill(st, g, m->kv8_out));
-    }
+    STEP(N550_PROF_ATTN, 2 * ((Sc + group - 1) / group), launch_kv8_prefill(st, a, m->kv8_out, group));
     return N550_OK;
 }
 

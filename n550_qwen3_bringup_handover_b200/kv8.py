@@ -175,6 +175,11 @@ def attention_sparse_kv8(q, cache, seq_ids, pos, blocks, layer, out=None, split=
     return out
 
 
+# Most bytes that attention_prefill_kv8 allocates as a workspace, if one sequence's
+# context as BF16 (4096 bytes a position) is not more: above it, sequences in groups.
+PREFILL_WORKSPACE_MAX = 4 << 30
+
+
 def attention_prefill_kv8(q, cache, seq_ids, L, pos0, layer, out=None, workspace=True):
     """Causal attention of len(seq_ids) sequences x L queries (rows of q, BF16) at
     positions pos0.. over the 8-bit cache, which holds their K/V already."""
@@ -187,6 +192,8 @@ def attention_prefill_kv8(q, cache, seq_ids, L, pos0, layer, out=None, workspace
     lb = lib()
     # (positions outside the cache need none: the call below refuses them)
     nbytes = lb.n550_attention_prefill_kv8_workspace(n, L, pos0) if workspace and pos0 + L <= cache.max_len else 0
+    if nbytes > PREFILL_WORKSPACE_MAX:
+        nbytes = min(nbytes, max(PREFILL_WORKSPACE_MAX, lb.n550_attention_prefill_kv8_workspace(1, L, pos0)))
     ws = _workspace(nbytes, q) if nbytes else None
     check(lb.n550_attention_prefill_kv8(st, q.data_ptr(), ldq, cache._ref, layer, seq_ids.data_ptr(), n,
                                         L, pos0, out.data_ptr(), ldo, ws.data_ptr() if nbytes else None, nbytes),

@@ -746,3 +746,67 @@ def test_scores_of_queries_and_keys_at_the_ends_of_the_range(qmax, kmax, L):
         for split in (True, False):
             out = n5.attention_decode_kv8(q.cuda(), c, i32([1]), i32([n - 1]), 1, split=split)
             assert_near(out, *ref.attend(q, [1], [n - 1]), weight=HALF + 2.0 ** -7 + 2.0 ** -11)
+
+
+def prefill_with(c, q, ids, L, pos0, nbytes):
+    """n550_attention_prefill_kv8 with a workspace of nbytes, nothing behind which is written."""
+    import ctypes as C
+    ws = torch.full((nbytes + 4096,), 0x7F, dtype=torch.uint8, device="cuda")
+    out = torch.empty((len(ids) * L, 2048), dtype=torch.bfloat16, device="cuda")
+    n5.check(n5.lib().n550_attention_prefill_kv8(n5.stream_ptr(), q.data_ptr(), 2048, C.byref(c._c), 1, i32(ids).data_ptr(), len(ids),
+                                                 L, pos0, out.data_ptr(), 2048, ws.data_ptr() if nbytes else None, nbytes))
+    torch.cuda.synchronize()
+    assert (ws[nbytes:] == 0x7F).all()
+    return out
+
+
+def test_prefill_in_groups_of_what_the_workspace_holds():
+    """A workspace of some of the sequences: the same bits as with all of them (one
+    sequence's rows do not depend on the others); of less than one, passes."""
+    L, pos0 = 130, 70
+    c, ref = filled(3, pos0 + L, 740)
+    ids = [2, 0, 5, 1, 0, 2, 1]                               # (a slot that is not there, too)
+    q = rows(len(ids) * L, 2048, torch.bfloat16, 741).cuda()
+    one = 4096 * (pos0 + L)
+    assert n5.lib().n550_attention_prefill_kv8_workspace(len(ids), L, pos0) == len(ids) * one
+    want = prefill_with(c, q, ids, L, pos0, len(ids) * one)
+    assert_near(want, *ref.attend(q.cpu(), ids, [pos0] * len(ids), L), weight=BF)
+    for nbytes in (one, 2 * one, 3 * one + 100, 4 * one, 6 * one, 7 * one - 1, 9 * one):
+        assert torch.equal(prefill_with(c, q, ids, L, pos0, nbytes), want), nbytes
+    none = prefill_with(c, q, ids, L, pos0, 0)
+    assert torch.equal(prefill_with(c, q, ids, L, pos0, one - 1), none)
+    assert_near(none, *ref.attend(q.cpu(), ids, [pos0] * len(ids), L))
+    assert n5.device_status() == n5.OK
+
+
+def test_prefill_splits_with_a_workspace_too_small_for_a_sequence():
+    """Room for the splits' partials, but for no context as BF16."""
+    L, pos0, ids = 20, 1900, [1, 0, 1, 0, 1, 0, 1, 0, 1, 0, 1, 0]
+    c, _ = filled(2, pos0 + L, 750)
+    q = rows(len(ids) * L, 2048, torch.bfloat16, 751).cuda()
+    lb = n5.lib()
+    split, one = lb.n550_attention_prefill_kv8_workspace(len(ids), 8, pos0), 4096 * (pos0 + L)
+    assert split < one < lb.n550_attention_prefill_kv8_workspace(len(ids), L, pos0)
+    got = prefill_with(c, q, ids, L, pos0, split)
+    # passes of 8, 8 and 4 queries with splits
+    for j in (0, 8, 16):
+        m = min(8, L - j)
+        part = q.view(len(ids), L, 2048)[:, j:j + m].reshape(-1, 2048).contiguous()
+        want = n5.attention_prefill_kv8(part, c, i32(ids), m, pos0 + j, 1)
+        assert torch.equal(got.view(len(ids), L, 2048)[:, j:j + m], want.view(len(ids), m, 2048))
+    # and without: as with no workspace at all
+    assert torch.equal(prefill_with(c, q, ids, L, pos0, split - 1), prefill_with(c, q, ids, L, pos0, 0))
+
+
+def test_prefill_wrapper_caps_its_workspace(monkeypatch):
+    c, _ = filled(2, 400, 760)
+    ids = i32([1, 0, 1, 0, 0])
+    q = rows(5 * 200, 2048, torch.bfloat16, 761).cuda()
+    want = n5.attention_prefill_kv8(q, c, ids, 200, 200, 1)
+    most = []
+    was = n5.kv8._workspace
+    monkeypatch.setattr(n5.kv8, "_workspace", lambda nbytes, q: most.append(nbytes) or was(nbytes, q))
+    for cap, nbytes in ((5 * 400 * 4096, 5 * 400 * 4096), (2 * 400 * 4096 + 7, 2 * 400 * 4096 + 7), (1, 400 * 4096)):
+        monkeypatch.setattr(n5.kv8, "PREFILL_WORKSPACE_MAX", cap)
+        assert torch.equal(n5.attention_prefill_kv8(q, c, ids, 200, 200, 1), want)
+        assert most.pop() == nbytes
