@@ -643,7 +643,11 @@ int model_setup(n550_model *m) {
     }
     const size_t T = (size_t)c.max_tokens, S = (size_t)c.max_seqs;
     const size_t kv = (size_t)c.max_seqs * NLAYER * NKVH * (size_t)c.max_len * HDIM;
-#define ALLOC(p, bytes) N550_CUDA_TRY(cudaMalloc((void **)&(p), (bytes)))
+#define ALLOC(p, bytes)                                                                         \
+    do {                                                                                        \
+        const cudaError_t e = cudaMalloc((void **)&(p), (bytes));                               \
+        if (e != cudaSuccess) return e == cudaErrorMemoryAllocation ? N550_ERR_OOM : N550_ERR_CUDA; \
+    } while (0)
     ALLOC(m->kc, kv * 2);
     ALLOC(m->vc, kv * 2);
     ALLOC(m->x, T * H * 4);
@@ -708,6 +712,14 @@ int check_cfg(const n550_model_config *c) {
     if (c->gemm_mode != N550_MODE_FAST && c->gemm_mode != N550_MODE_EXACT) return N550_ERR_ARG;
     if (c->gemm_mode == N550_MODE_EXACT && c->kblock != 16 && c->kblock != 32) return N550_ERR_ARG;
     return N550_OK;
+}
+
+// An init that fails: nothing of it stays, its CUDA error included (the next launch
+// would report it as its own).
+int init_failed(n550_model *m, int rc) {
+    model_release(m);
+    (void)cudaGetLastError();
+    return rc;
 }
 
 // A [M,K] BF16 . W[N,K]^T with epilogue `epi` into c (ldc). SILU takes W2.
@@ -1174,19 +1186,17 @@ int n550_qwen3_init(n550_model_t **out, const void *blob, size_t blob_size,
     m->cfg = *cfg;
     bool tiled = false;
     rc = parse_qw3m((const uint8_t *)blob, blob_size, m->off, &tiled);
-    if (rc) { model_release(m); return rc; }
+    if (rc) return init_failed(m, rc);
     cudaGetDevice(&m->dev);
     m->blob_size = blob_size;
-    if (cudaMalloc(&m->blob, blob_size) != cudaSuccess) { model_release(m); return N550_ERR_OOM; }
-    if (cudaMemcpy(m->blob, blob, blob_size, cudaMemcpyHostToDevice) != cudaSuccess) {
-        model_release(m);
-        return N550_ERR_CUDA;
-    }
+    if (cudaMalloc(&m->blob, blob_size) != cudaSuccess) return init_failed(m, N550_ERR_OOM);
+    if (cudaMemcpy(m->blob, blob, blob_size, cudaMemcpyHostToDevice) != cudaSuccess)
+        return init_failed(m, N550_ERR_CUDA);
     if (tiled) {
         // Tile-major GEMM weights are put back into row-major order in place
         // (through a scratch copy), so every kernel sees one layout.
         uint16_t *tmp = nullptr;
-        if (cudaMalloc(&tmp, (size_t)INTER * H * 2) != cudaSuccess) { model_release(m); return N550_ERR_OOM; }
+        if (cudaMalloc(&tmp, (size_t)INTER * H * 2) != cudaSuccess) return init_failed(m, N550_ERR_OOM);
         for (int t = 0; t < N_TENSORS && !rc; t++) {
             int N = 0, K = 0;
             if (!is_gemm_weight(t, &N, &K)) continue;
@@ -1200,10 +1210,10 @@ int n550_qwen3_init(n550_model_t **out, const void *blob, size_t blob_size,
         }
         if (!rc && cudaDeviceSynchronize() != cudaSuccess) rc = N550_ERR_CUDA;
         cudaFree(tmp);
-        if (rc) { model_release(m); return rc; }
+        if (rc) return init_failed(m, rc);
     }
     rc = model_setup(m);
-    if (rc) { model_release(m); return rc; }
+    if (rc) return init_failed(m, rc);
     *out = m;
     return N550_OK;
 }
@@ -1220,14 +1230,12 @@ int n550_qwen3_init_random(n550_model_t **out, uint64_t seed, double sigma,
     make_header(hdr);
     m->blob_size = qw3m_row_size();
     rc = parse_qw3m(hdr, m->blob_size, m->off);
-    if (rc) { model_release(m); return rc; }
+    if (rc) return init_failed(m, rc);
     cudaGetDevice(&m->dev);
-    if (cudaMalloc(&m->blob, m->blob_size) != cudaSuccess) { model_release(m); return N550_ERR_OOM; }
+    if (cudaMalloc(&m->blob, m->blob_size) != cudaSuccess) return init_failed(m, N550_ERR_OOM);
     if (cudaMemset(m->blob, 0, m->blob_size) != cudaSuccess ||
-        cudaMemcpy(m->blob, hdr, 256, cudaMemcpyHostToDevice) != cudaSuccess) {
-        model_release(m);
-        return N550_ERR_CUDA;
-    }
+        cudaMemcpy(m->blob, hdr, 256, cudaMemcpyHostToDevice) != cudaSuccess)
+        return init_failed(m, N550_ERR_CUDA);
     const float scale = synth_normal_scale(sigma);
     for (int t = 0; t < N_TENSORS; t++) {
         bool nrm;
@@ -1235,10 +1243,10 @@ int n550_qwen3_init_random(n550_model_t **out, uint64_t seed, double sigma,
         uint16_t *dst = (uint16_t *)(m->blob + m->off[t]);
         if (nrm) fill_u16_kernel<<<grid1(n), 256>>>(dst, n, (uint16_t)0x3F80);
         else synth_bf16_kernel<<<148 * 16, 256>>>(dst, n, synth_key(seed, (uint64_t)t), scale);
-        if (cudaPeekAtLastError() != cudaSuccess) { model_release(m); return N550_ERR_CUDA; }
+        if (cudaPeekAtLastError() != cudaSuccess) return init_failed(m, N550_ERR_CUDA);
     }
     rc = model_setup(m);
-    if (rc) { model_release(m); return rc; }
+    if (rc) return init_failed(m, rc);
     *out = m;
     return N550_OK;
 }

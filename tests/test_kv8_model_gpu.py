@@ -257,3 +257,17 @@ def test_no_room_for_the_cache_to_go_back_to(cuda):
         hold = None
         m.close()
         torch.cuda.empty_cache()
+
+
+def test_a_model_that_does_not_fit_leaves_no_error_behind(cuda):
+    """229 GB of BF16 cache: N550_ERR_OOM, and the next model is built and runs."""
+    torch.cuda.empty_cache()
+    for _ in range(2):
+        with pytest.raises(n5.N550Error) as e:
+            n5.Model(seed=0, max_seqs=1, max_len=2_000_000, max_tokens=16)
+        assert e.value.status == n5.ERR_OOM
+        m = n5.Model(seed=0, max_seqs=1, max_len=64, max_tokens=16)
+        try:
+            assert m.forward_batch(np.arange(4, dtype=np.int32), 0)[0] >= 0
+        finally:
+            m.close()
