@@ -394,9 +394,13 @@ typedef struct {
     int    max_seqs;     /* sequences with their own KV cache              */
     int    max_len;      /* positions per sequence (QWEN3_MAX_SEQ)          */
     int    max_tokens;   /* tokens per forward call (activation capacity)   */
-    int    gemm_mode;    /* N550_MODE_FAST or N550_MODE_EXACT               */
+    int    gemm_mode;    /* N550_MODE_FAST (| N550_MODEL_KV8) or N550_MODE_EXACT */
     int    kblock;       /* exact-mode K-block (16 or 32)                   */
 } n550_model_config;
+
+/* With N550_MODE_FAST in gemm_mode: the model starts with the 8-bit KV cache
+ * (n550_qwen3_use_kv8), and the BF16 cache, twice its size, is not allocated. */
+#define N550_MODEL_KV8 0x100
 
 /* Parses a QW3M blob in host memory (qwen3.c:87-146: same header checks and
  * error codes) and uploads it to the current device. */
@@ -467,8 +471,8 @@ int n550_qwen3_fused_attention_prep(int on);
 int n550_qwen3_fused_decode(int on);
 
 /* Holds the model's KV cache as the 8-bit cache (n550_kv8_cache: e4m3 codes, half
- * the bytes a decode step reads) instead of BF16 (on = 1), or goes back (0, the
- * default). Either way the cache starts empty: call it before the first prefill.
+ * the bytes a decode step reads) instead of BF16 (on = 1), or goes back (0). (A model
+ * of N550_MODEL_KV8 starts with it, others with BF16.) Either way the cache starts empty: call it before the first prefill.
  * Synchronises and allocates; the other cache's memory is freed first, and so are
  * the pointers of an n550_qwen3_kv8_cache. N550_ERR_OOM: the new cache does not fit,
  * the BF16 one is (again) the model's; if that does not fit either, the forwards

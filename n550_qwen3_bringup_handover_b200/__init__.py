@@ -22,6 +22,7 @@ KV8_SELECT_MAX_BLOCKS = 24576  # N550_KV8_SELECT_MAX_BLOCKS
 ERR_MAGIC, ERR_VERSION, ERR_DTYPE, ERR_SHAPE, ERR_SIZE, ERR_OOM, ERR_LAYOUT = -1, -2, -3, -4, -5, -6, -7
 ERR_ARG, ERR_CUDA, ERR_UNSUPPORTED, ERR_TIMEOUT = -101, -102, -103, -104
 MODE_EXACT, MODE_FAST = 0, 1
+MODEL_KV8 = 0x100              # N550_MODEL_KV8
 N550_TOK_ERR_MAGIC, N550_TOK_ERR_VERSION, N550_TOK_ERR_SIZE, N550_TOK_ERR_OVERFLOW = -1, -2, -3, -5
 F32, BF16 = 0, 1
 LAYOUT_ROW, LAYOUT_TILE = 0, 1

@@ -518,7 +518,8 @@ struct n550_model {
     uint16_t *fused_qkv = nullptr;          // only if q/k/v are not contiguous
     const uint16_t *wqkv[NLAYER] = {};
     uint16_t *kc = nullptr, *vc = nullptr;
-    // the 8-bit cache instead of kc / vc (n550_qwen3_use_kv8)
+    // the 8-bit cache instead of kc / vc (N550_MODEL_KV8, n550_qwen3_use_kv8)
+    bool starts_kv8 = false;                // created with N550_MODEL_KV8 (cfg.gemm_mode is without it)
     n550_kv8_cache kv8{};
     uint16_t *kv_rows = nullptr;            // K and V rows of one layer's tokens [max_tokens][2048]
     void *kv8_ws = nullptr, *kv8_out = nullptr;   // split partials; the context written out as BF16
@@ -619,6 +620,68 @@ void model_release(n550_model *m) {
     delete m;
 }
 
+template <class T>
+void give_back(T *&p) {
+    if (p) cudaFree(p);
+    p = nullptr;
+}
+size_t cache_elems(const n550_model_config &c) {
+    return (size_t)c.max_seqs * NLAYER * NKVH * (size_t)c.max_len * HDIM;
+}
+
+// The BF16 cache, zeroed. N550_ERR_OOM: nothing is held.
+int bf16_cache_get(n550_model *m) {
+    const size_t bytes = cache_elems(m->cfg) * 2;
+    if (cudaMalloc((void **)&m->kc, bytes) != cudaSuccess || cudaMalloc((void **)&m->vc, bytes) != cudaSuccess) {
+        (void)cudaGetLastError();
+        give_back(m->kc); give_back(m->vc);
+        return N550_ERR_OOM;
+    }
+    N550_CUDA_TRY(cudaMemset(m->kc, 0, bytes));
+    N550_CUDA_TRY(cudaMemset(m->vc, 0, bytes));
+    N550_CUDA_TRY(cudaDeviceSynchronize());
+    return N550_OK;
+}
+
+void kv8_cache_free(n550_model *m) {
+    give_back(m->kv8.k); give_back(m->kv8.v); give_back(m->kv8.k_scale); give_back(m->kv8.v_scale);
+    give_back(m->kv8.k_bounds); give_back(m->kv_rows); give_back(m->kv8_ws); give_back(m->kv8_out);
+}
+
+// The 8-bit cache and what its attention needs, empty. N550_ERR_OOM: nothing is held.
+int kv8_cache_get(n550_model *m) {
+    const n550_model_config &c = m->cfg;
+    const size_t codes = cache_elems(c);
+    const size_t scales = (size_t)c.max_seqs * NLAYER * NKVH * (((size_t)c.max_len + N550_KV8_BLOCK - 1) / N550_KV8_BLOCK);
+    // contexts as BF16 for prefill attention: one whole sequence, or up to 256 MB of them
+    const size_t one = kv8_prefill_workspace(1, c.max_len, 0);
+    m->kv8_out_bytes = std::max(one, std::min(one * c.max_seqs, (size_t)256 << 20));
+    const struct { void **p; size_t n; } want[] = {
+        {(void **)&m->kv8.k, codes}, {(void **)&m->kv8.v, codes},
+        {(void **)&m->kv8.k_scale, scales * 4}, {(void **)&m->kv8.v_scale, scales * 4},
+        {(void **)&m->kv8.k_bounds, scales * 2 * HDIM},
+        {(void **)&m->kv_rows, (size_t)c.max_tokens * 2 * KVD * 2},
+        {&m->kv8_ws, kv8_attn_workspace(c.max_seqs, KV8_FEW)}, {&m->kv8_out, m->kv8_out_bytes}};
+    for (const auto &w : want)
+        if (cudaMalloc(w.p, w.n) != cudaSuccess) {
+            (void)cudaGetLastError();
+            kv8_cache_free(m);
+            return N550_ERR_OOM;
+        }
+    m->kv8.n_slots = c.max_seqs;
+    m->kv8.n_layers = NLAYER;
+    m->kv8.max_len = c.max_len;
+    // positions never written read as zeros, like the BF16 cache's
+    N550_CUDA_TRY(cudaMemset(m->kv8.k, 0, codes));
+    N550_CUDA_TRY(cudaMemset(m->kv8.v, 0, codes));
+    N550_CUDA_TRY(cudaMemset(m->kv8.k_bounds, 0, scales * 2 * HDIM));
+    fill_f32_kernel<<<grid1(scales), 256>>>(m->kv8.k_scale, scales, 0x1p-126f);
+    fill_f32_kernel<<<grid1(scales), 256>>>(m->kv8.v_scale, scales, 0x1p-126f);
+    N550_LAUNCH_CHECK();
+    N550_CUDA_TRY(cudaDeviceSynchronize());
+    return N550_OK;
+}
+
 // Allocations that depend on the config; the blob must already be on device.
 int model_setup(n550_model *m) {
     const n550_model_config &c = m->cfg;
@@ -642,14 +705,12 @@ int model_setup(n550_model *m) {
         }
     }
     const size_t T = (size_t)c.max_tokens, S = (size_t)c.max_seqs;
-    const size_t kv = (size_t)c.max_seqs * NLAYER * NKVH * (size_t)c.max_len * HDIM;
+    if (const int rc = m->starts_kv8 ? kv8_cache_get(m) : bf16_cache_get(m)) return rc;
 #define ALLOC(p, bytes)                                                                         \
     do {                                                                                        \
         const cudaError_t e = cudaMalloc((void **)&(p), (bytes));                               \
         if (e != cudaSuccess) return e == cudaErrorMemoryAllocation ? N550_ERR_OOM : N550_ERR_CUDA; \
     } while (0)
-    ALLOC(m->kc, kv * 2);
-    ALLOC(m->vc, kv * 2);
     ALLOC(m->x, T * H * 4);
     ALLOC(m->xb, T * H * 2);
     ALLOC(m->qkv, T * QKVD * 4);
@@ -697,8 +758,6 @@ int model_setup(n550_model *m) {
                                W(m, l, 7), W(m, l, 8), W(m, l, 9), W(m, l, 10)};
         N550_CUDA_TRY(cudaMemcpy(m->fd_layers, fl, sizeof fl, cudaMemcpyHostToDevice));
     }
-    N550_CUDA_TRY(cudaMemset(m->kc, 0, kv * 2));
-    N550_CUDA_TRY(cudaMemset(m->vc, 0, kv * 2));
     int rc = ensure_rope_table();
     if (rc) return rc;
     rope_table_kernel<<<(c.max_len * 64 + 255) / 256, 256>>>(m->rope, c.max_len);
@@ -709,9 +768,19 @@ int model_setup(n550_model *m) {
 
 int check_cfg(const n550_model_config *c) {
     if (!c || c->max_seqs < 1 || c->max_len < 1 || c->max_tokens < 1) return N550_ERR_ARG;
-    if (c->gemm_mode != N550_MODE_FAST && c->gemm_mode != N550_MODE_EXACT) return N550_ERR_ARG;
-    if (c->gemm_mode == N550_MODE_EXACT && c->kblock != 16 && c->kblock != 32) return N550_ERR_ARG;
+    const int mode = c->gemm_mode & ~N550_MODEL_KV8;
+    if (mode != N550_MODE_FAST && mode != N550_MODE_EXACT) return N550_ERR_ARG;
+    if (mode == N550_MODE_EXACT && c->kblock != 16 && c->kblock != 32) return N550_ERR_ARG;
+    if (mode == N550_MODE_EXACT && c->gemm_mode != mode) return N550_ERR_UNSUPPORTED;
     return N550_OK;
+}
+
+n550_model *new_model(const n550_model_config &c) {
+    n550_model *m = new n550_model();
+    m->cfg = c;
+    m->starts_kv8 = c.gemm_mode & N550_MODEL_KV8;
+    m->cfg.gemm_mode &= ~N550_MODEL_KV8;
+    return m;
 }
 
 // An init that fails: nothing of it stays, its CUDA error included (the next launch
@@ -1182,8 +1251,7 @@ int n550_qwen3_init(n550_model_t **out, const void *blob, size_t blob_size,
     *out = nullptr;
     int rc = check_cfg(cfg);
     if (rc) return rc;
-    n550_model *m = new n550_model();
-    m->cfg = *cfg;
+    n550_model *m = new_model(*cfg);
     bool tiled = false;
     rc = parse_qw3m((const uint8_t *)blob, blob_size, m->off, &tiled);
     if (rc) return init_failed(m, rc);
@@ -1224,8 +1292,7 @@ int n550_qwen3_init_random(n550_model_t **out, uint64_t seed, double sigma,
     *out = nullptr;
     int rc = check_cfg(cfg);
     if (rc) return rc;
-    n550_model *m = new n550_model();
-    m->cfg = *cfg;
+    n550_model *m = new_model(*cfg);
     uint8_t hdr[256];
     make_header(hdr);
     m->blob_size = qw3m_row_size();
@@ -1264,63 +1331,19 @@ static void drop_graphs(n550_model_t *m) {
 
 int n550_qwen3_use_kv8(n550_model_t *m, int on) {
     if (!m) return N550_ERR_ARG;
-    const n550_model_config &c = m->cfg;
-    if (c.gemm_mode != N550_MODE_FAST) return N550_ERR_UNSUPPORTED;
+    if (m->cfg.gemm_mode != N550_MODE_FAST) return N550_ERR_UNSUPPORTED;
     if (on ? m->kv8.k != nullptr : m->kc != nullptr) return N550_OK;
     N550_CUDA_TRY(cudaDeviceSynchronize());
     drop_graphs(m);
-    const size_t planes = (size_t)c.max_seqs * NLAYER * NKVH, codes = planes * (size_t)c.max_len * HDIM;
-    const size_t scales = planes * (((size_t)c.max_len + N550_KV8_BLOCK - 1) / N550_KV8_BLOCK);
-    auto give_back = [](auto &p) { if (p) cudaFree(p); p = nullptr; };
-    auto kv8_free = [&]() {
-        give_back(m->kv8.k); give_back(m->kv8.v); give_back(m->kv8.k_scale); give_back(m->kv8.v_scale);
-        give_back(m->kv8.k_bounds); give_back(m->kv_rows); give_back(m->kv8_ws); give_back(m->kv8_out);
-    };
-    auto bf16_get = [&]() -> int {
-        if (cudaMalloc((void **)&m->kc, codes * 2) != cudaSuccess || cudaMalloc((void **)&m->vc, codes * 2) != cudaSuccess) {
-            (void)cudaGetLastError();
-            give_back(m->kc); give_back(m->vc);
-            return N550_ERR_OOM;
-        }
-        N550_CUDA_TRY(cudaMemset(m->kc, 0, codes * 2));
-        N550_CUDA_TRY(cudaMemset(m->vc, 0, codes * 2));
-        N550_CUDA_TRY(cudaDeviceSynchronize());
-        return N550_OK;
-    };
     if (!on) {
-        kv8_free();
-        return bf16_get();
+        kv8_cache_free(m);
+        return bf16_cache_get(m);
     }
     // the BF16 cache makes room first; it comes back if the 8-bit one does not fit
     give_back(m->kc); give_back(m->vc);
-    // contexts as BF16 for prefill attention: one whole sequence, or up to 256 MB of them
-    const size_t one = kv8_prefill_workspace(1, c.max_len, 0);
-    m->kv8_out_bytes = std::max(one, std::min(one * c.max_seqs, (size_t)256 << 20));
-    const struct { void **p; size_t n; } want[] = {
-        {(void **)&m->kv8.k, codes}, {(void **)&m->kv8.v, codes},
-        {(void **)&m->kv8.k_scale, scales * 4}, {(void **)&m->kv8.v_scale, scales * 4},
-        {(void **)&m->kv8.k_bounds, scales * 2 * HDIM},
-        {(void **)&m->kv_rows, (size_t)c.max_tokens * 2 * KVD * 2},
-        {&m->kv8_ws, kv8_attn_workspace(c.max_seqs, KV8_FEW)}, {&m->kv8_out, m->kv8_out_bytes}};
-    for (const auto &w : want)
-        if (cudaMalloc(w.p, w.n) != cudaSuccess) {
-            (void)cudaGetLastError();
-            kv8_free();
-            const int rc = bf16_get();
-            return rc ? rc : N550_ERR_OOM;
-        }
-    m->kv8.n_slots = c.max_seqs;
-    m->kv8.n_layers = NLAYER;
-    m->kv8.max_len = c.max_len;
-    // positions never written read as zeros, like the BF16 cache's
-    N550_CUDA_TRY(cudaMemset(m->kv8.k, 0, codes));
-    N550_CUDA_TRY(cudaMemset(m->kv8.v, 0, codes));
-    N550_CUDA_TRY(cudaMemset(m->kv8.k_bounds, 0, scales * 2 * HDIM));
-    fill_f32_kernel<<<grid1(scales), 256>>>(m->kv8.k_scale, scales, 0x1p-126f);
-    fill_f32_kernel<<<grid1(scales), 256>>>(m->kv8.v_scale, scales, 0x1p-126f);
-    N550_LAUNCH_CHECK();
-    N550_CUDA_TRY(cudaDeviceSynchronize());
-    return N550_OK;
+    int rc = kv8_cache_get(m);
+    if (rc == N550_ERR_OOM && (rc = bf16_cache_get(m)) == N550_OK) rc = N550_ERR_OOM;
+    return rc;
 }
 
 int n550_qwen3_kv8_cache(const n550_model_t *m, n550_kv8_cache *c) {
@@ -1538,6 +1561,7 @@ int n550_qwen3_split_rows(int rows) {
 int n550_qwen3_get_config(const n550_model_t *m, n550_model_config *cfg) {
     if (!m || !cfg) return N550_ERR_ARG;
     *cfg = m->cfg;
+    if (m->starts_kv8) cfg->gemm_mode |= N550_MODEL_KV8;
     return N550_OK;
 }
 

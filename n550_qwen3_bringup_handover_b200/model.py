@@ -7,7 +7,7 @@ import ctypes as C
 
 import numpy as np
 
-from . import MODE_FAST, ModelConfig, SpecStats, check, lib
+from . import MODE_FAST, MODEL_KV8, ModelConfig, SpecStats, check, lib
 
 VOCAB = 151936
 EOS_IDS = (151645, 151643)          # QWEN3_EOS_TOKEN_ID_0 / _1 (qwen3_config.h:29-30)
@@ -19,8 +19,8 @@ class Model:
     def __init__(self, *, blob: np.ndarray | None = None, seed: int = 0, sigma: float = 0.02,
                  max_seqs: int = 1, max_len: int = 2048, max_tokens: int = 512,
                  gemm_mode: int = MODE_FAST, kblock: int = 16, kv8: bool = False):
-        """kv8: hold the KV cache in 8 bits (n550_qwen3_use_kv8; fast mode)."""
-        self.cfg = ModelConfig(max_seqs, max_len, max_tokens, gemm_mode, kblock)
+        """kv8: hold the KV cache in 8 bits (N550_MODEL_KV8; fast mode)."""
+        self.cfg = ModelConfig(max_seqs, max_len, max_tokens, gemm_mode | (MODEL_KV8 if kv8 else 0), kblock)
         # held for close(): at interpreter exit the module's globals may be gone
         self._lib = lib()
         h = C.c_void_p()
@@ -32,8 +32,6 @@ class Model:
             rc = lib().n550_qwen3_init_random(C.byref(h), seed, sigma, C.byref(self.cfg))
         check(rc, "n550_qwen3_init")
         self._h = h
-        if kv8:
-            self.use_kv8()
 
     @property
     def handle(self):

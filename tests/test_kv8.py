@@ -153,3 +153,12 @@ def test_wrappers_refuse_numbers_beyond_a_c_int():
         n5.attention_decode_kv8(far, None, ids, ids, 0)
     with pytest.raises(ValueError, match="row stride"):
         n5.attention_decode_kv8(q, None, ids, ids, 0, out=far)
+
+
+def test_exact_mode_with_the_8_bit_cache_is_refused():
+    h = C.c_void_p()
+    for mode, want in [(n5.MODE_EXACT | n5.MODEL_KV8, n5.ERR_UNSUPPORTED), (7, n5.ERR_ARG), (7 | n5.MODEL_KV8, n5.ERR_ARG),
+                       (n5.MODE_FAST | 2 * n5.MODEL_KV8, n5.ERR_ARG), (-1, n5.ERR_ARG)]:
+        cfg = n5.ModelConfig(1, 64, 16, mode, 16)
+        assert n5.lib().n550_qwen3_init_random(C.byref(h), 0, 0.02, C.byref(cfg)) == want
+        assert not h

@@ -271,3 +271,38 @@ def test_a_model_that_does_not_fit_leaves_no_error_behind(cuda):
             assert m.forward_batch(np.arange(4, dtype=np.int32), 0)[0] >= 0
         finally:
             m.close()
+
+
+def test_a_cache_that_fits_in_8_bits_alone(cuda):
+    """115 GB of codes where the BF16 cache would be 229 GB: the model is created with it, its
+    steps are those of a small model, and there is no way to BF16 from it."""
+    import ctypes as C
+    torch.cuda.empty_cache()
+    t, ids = toks(21, 81), i32([0])
+    got = []
+    for max_len in (64, 2_000_000):
+        m = n5.Model(seed=0, max_seqs=1, max_len=max_len, max_tokens=64, kv8=True)
+        try:
+            cfg = n5.ModelConfig()
+            n5.check(n5.lib().n550_qwen3_get_config(m.handle, C.byref(cfg)))
+            assert cfg.gemm_mode == n5.MODE_FAST | n5.MODEL_KV8 and cfg.max_len == max_len
+
+            def step():
+                a, b = logits(1), logits(1)
+                m.prefill(t[:20].view(1, 20), ids, 0, a)
+                m.decode(t[20:], ids, i32([20]), b)
+                torch.cuda.synchronize()
+                return [a, b]
+
+            got.append(step())
+            if max_len > 64:
+                with pytest.raises(n5.N550Error) as e:
+                    m.use_kv8(False)
+                assert e.value.status == n5.ERR_OOM
+                m.use_kv8()
+                got.append(step())
+        finally:
+            m.close()
+    assert n5.device_status() == n5.OK
+    for x in got[1:]:
+        assert torch.equal(x[0], got[0][0]) and torch.equal(x[1], got[0][1])
