@@ -156,8 +156,10 @@ class Model:
         nb = -(-c.max_len // KV8_BLOCK)
 
         def view(ptr, shape, kind, dtype):
-            n = int(np.prod(shape))
-            return torch.as_tensor(_DeviceArray(ptr, n, kind), device="cuda").view(dtype).view(shape)
+            t = torch.as_tensor(_DeviceArray(ptr, int(np.prod(shape)), kind), device="cuda")
+            if t.data_ptr() != ptr:           # torch copied it over
+                raise ValueError("the model is on another device than the current one")
+            return t.view(dtype).view(shape)
 
         e4 = torch.float8_e4m3fn
         return KV8Cache(k=view(c.k, plane + (c.max_len, 128), "|u1", e4),

@@ -306,3 +306,13 @@ def test_a_cache_that_fits_in_8_bits_alone(cuda):
     assert n5.device_status() == n5.OK
     for x in got[1:]:
         assert torch.equal(x[0], got[0][0]) and torch.equal(x[1], got[0][1])
+
+
+def test_the_cache_of_a_model_on_another_device_is_refused(model, monkeypatch):
+    """torch copies memory of another device to the current one: appends to such a
+    copy would be lost. (Here a copy on the same device stands in for it.)"""
+    assert model.kv8_cache().k.data_ptr() == model.kv8_cache()._c.k
+    was = torch.as_tensor
+    monkeypatch.setattr(torch, "as_tensor", lambda *a, **kw: was(*a, **kw).clone())
+    with pytest.raises(ValueError, match="another device"):
+        model.kv8_cache()
