@@ -36,8 +36,9 @@ constexpr int BK = 64;            // one 128-byte swizzle row of BF16
 constexpr int UMMA_K = 16;
 // Epilogue warps: 4 (one per TMEM lane quarter); the two-head QKV tile gets
 // 8 (one head each), because its per-row RMSNorm + RoPE work is latency-bound.
+__host__ __device__ constexpr bool tc_is_qkv(int EPI) { return EPI == TC_EPI_QKV_ROPE || EPI == TC_EPI_QKV_ROWS; }
 __host__ __device__ constexpr int tc_epi_warps(int BN, int EPI) {
-    return (EPI == TC_EPI_QKV_ROPE && BN == 256) ? 16 : 4;
+    return (tc_is_qkv(EPI) && BN == 256) ? 16 : 4;
 }
 
 // Staging tiles per epilogue warp: the residual epilogue double-buffers the
@@ -238,6 +239,9 @@ __device__ __forceinline__ float4 rope_cs2(int pos, int i) {
 // at a time) to keep register use low. Lane r owns tile row r: it reads that
 // row's token position / slot once, and the store loops take other rows'
 // destination addresses from their owners by shuffle.
+// ROWS: K and V heads go to rows of kv_rows instead (a template parameter: the
+// cache's address is not formed beside it).
+template <bool ROWS>
 __device__ __forceinline__ void epilogue_qkv(const TcQkv &p, uint32_t *stg, int lane, uint32_t taddr,
                                              int row0, int M, int head, const AccRelease *rel,
                                              const uint16_t *norm_w) {
@@ -251,12 +255,13 @@ __device__ __forceinline__ void epilogue_qkv(const TcQkv &p, uint32_t *stg, int 
     uint16_t *dst_row;                     // column 0 of this head in the destination row
     if (head < 16) {
         dst_row = p.q_bf16 + (size_t)mc * p.ldq + head * 128;
+    } else if (ROWS) {
+        dst_row = p.kv_rows + (size_t)mc * 2048 + (head - 16) * 128;
     } else {
         const int kvh = (head - 16) & 7;
         uint16_t *cache = head < 24 ? p.kc : p.vc;
         const size_t slot = ((size_t)p.tok_seq[mc] * 28 + p.layer) * 8 + kvh;
-        dst_row = p.kv_rows ? p.kv_rows + (size_t)mc * 2048 + (head - 16) * 128
-                            : cache + (slot * p.max_len + pos) * 128;
+        dst_row = cache + (slot * p.max_len + pos) * 128;
     }
     if (!row_ok) dst_row = nullptr;
     float scale = 1.f;
@@ -336,6 +341,7 @@ __device__ __forceinline__ void epilogue_qkv(const TcQkv &p, uint32_t *stg, int 
 // shared memory (xss, [parity][head][half][128 rows], parity alternating per
 // tile so a slot is rewritten only after the partner passed the next
 // barrier) behind the pair's 64-thread named barrier bar_id.
+template <bool ROWS>
 __device__ __forceinline__ void epilogue_qkv_half(const TcQkv &p, uint32_t *stg, int lane, uint32_t taddr,
                                                   int row0, int M, int head, const AccRelease *rel,
                                                   const uint16_t *norm_w, int half, int hh, int qrow,
@@ -349,12 +355,13 @@ __device__ __forceinline__ void epilogue_qkv_half(const TcQkv &p, uint32_t *stg,
     uint16_t *dst_row;
     if (head < 16) {
         dst_row = p.q_bf16 + (size_t)mc * p.ldq + head * 128;
+    } else if (ROWS) {
+        dst_row = p.kv_rows + (size_t)mc * 2048 + (head - 16) * 128;
     } else {
         const int kvh = (head - 16) & 7;
         uint16_t *cache = head < 24 ? p.kc : p.vc;
         const size_t slot = ((size_t)p.tok_seq[mc] * 28 + p.layer) * 8 + kvh;
-        dst_row = p.kv_rows ? p.kv_rows + (size_t)mc * 2048 + (head - 16) * 128
-                            : cache + (slot * p.max_len + pos) * 128;
+        dst_row = cache + (slot * p.max_len + pos) * 128;
     }
     if (!row_ok) dst_row = nullptr;
     float scale = 1.f;
@@ -481,7 +488,7 @@ gemm_tc_kernel(const __grid_constant__ CUtensorMap tmA,
         mbar_init(done, 1);
         fence_mbar_init();
     }
-    if (EPI == TC_EPI_QKV_ROPE && warp >= 2 && threadIdx.x - 64 < 32) {
+    if (tc_is_qkv(EPI) && warp >= 2 && threadIdx.x - 64 < 32) {
         // 32 threads copy the two norm weight vectors (2 x 256 B) once
         const int i = threadIdx.x - 64;
         ((uint4 *)norm_w)[i] = i < 16 ? ((const uint4 *)ep.qkv.q_norm)[i]
@@ -666,22 +673,23 @@ gemm_tc_kernel(const __grid_constant__ CUtensorMap tmA,
                                      (ldw % 4) == 0 && (n % 4) == 0);
                     __syncwarp();
                 }
-            } else if (EPI == TC_EPI_QKV_ROPE) {
+            } else if (tc_is_qkv(EPI)) {
+                constexpr bool ROWS = EPI == TC_EPI_QKV_ROWS;
                 if (NEPI == 16) {
                     // warps 2-9: first head of the tile, 10-17: second; within
                     // a head, warps 2-5 / 10-13 take rotation pairs 0-31 and
                     // 6-9 / 14-17 pairs 32-63 of their lane quarter
                     const int sw = warp - 2;
                     const int hh = sw >> 3, half = (sw >> 2) & 1;
-                    epilogue_qkv_half(ep.qkv, stg, lane, taddr + hh * 128, row0, M, nb * 2 + hh, &rel,
-                                      norm_w, half, hh, q * 32 + lane, xss, ab_tiles & 1,
-                                      1 + hh * 4 + q);
+                    epilogue_qkv_half<ROWS>(ep.qkv, stg, lane, taddr + hh * 128, row0, M, nb * 2 + hh, &rel,
+                                            norm_w, half, hh, q * 32 + lane, xss, ab_tiles & 1,
+                                            1 + hh * 4 + q);
                     ab_tiles++;
                 } else {
 #pragma unroll 1
                     for (int hh = 0; hh < BN / 128; hh++)
-                        epilogue_qkv(ep.qkv, stg, lane, taddr + hh * 128, row0, M,
-                                     nb * (BN / 128) + hh, hh + 1 == BN / 128 ? &rel : nullptr, norm_w);
+                        epilogue_qkv<ROWS>(ep.qkv, stg, lane, taddr + hh * 128, row0, M,
+                                           nb * (BN / 128) + hh, hh + 1 == BN / 128 ? &rel : nullptr, norm_w);
                 }
             } else if (EPI == TC_EPI_ARGMAX) {
                 // running (max, lowest column of the max) of this row over the
@@ -1016,10 +1024,14 @@ int launch_gemm_tc_qkv(cudaStream_t st, const uint16_t *a, int lda, const uint16
     if (bn == 256 && tc_use_pair(M, bn)) {
         // pair tiles: each CTA's B box is one head (128 rows)
         if ((rc = make_tmap(&tb, w, 4096, K, K, 128))) return rc;
-        return launch_impl<256, TC_EPI_QKV_ROPE, true>(st, ta, tb, tb, ep, M, 4096, K, max_ctas);
+        return q.kv_rows ? launch_impl<256, TC_EPI_QKV_ROWS, true>(st, ta, tb, tb, ep, M, 4096, K, max_ctas)
+                         : launch_impl<256, TC_EPI_QKV_ROPE, true>(st, ta, tb, tb, ep, M, 4096, K, max_ctas);
     }
-    if (bn == 256) return launch_impl<256, TC_EPI_QKV_ROPE>(st, ta, tb, tb, ep, M, 4096, K, max_ctas);
-    return launch_impl<128, TC_EPI_QKV_ROPE>(st, ta, tb, tb, ep, M, 4096, K, max_ctas);
+    if (bn == 256)
+        return q.kv_rows ? launch_impl<256, TC_EPI_QKV_ROWS>(st, ta, tb, tb, ep, M, 4096, K, max_ctas)
+                         : launch_impl<256, TC_EPI_QKV_ROPE>(st, ta, tb, tb, ep, M, 4096, K, max_ctas);
+    return q.kv_rows ? launch_impl<128, TC_EPI_QKV_ROWS>(st, ta, tb, tb, ep, M, 4096, K, max_ctas)
+                     : launch_impl<128, TC_EPI_QKV_ROPE>(st, ta, tb, tb, ep, M, 4096, K, max_ctas);
 }
 
 // 0: automatic; 128 / 256: single-CTA tiles of that width; 512: 256 x 256

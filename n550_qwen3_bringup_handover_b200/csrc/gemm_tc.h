@@ -13,7 +13,8 @@ enum {
     TC_EPI_RESID_F32 = 2,  // C (FP32) += acc           (residual add fused)
     TC_EPI_SILU_BF16 = 3,  // C (BF16) = silu(acc_gate) * acc_up (SwiGLU fused)
     TC_EPI_QKV_ROPE = 4,   // per-head RMSNorm + RoPE of q/k, q out, k/v into the KV cache
-    TC_EPI_ARGMAX = 5      // per row and tile: (max, lowest index of the max), no C written
+    TC_EPI_ARGMAX = 5,     // per row and tile: (max, lowest index of the max), no C written
+    TC_EPI_QKV_ROWS = 6    // TC_EPI_QKV_ROPE with k and v as rows (for the 8-bit cache's append)
 };
 
 // Operands of the fused QKV epilogue (qwen3.c:477-511): a 128-column tile is
@@ -22,7 +23,7 @@ struct TcQkv {
     uint16_t *q_bf16;          // [M, ldq] BF16 queries
     int ldq;
     uint16_t *kc, *vc;         // KV cache [seq][layer][kv_head][pos][128]
-    uint16_t *kv_rows;         // instead of the caches: K and V heads as rows [M][2048] (or NULL)
+    uint16_t *kv_rows;         // not NULL: K and V heads as rows [M][2048], instead of the caches
     int layer, max_len;
     const int32_t *tok_pos, *tok_seq;   // per row
     const uint16_t *q_norm, *k_norm;    // BF16 [128]
