@@ -274,7 +274,10 @@ size_t n550_attention_decode_workspace(int n_seqs, int max_len);
  *   k_bounds          [n_slots][n_layers][8][n_blocks][2][128] codes: the smallest
  *                     and the largest K code of the block in each channel
  *                     (NULL: not kept; n550_kv8_select_blocks needs them)
- * A value is its code times its block's scale, which BF16 holds exactly. k, v
+ * A value is its code times its block's scale, which BF16 holds exactly for scales
+ * from 2^-124 to 2^119. (Below, blocks of magnitudes under 448 * 2^-125, it may lie
+ * under BF16's smallest number; at 2^120, blocks with a magnitude over 448 * 2^119, codes
+ * of 256 and more, also those of infinities, are infinite.) k, v
  * and k_bounds are 16-byte aligned. Nothing needs to be initialised:
  * n550_kv8_append defines what later calls read. max_len (up to 2^30) need not be
  * a multiple of the block.

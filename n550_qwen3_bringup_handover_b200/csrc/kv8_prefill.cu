@@ -1,7 +1,7 @@
 // Attention of many queries per sequence over the 8-bit KV cache: the context's
-// codes are written out once as BF16 (exactly: e4m3 times a power of two) in
-// the plane order of the BF16 cache, packed for these sequences, and the tcgen05
-// prefill kernel runs over that.
+// codes are written out once as BF16 (e4m3 times a power of two: exactly, for scales from
+// 2^-124 to 2^119) in the plane order of the BF16 cache, packed for these sequences, and the
+// tcgen05 prefill kernel runs over that.
 //
 // Bound: the tensor cores, from about 64 queries on. Writing out costs 768 bytes
 // of traffic per position and KV head (256 read, 512 written) against 1024 flop
@@ -54,7 +54,8 @@ kv8_write_out_kernel(const Kv8View c, const int32_t *seq_ids, int len, uint16_t 
 #pragma unroll
             for (int j = 0; j < 2; j++) {
                 const float2 a = e4m3x2_to_f32x2(x[j] & 0xFFFFu), d = e4m3x2_to_f32x2(x[j] >> 16);
-                // exact products: their BF16 form is their upper half
+                // exact products: their BF16 form is their upper half (a scale below 2^-124 may
+                // leave bits under 2^-133, which are cut off)
                 o[2 * j] = __byte_perm(__float_as_uint(a.x * sc), __float_as_uint(a.y * sc), 0x7632);
                 o[2 * j + 1] = __byte_perm(__float_as_uint(d.x * sc), __float_as_uint(d.y * sc), 0x7632);
             }

@@ -162,3 +162,20 @@ def test_exact_mode_with_the_8_bit_cache_is_refused():
         cfg = n5.ModelConfig(1, 64, 16, mode, 16)
         assert n5.lib().n550_qwen3_init_random(C.byref(h), 0, 0.02, C.byref(cfg)) == want
         assert not h
+
+
+def test_values_are_bf16_numbers_for_scales_in_range():
+    """Every code times 2^-124 .. 2^119 (and neither 2^-125 nor 2^120) is a finite BF16 number."""
+    v = values(torch.arange(256).to(torch.uint8))
+    v = v[~v.isnan()]
+
+    def whole(e):
+        x = v * 2.0 ** e
+        return torch.equal(x.to(torch.float32).to(torch.bfloat16).double(), x)
+
+    assert all(whole(e) for e in range(-124, 120))
+    assert not whole(-125) and not whole(120)
+    # the smallest scale that append gives blocks at the statement's borders
+    assert scale_for(torch.tensor([448.0 * 2.0 ** -125], dtype=torch.float64)) == 2.0 ** -125
+    assert scale_for(torch.tensor([448.0 * 2.0 ** 119], dtype=torch.float64)) == 2.0 ** 119
+    assert scale_for(torch.tensor([448.5 * 2.0 ** 119], dtype=torch.float64)) == 2.0 ** 120

@@ -810,3 +810,23 @@ def test_prefill_wrapper_caps_its_workspace(monkeypatch):
         monkeypatch.setattr(n5.kv8, "PREFILL_WORKSPACE_MAX", cap)
         assert torch.equal(n5.attention_prefill_kv8(q, c, ids, 200, 200, 1), want)
         assert most.pop() == nbytes
+
+
+@pytest.mark.parametrize("e", [-124, -60, 0, 119])
+def test_attention_reads_values_at_the_ends_of_the_range(e):
+    """One position's V is what every code times 2^e is, to the bit, on both prefill
+    routes and in decode; the others' are zero, and so are the scores."""
+    n = 140
+    v0 = torch.arange(128, dtype=torch.uint8).view(torch.float8_e4m3fn).float().nan_to_num(nan=448.0)
+    v0[1::2] *= -1
+    v = torch.zeros((n, 8, 128))
+    v[0] = v0 * 2.0 ** e
+    c = fresh(1, n)
+    n5.kv8_append(c, torch.zeros((n, 1024), device="cuda"), v.view(n, 1024).cuda(), i32([0]), i32([0]), n, 1)
+    assert (c.v_scale[0, 1, :, 0] == 2.0 ** e).all()
+    q = rows(n, 2048, torch.bfloat16, 770).cuda()
+    want = v[0].to(torch.bfloat16)[:, None].expand(8, 2, 128)
+    for out in (n5.attention_decode_kv8(q[:1], c, i32([0]), i32([0]), 1), n5.attention_prefill_kv8(q[:5], c, i32([0]), 5, 0, 1),
+                n5.attention_prefill_kv8(q, c, i32([0]), n, 0, 1)):
+        assert torch.isfinite(out).all()
+        assert torch.equal(out[0].view(8, 2, 128).cpu().float(), want.float())
