@@ -86,12 +86,11 @@ def _ids(seq_ids, pos=None):
 _INT_MAX = 2 ** 31 - 1
 
 
-def _c_ints(**values):
+def _c_int(name, x):
     """Numbers that the library takes as C ints: ctypes would cut larger ones to their
     lower 32 bits."""
-    for name, x in values.items():
-        if not -_INT_MAX <= x <= _INT_MAX:
-            raise ValueError(f"{name} = {x} does not fit 32 bits")
+    if not -_INT_MAX <= x <= _INT_MAX:
+        raise ValueError(f"{name} = {x} does not fit 32 bits")
 
 
 def _rows(name, t, rows, cols, dtypes):
@@ -109,7 +108,8 @@ def kv8_append(cache, k, v, seq_ids, pos, L, layer):
     """Quantise len(seq_ids) x L rows of k and v ([n_seqs*L, >= 1024] float32 or
     bfloat16) into positions pos[s] .. pos[s]+L-1 of slot seq_ids[s]."""
     import torch
-    _c_ints(layer=layer, L=L)
+    _c_int("layer", layer)
+    _c_int("L", L)
     st = _stream(cache, k, v, seq_ids, pos)
     n = _ids(seq_ids, pos)
     if L < 0:
@@ -142,7 +142,7 @@ def attention_decode_kv8(q, cache, seq_ids, pos, layer, out=None, split=True):
     cache; split=True passes a split-KV workspace, split=False runs one CTA per
     (sequence, KV head)."""
     n = _ids(seq_ids, pos)
-    _c_ints(layer=layer)
+    _c_int("layer", layer)
     ldq, out, ldo = _q_out(q, n, out)
     st = _stream(cache, q, seq_ids, pos, out)
     L = lib()
@@ -163,7 +163,8 @@ def attention_sparse_kv8(q, cache, seq_ids, pos, blocks, layer, out=None, split=
     if blocks.dtype != torch.int32 or len(shape) != 3 or shape[0] != n or shape[1] != _NKV or \
             not blocks.is_contiguous():
         raise ValueError(f"blocks must be a contiguous int32 tensor [{n}, 8, n_select]")
-    _c_ints(layer=layer, n_select=shape[2])
+    _c_int("layer", layer)
+    _c_int("n_select", shape[2])
     ldq, out, ldo = _q_out(q, n, out)
     st = _stream(cache, q, seq_ids, pos, blocks, out)
     L = lib()
@@ -184,7 +185,9 @@ def attention_prefill_kv8(q, cache, seq_ids, L, pos0, layer, out=None, workspace
     """Causal attention of len(seq_ids) sequences x L queries (rows of q, BF16) at
     positions pos0.. over the 8-bit cache, which holds their K/V already."""
     n = _ids(seq_ids)
-    _c_ints(L=L, pos0=pos0, layer=layer)
+    _c_int("L", L)
+    _c_int("pos0", pos0)
+    _c_int("layer", layer)
     if L < 0:
         raise ValueError("L must not be negative")
     ldq, out, ldo = _q_out(q, n * L, out)
@@ -207,7 +210,10 @@ def kv8_select_blocks(q, cache, seq_ids, pos, layer, n_select, n_sink=1, n_recen
     -1 behind the last."""
     import torch
     n = _ids(seq_ids, pos)
-    _c_ints(layer=layer, n_select=n_select, n_sink=n_sink, n_recent=n_recent)
+    _c_int("layer", layer)
+    _c_int("n_select", n_select)
+    _c_int("n_sink", n_sink)
+    _c_int("n_recent", n_recent)
     ldq = _rows("q", q, n, _NH * _HD, (torch.bfloat16,))
     if out is None:
         out = torch.empty((n, _NKV, max(n_select, 0)), dtype=torch.int32, device=q.device)
