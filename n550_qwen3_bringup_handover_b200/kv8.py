@@ -27,7 +27,12 @@ class KV8Cache:
     positions and KV head (n550_kv8_cache). Tensors: k, v [n_slots, n_layers, 8,
     max_len, 128] float8_e4m3fn, k_scale, v_scale [n_slots, n_layers, 8, n_blocks]
     float32, k_bounds [n_slots, n_layers, 8, n_blocks, 2, 128] float8_e4m3fn or
-    None. Allocated here, or handed over by keyword."""
+    None. Allocated here, or handed over by keyword; the calls below read and write
+    these tensors' memory, so another tensor cannot take one's place."""
+
+    k, v = property(lambda c: c._tensors[0]), property(lambda c: c._tensors[1])
+    k_scale, v_scale = property(lambda c: c._tensors[2]), property(lambda c: c._tensors[3])
+    k_bounds = property(lambda c: c._tensors[4])
 
     def __init__(self, n_slots=None, max_len=None, n_layers=_LAYERS, device="cuda", bounds=True, *,
                  k=None, v=None, k_scale=None, v_scale=None, k_bounds=None):
@@ -62,7 +67,7 @@ class KV8Cache:
                 raise ValueError(f"{name} must be a contiguous {dt} tensor of shape {shape}")
             if t.device.type != "cuda" or t.device != k.device:
                 raise ValueError("the cache's tensors must be on one CUDA device")
-        self.k, self.v, self.k_scale, self.v_scale, self.k_bounds = k, v, k_scale, v_scale, k_bounds
+        self._tensors = (k, v, k_scale, v_scale, k_bounds)
         self.n_slots, self.n_layers, self.max_len, self.n_blocks = k.shape[0], k.shape[1], k.shape[3], nb
         self.device_index = k.get_device()
         self._c = KV8CacheStruct(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),

@@ -830,3 +830,17 @@ def test_attention_reads_values_at_the_ends_of_the_range(e):
                 n5.attention_prefill_kv8(q, c, i32([0]), n, 0, 1)):
         assert torch.isfinite(out).all()
         assert torch.equal(out[0].view(8, 2, 128).cpu().float(), want.float())
+
+
+def test_the_tensors_of_a_cache_stay_its_tensors():
+    """The library holds their addresses: an assignment would leave the calls with the old
+    tensor's memory, freed or not."""
+    c = n5.KV8Cache(1, 64, n_layers=1)
+    for name in ("k", "v", "k_scale", "v_scale", "k_bounds"):
+        t = getattr(c, name)
+        with pytest.raises(AttributeError):
+            setattr(c, name, t.clone())
+        assert getattr(c, name) is t
+    assert (c._c.k, c._c.v, c._c.k_scale, c._c.v_scale, c._c.k_bounds) == tuple(
+        t.data_ptr() for t in (c.k, c.v, c.k_scale, c.v_scale, c.k_bounds))
+    assert n5.KV8Cache(1, 64, n_layers=1, bounds=False).k_bounds is None
