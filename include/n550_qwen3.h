@@ -320,7 +320,9 @@ int n550_kv8_append(void *stream, const n550_kv8_cache *c, int layer, const void
  * workspace may be NULL (one CTA per sequence and KV head) or
  * n550_attention_kv8_workspace(n_seqs) bytes, 16-byte aligned, not shared by calls
  * that can overlap; its contents before and after a call mean nothing (a
- * smaller or unaligned one counts as NULL). */
+ * smaller or unaligned one counts as NULL). Query elements below 2^-13 of their
+ * head's largest are taken as multiples of 2^-20 of it; softmax weights have 11 bits (small
+ * ones are multiples of 2^-25 of the largest near them), sums are FP32. */
 int n550_attention_decode_kv8(void *stream, const uint16_t *q, int ldq, const n550_kv8_cache *c,
                               int layer, const int32_t *seq_ids, const int32_t *pos, int n_seqs,
                               uint16_t *out, int ldo, void *workspace, size_t workspace_bytes);
@@ -329,7 +331,8 @@ size_t n550_attention_kv8_workspace(int n_seqs);
 /* n550_attention_prefill over the 8-bit cache: n_seqs x L queries at positions
  * pos0 .. pos0+L-1 whose K/V were appended, causal; q and out [n_seqs*L] rows.
  * As in the BF16 prefill, a NaN in the V of one of these L positions also reaches
- * that dimension of the queries before it. workspace may be NULL (slower) or
+ * that dimension of the queries before it. Up to 8 queries are rounded as in the decode;
+ * where the workspace holds contexts as BF16 the softmax weights are BF16 too. workspace may be NULL (slower) or
  * n550_attention_prefill_kv8_workspace(n_seqs, L, pos0) bytes, as above. Up to 8
  * queries (and more, where few sequences have long contexts) stream the codes in
  * passes of 8; otherwise the workspace holds the context as BF16, 4096 bytes
@@ -482,7 +485,11 @@ int n550_qwen3_fused_decode(int on);
  * return N550_ERR_OOM until a call of this function succeeds. The q/k/v step
  * then appends its K/V rows (after QK-norm and RoPE) itself in a decode step and leaves
  * them to n550_kv8_append otherwise, and the attention runs as
- * n550_attention_decode_kv8 / n550_attention_prefill_kv8. Fast mode only
+ * n550_attention_decode_kv8 / n550_attention_prefill_kv8. Logits differ from the BF16 cache's
+ * by what 4-bit significands of K and V cost (5 % in the mean square with random
+ * weights), and so may the greedy choice; with drafts (n550_qwen3_generate_lookup) the ids may
+ * also part from those without, for rows verified together are rounded together and
+ * a rejected draft can raise its block's scale. Fast mode only
  * (N550_ERR_UNSUPPORTED otherwise, and for a forward with the tensor dump on).
  * n550_qwen3_kv8_cache gives the cache of such a model (28 layers, max_seqs slots)
  * for calls of the entry points above, N550_ERR_ARG without one. No counterpart

@@ -18,8 +18,8 @@
 // 390 instructions per warp and 16 positions and stopped at 4.7 TB/s (256
 // sequences x 1152 positions, 114 us; now 103, 5.2 TB/s). The 16-column side has room for
 // queries and weights in e4m3 parts, four bits a part:
-//   q = 2^a (h + l / 16): two parts hold a BF16 value whole, down to 2^-21 of the
-//       row's largest;
+//   q = 2^a (h + l / 16): two parts hold a BF16 value whole if it is at least 2^-13 of
+//       its head's largest, and a smaller one as a multiple of 2^-20 of that at worst;
 //   w = 2^-8 (w1 + w2 / 16 + w3 / 256): a softmax weight is rounded to FP16's 11 bits
 //       (2^-12 of it at most), which three parts hold whole, or as a multiple of
 //       2^-25 of the tile's largest where it is small.
