@@ -350,7 +350,8 @@ size_t n550_attention_prefill_kv8_workspace(int n_seqs, int L, int pos0);
  * which no q . k_t of the block exceeds. The first n_sink and the last n_recent
  * blocks of the context are always among them (n_sink + n_recent <= n_select;
  * the block of position pos[s] is the last one); then the largest scores, the
- * lower index first among equals (a NaN score ranks last). blocks
+ * lower index first among equals (a head whose sum is NaN does not count; a block
+ * without one that does ranks last). blocks
  * [n_seqs][8][n_select] int32 receives the indices in ascending order and -1
  * behind them when the context has fewer blocks. Caches of more than
  * N550_KV8_SELECT_MAX_BLOCKS blocks: N550_ERR_UNSUPPORTED. */

@@ -844,3 +844,17 @@ def test_the_tensors_of_a_cache_stay_its_tensors():
     assert (c._c.k, c._c.v, c._c.k_scale, c._c.v_scale, c._c.k_bounds) == tuple(
         t.data_ptr() for t in (c.k, c.v, c.k_scale, c.v_scale, c.k_bounds))
     assert n5.KV8Cache(1, 64, n_layers=1, bounds=False).k_bounds is None
+
+
+@pytest.mark.parametrize("strange", [float("nan"), float("inf"), -float("inf")])
+def test_select_with_one_strange_head(strange):
+    """A NaN in one of a KV head's two query heads leaves the other's order; an infinity
+    puts every block with that sign of K in the channel first (lower index among equals)."""
+    c, ref = filled(2, 1000, 780)
+    q = rows(3, 2048, torch.bfloat16, 781)
+    q[0, 5 * 128 + 7] = strange
+    q[2, 12 * 128] = strange
+    ids, pos = [1, 0, 1], [999, 700, 640]
+    for n_select, sink, recent in [(4, 1, 1), (7, 0, 0)]:
+        got = n5.kv8_select_blocks(q.cuda(), c, i32(ids), i32(pos), 1, n_select, sink, recent)
+        assert torch.equal(got.cpu(), ref.select(q, ids, pos, n_select, sink, recent))
